@@ -12,6 +12,11 @@ Beyond the reference:
   causal_conv1d_fwd_states  prefill with the Dao-AILab extras (seq_idx, initial_states, final
                             states), which dao_compat serves instead of passing them upstream
   CausalConv1d              layer object
+  gated_delta_rule_varlen_fn, gated_delta_rule_fn, gated_delta_rule_update
+                            the recurrence behind the conv of a Gated DeltaNet layer: packed and
+                            dense prefill, decode and speculative verify
+  rms_norm_gated            the gated norm behind the recurrence
+  StateSlots                copies, forks, clears and compacts the slots of state caches
 
 Every entry point runs hand-written CUDA kernels from libcc1d.so (C ABI: include/cc1d.h). There is
 no CPU fallback: calls the kernels cannot serve raise functional.Unsupported.
@@ -30,10 +35,18 @@ from .functional import (
     causal_conv1d_varlen_fn,
     supported,
 )
+from .gated_delta import (
+    gated_delta_rule_fn,
+    gated_delta_rule_update,
+    gated_delta_rule_varlen_fn,
+    rms_norm_gated,
+)
 from .ring import from_ring, to_ring
+from .slots import StateSlots
 
 __all__ = [
     "CausalConv1d",
+    "StateSlots",
     "Unsupported",
     "causal_conv1d_fn",
     "causal_conv1d_fwd_states",
@@ -42,6 +55,10 @@ __all__ = [
     "causal_conv1d_varlen_fn",
     "device_status",
     "from_ring",
+    "gated_delta_rule_fn",
+    "gated_delta_rule_update",
+    "gated_delta_rule_varlen_fn",
+    "rms_norm_gated",
     "set_device_checks",
     "supported",
     "to_ring",

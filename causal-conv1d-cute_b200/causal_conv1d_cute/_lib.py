@@ -6,6 +6,7 @@ There is no fallback: if it is missing or does not load, every entry point raise
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 import torch
@@ -15,7 +16,7 @@ LIB_PATH = Path(os.environ.get("CC1D_LIBRARY", Path(__file__).with_name("libcc1d
 BF16, F16, F32 = 0, 1, 2
 DTYPE_CODES = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32}
 
-DEV_BAD_SLOT, DEV_BAD_QSL, DEV_BAD_INTER_SLOT = 1, 2, 4
+DEV_BAD_SLOT, DEV_BAD_QSL, DEV_BAD_INTER_SLOT, DEV_TIMEOUT = 1, 2, 4, 8
 
 _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -39,8 +40,18 @@ SIGNATURES = {
                     _p, _p, _p, _i64, _i64, _i64, _i64, _i32, _i64, _i32, _i32, _i32, _p, _p],
     "cc1d_update_unpack": [_p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _i32,
                            _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _p],
+    "cc1d_gdr_update": [_p, _p],
+    "cc1d_gdr_varlen": [_p, _p],
+    "cc1d_rms_norm_gated": [_p, _p],
+    "cc1d_slots_copy": [_p, _i32, _p, _p, _i64, _i64, _i64, _i32, _p, _p],
+    "cc1d_slots_compact": [_p, _i32, _p, _i64, _p, _p, _p, _p],
     "cc1d_copy": [_p, _p, _i64, _p],
 }
+
+# Argument blocks (cc1d_gdr_args, cc1d_norm_args) are packed by struct in one call, which costs the
+# host less than setting the fields of a ctypes structure: pointers, then int64, int32 and float.
+GDR_ARGS = struct.Struct("15P33q13if")
+NORM_ARGS = struct.Struct("4P9q2if4x")
 
 EXPORTS = ("cc1d_abi_version", "cc1d_status_string", "cc1d_last_error", *SIGNATURES)
 

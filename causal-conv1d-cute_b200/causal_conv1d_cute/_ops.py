@@ -1,6 +1,7 @@
 """Tensor-level calls into libcc1d.so, registered as torch.library ops (cc1d::fwd, cc1d::update,
 cc1d::update_ring, cc1d::varlen, cc1d::update_unpack, cc1d::fwd_states, cc1d::to_ring,
-cc1d::from_ring).
+cc1d::from_ring, cc1d::gdr_update, cc1d::gdr_varlen, cc1d::rms_norm_gated, cc1d::slots_copy,
+cc1d::slots_compact).
 
 Each op passes data pointers, element strides and sizes of already-validated CUDA tensors to
 one C entry point, on the current stream of the tensors' device. No host synchronisation, no
@@ -16,7 +17,7 @@ clears it. Checks are off by default so that no call allocates anything.
 import torch
 
 from . import _lib
-from ._lib import check, dtype_code, load
+from ._lib import F32, GDR_ARGS, NORM_ARGS, check, dtype_code, load
 
 _checks = False
 _status = {}
@@ -215,6 +216,77 @@ def _update_unpack_impl(qkvz, ba, state, weight, bias, out, z, b, a, idx, heads,
     return out, z, b, a
 
 
+def _gdr_args(q, k, v, g, beta, a_log, dt_bias, out, states, inter, idx, iidx, qsl, hinit, rows,
+              tokens, steps, scale, l2norm, update, pad):
+    """The packed cc1d_gdr_args; the token-major tensors are (rows, steps, ...) or (tokens, ...)."""
+    zero = (0,) if q.dim() == 3 else ()
+    ss, nslots = ((0, 0, 0), 0) if states is None else (states.stride()[:3], states.shape[0])
+    si, ni = ((0, 0, 0, 0), 0) if inter is None else (inter.stride()[:4], inter.shape[0])
+    return GDR_ARGS.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(),
+        0 if a_log is None else a_log.data_ptr(), 0 if dt_bias is None else dt_bias.data_ptr(),
+        out.data_ptr(), 0 if states is None else states.data_ptr(),
+        0 if inter is None else inter.data_ptr(),
+        0 if idx is None else idx.data_ptr(), 0 if iidx is None else iidx.data_ptr(),
+        0 if qsl is None else qsl.data_ptr(), 0 if hinit is None else hinit.data_ptr(),
+        _status_ptr(q.device) or 0,
+        *zero, *q.stride(), *zero, *k.stride(), *zero, *v.stride(), *zero, *out.stride(),
+        *zero, *g.stride(), *zero, *beta.stride(), *ss, *si,
+        rows, tokens, nslots, ni,
+        steps, q.shape[-2], v.shape[-2], q.shape[-1], v.shape[-1],
+        dtype_code(q.dtype), dtype_code(g.dtype), dtype_code(beta.dtype),
+        F32 if a_log is None else dtype_code(a_log.dtype),
+        F32 if states is None else dtype_code(states.dtype),
+        int(l2norm), int(update), pad, scale,
+    )
+
+
+def _gdr_update_impl(q, k, v, g, beta, a_log, dt_bias, out, states, idx, inter, iidx, scale,
+                     l2norm, update, pad):
+    """Gated delta rule decode (cc1d_gdr_update): (rows, steps, heads, dim), or (rows, heads, dim)
+    for one step."""
+    if q.dim() == 3:
+        q, k, v, g, beta, out = (t.unsqueeze(1) for t in (q, k, v, g, beta, out))
+    args = _gdr_args(q, k, v, g, beta, a_log, dt_bias, out, states, inter, idx, iidx, None, None,
+                     q.shape[0], 0, q.shape[1], scale, l2norm, update, pad)
+    check(load().cc1d_gdr_update(args, _stream(q.device)))
+
+
+def _gdr_varlen_impl(q, k, v, g, beta, a_log, dt_bias, out, states, qsl, idx, hinit, scale,
+                     l2norm, pad):
+    """Gated delta rule over packed sequences (cc1d_gdr_varlen): (tokens, heads, dim)."""
+    args = _gdr_args(q, k, v, g, beta, a_log, dt_bias, out, states, None, idx, None, qsl, hinit,
+                     qsl.numel() - 1, q.shape[0], 0, scale, l2norm, True, pad)
+    check(load().cc1d_gdr_varlen(args, _stream(q.device)))
+
+
+def _rms_norm_gated_impl(x, z, weight, eps, out):
+    """Gated RMS norm of (n0, n1, dim) rows (cc1d_rms_norm_gated)."""
+    args = NORM_ARGS.pack(
+        x.data_ptr(), 0 if z is None else z.data_ptr(), weight.data_ptr(), out.data_ptr(),
+        x.stride(0), x.stride(1), *((0, 0) if z is None else z.stride()[:2]),
+        out.stride(0), out.stride(1), *x.shape,
+        dtype_code(x.dtype), dtype_code(weight.dtype), eps,
+    )
+    check(load().cc1d_rms_norm_gated(args, _stream(x.device)))
+
+
+def _slots_copy_impl(caches, sources, table, ncaches, src, dst, src_slots, dst_slots, pad):
+    """Slot copies between caches (cc1d_slots_copy); table is the address of a cc1d_slot_cache
+    array that describes caches (and sources, where they are not the caches themselves)."""
+    dev = caches[0].device
+    check(load().cc1d_slots_copy(table, ncaches, src.data_ptr(), dst.data_ptr(), src.numel(),
+                                 src_slots, dst_slots, pad, _status_ptr(dev), _stream(dev)))
+
+
+def _slots_compact_impl(caches, table, ncaches, live, remap, count, moves):
+    """Live slots to the front of the caches (cc1d_slots_compact)."""
+    dev = live.device
+    check(load().cc1d_slots_compact(table or None, ncaches, live.data_ptr(), live.numel(),
+                                    remap.data_ptr(), count.data_ptr(), moves.data_ptr(),
+                                    _stream(dev)))
+
+
 # ---------------------------------------------------------------------------------------------
 # torch.library registration: the entry points as dispatcher ops cc1d::<name>, with the mutated
 # arguments (outputs and caches) marked in the schemas and fake implementations for meta/fake
@@ -248,12 +320,36 @@ _SCHEMAS = {
         "Tensor(b!) out, Tensor(c!) z, Tensor(d!) b, Tensor(e!) a, Tensor idx, int heads, "
         "bool silu, int pad) -> ()"
     ),
+    "gdr_update": (
+        "gdr_update(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor? a_log, "
+        "Tensor? dt_bias, Tensor(a!) out, Tensor(b!) states, Tensor? idx, Tensor(c!)? inter, "
+        "Tensor? iidx, float scale, bool l2norm, bool update, int pad) -> ()"
+    ),
+    "gdr_varlen": (
+        "gdr_varlen(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor? a_log, "
+        "Tensor? dt_bias, Tensor(a!) out, Tensor(b!)? states, Tensor qsl, Tensor? idx, "
+        "Tensor? hinit, float scale, bool l2norm, int pad) -> ()"
+    ),
+    "rms_norm_gated": (
+        "rms_norm_gated(Tensor x, Tensor? z, Tensor weight, float eps, Tensor(a!) out) -> ()"
+    ),
+    "slots_copy": (
+        "slots_copy(Tensor(a!)[] caches, Tensor[] sources, int table, int ncaches, Tensor src, "
+        "Tensor dst, int src_slots, int dst_slots, int pad) -> ()"
+    ),
+    "slots_compact": (
+        "slots_compact(Tensor(a!)[] caches, int table, int ncaches, Tensor live, "
+        "Tensor(b!) remap, Tensor(c!) count, Tensor(d!) moves) -> ()"
+    ),
 }
 _IMPLS = {
     "fwd": _fwd_impl, "fwd_states": _fwd_states_impl, "update": _update_impl,
     "update_ring": _update_ring_impl, "to_ring": _to_ring_impl, "from_ring": _from_ring_impl,
     "varlen": _varlen_impl,
     "update_unpack": _update_unpack_impl,
+    "gdr_update": _gdr_update_impl, "gdr_varlen": _gdr_varlen_impl,
+    "rms_norm_gated": _rms_norm_gated_impl,
+    "slots_copy": _slots_copy_impl, "slots_compact": _slots_compact_impl,
 }
 
 
@@ -333,7 +429,14 @@ def update_unpack(qkvz, ba, state, weight, bias, out, z, b, a, idx, heads, silu,
     return out, z, b, a
 
 
+gdr_update = _op.gdr_update  # gated delta rule decode into `out`, in place on the states
+gdr_varlen = _op.gdr_varlen  # gated delta rule over packed sequences
+rms_norm_gated = _op.rms_norm_gated
+slots_copy = _op.slots_copy
+slots_compact = _op.slots_compact
+
 __all__ = [
-    "device_status", "from_ring", "fwd", "fwd_states", "to_ring", "set_device_checks", "update", "update_ring", "update_unpack",
-    "varlen", "_lib",
+    "device_status", "from_ring", "fwd", "fwd_states", "gdr_update", "gdr_varlen", "rms_norm_gated",
+    "slots_compact", "slots_copy", "to_ring", "set_device_checks", "update", "update_ring",
+    "update_unpack", "varlen", "_lib",
 ]

@@ -64,6 +64,38 @@ int64_t span_bytes(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t n2, i
     return ((n0 - 1) * s0 + (n1 - 1) * s1 + (n2 - 1) * s2 + 1) * esize;
 }
 
+bool known_dtype(int32_t d) { return d == CC1D_BF16 || d == CC1D_F16 || d == CC1D_F32; }
+
+// The checks that both gated delta rule entry points share.
+cc1d_status_t check_gdr(const cc1d_gdr_args& a) {
+    if (!known_dtype(a.dtype) || !known_dtype(a.gdtype) || !known_dtype(a.bdtype) ||
+        !known_dtype(a.pdtype))
+        return fail(CC1D_ERR_DTYPE, "dtypes %d, %d, %d, %d are not bf16 (0), fp16 (1) or fp32 (2)",
+                    a.dtype, a.gdtype, a.bdtype, a.pdtype);
+    if (a.sdtype != CC1D_F32 && a.sdtype != a.dtype)
+        return fail(CC1D_ERR_DTYPE, "state dtype %d is neither fp32 nor the input dtype", a.sdtype);
+    if (a.rows < 0 || a.tokens < 0 || a.heads_k < 1 || a.heads_v < 1 || a.nslots < 0 ||
+        a.heads_v % a.heads_k)
+        return fail(CC1D_ERR_INVALID, "%lld rows, %lld tokens, %d query/key and %d value heads",
+                    (long long)a.rows, (long long)a.tokens, a.heads_k, a.heads_v);
+    if (a.dk < 1 || a.dk > 256 || a.dv < 1)
+        return fail(CC1D_ERR_INVALID, "head dims %d and %d (dk is 1..256)", a.dk, a.dv);
+    if ((a.a_log == nullptr) != (a.dt_bias == nullptr))
+        return fail(CC1D_ERR_INVALID, "a_log and dt_bias come together");
+    return CC1D_OK;
+}
+
+cc1d_status_t check_slots(const cc1d_slot_cache* table, int32_t ncaches) {
+    if (ncaches < 0 || ncaches > CC1D_MAX_CACHES)
+        return fail(CC1D_ERR_INVALID, "%d caches (at most %d a call)", ncaches, CC1D_MAX_CACHES);
+    if (ncaches > 0 && table == nullptr) return fail(CC1D_ERR_INVALID, "table is NULL");
+    for (int32_t i = 0; i < ncaches; ++i)
+        if (table[i].dst == nullptr || table[i].src == nullptr || table[i].row_bytes < 0 ||
+            table[i].dst_stride < table[i].row_bytes || table[i].src_stride < table[i].row_bytes)
+            return fail(CC1D_ERR_INVALID, "cache %d has a NULL pointer or overlapping slots", i);
+    return CC1D_OK;
+}
+
 bool overlap(const void* p, int64_t np, const void* q, int64_t nq) {
     const char* a = (const char*)p;
     const char* b = (const char*)q;
@@ -318,6 +350,99 @@ cc1d_status_t cc1d_update_unpack(const void* qkvz, int64_t q_sb, const void* ba,
     if (cc1d_status_t s = bind_stream(stream)) return s;
     return from_cuda(cc1d::launch_unpack(args, width, dtype, (cudaStream_t)stream),
                      "cc1d_update_unpack");
+}
+
+cc1d_status_t cc1d_gdr_update(const cc1d_gdr_args* args, void* stream) {
+    if (args == nullptr) return fail(CC1D_ERR_INVALID, "args is NULL");
+    const cc1d_gdr_args& a = *args;
+    if (cc1d_status_t s = check_gdr(a)) return s;
+    if (a.steps < 1) return fail(CC1D_ERR_INVALID, "%d steps", a.steps);
+    if (a.rows == 0) return ok();
+    if (!a.q || !a.k || !a.v || !a.g || !a.beta || !a.out || !a.states)
+        return fail(CC1D_ERR_INVALID, "a required pointer is NULL");
+    if (a.indices == nullptr && a.nslots < a.rows)
+        return fail(CC1D_ERR_INVALID, "%lld slots for %lld rows without indices",
+                    (long long)a.nslots, (long long)a.rows);
+    if (cc1d_status_t s = bind_stream(stream)) return s;
+    return from_cuda(cc1d::launch_gdr_recurrent(a, false, (cudaStream_t)stream), "cc1d_gdr_update");
+}
+
+cc1d_status_t cc1d_gdr_varlen(const cc1d_gdr_args* args, void* stream) {
+    if (args == nullptr) return fail(CC1D_ERR_INVALID, "args is NULL");
+    const cc1d_gdr_args& a = *args;
+    if (cc1d_status_t s = check_gdr(a)) return s;
+    if (a.tokens > INT32_MAX) return fail(CC1D_ERR_INVALID, "more than 2^31 - 1 tokens");
+    if (a.inter != nullptr) return fail(CC1D_ERR_INVALID, "packed prefill records no step states");
+    if (a.rows == 0 || a.tokens == 0) return ok();
+    if (!a.q || !a.k || !a.v || !a.g || !a.beta || !a.out || !a.query_start_loc)
+        return fail(CC1D_ERR_INVALID, "a required pointer is NULL");
+    if (a.states != nullptr && a.indices == nullptr && a.nslots < a.rows)
+        return fail(CC1D_ERR_INVALID, "%lld slots for %lld sequences without indices",
+                    (long long)a.nslots, (long long)a.rows);
+    if (cc1d_status_t s = bind_stream(stream)) return s;
+    return from_cuda(cc1d::launch_gdr_recurrent(a, true, (cudaStream_t)stream), "cc1d_gdr_varlen");
+}
+
+cc1d_status_t cc1d_rms_norm_gated(const cc1d_norm_args* args, void* stream) {
+    if (args == nullptr) return fail(CC1D_ERR_INVALID, "args is NULL");
+    const cc1d_norm_args& a = *args;
+    if (!known_dtype(a.dtype)) return fail(CC1D_ERR_DTYPE, "dtype %d is not bf16, fp16 or fp32", a.dtype);
+    if (a.wdtype != CC1D_F32 && a.wdtype != a.dtype)
+        return fail(CC1D_ERR_DTYPE, "weight dtype %d is neither fp32 nor the input dtype", a.wdtype);
+    if (a.n0 < 0 || a.n1 < 0 || a.dim < 1)
+        return fail(CC1D_ERR_INVALID, "shape (%lld, %lld, %lld)", (long long)a.n0, (long long)a.n1,
+                    (long long)a.dim);
+    if (a.n0 == 0 || a.n1 == 0) return ok();
+    if (!a.x || !a.weight || !a.out) return fail(CC1D_ERR_INVALID, "a required pointer is NULL");
+    if (cc1d_status_t s = bind_stream(stream)) return s;
+    return from_cuda(cc1d::launch_norm(a, (cudaStream_t)stream), "cc1d_rms_norm_gated");
+}
+
+cc1d_status_t cc1d_slots_copy(const cc1d_slot_cache* table, int32_t ncaches,
+                              const int32_t* src_indices, const int32_t* dst_indices,
+                              int64_t npairs, int64_t src_nslots, int64_t dst_nslots,
+                              int32_t pad, int32_t* dev_status, void* stream) {
+    if (cc1d_status_t s = check_slots(table, ncaches)) return s;
+    if (npairs < 0 || npairs > INT32_MAX || src_nslots < 0 || dst_nslots < 0 ||
+        src_nslots > INT32_MAX || dst_nslots > INT32_MAX)
+        return fail(CC1D_ERR_INVALID, "%lld pairs, %lld and %lld slots", (long long)npairs,
+                    (long long)src_nslots, (long long)dst_nslots);
+    if (npairs == 0 || ncaches == 0) return ok();
+    if (!src_indices || !dst_indices) return fail(CC1D_ERR_INVALID, "an index list is NULL");
+    // A source group either is the destination group or lies apart from it.
+    int32_t same = 0;
+    for (int32_t i = 0; i < ncaches; ++i) {
+        if (table[i].src == table[i].dst && table[i].src_stride == table[i].dst_stride) {
+            ++same;
+        } else if (overlap(table[i].dst, dst_nslots * table[i].dst_stride, table[i].src,
+                           src_nslots * table[i].src_stride)) {
+            return fail(CC1D_ERR_INVALID, "source and destination of cache %d overlap", i);
+        }
+    }
+    if (same != 0 && (same != ncaches || src_nslots != dst_nslots))
+        return fail(CC1D_ERR_INVALID, "%d of %d caches are their own source", same, ncaches);
+    if (cc1d_status_t s = bind_stream(stream)) return s;
+    return from_cuda(cc1d::launch_slots_copy(table, ncaches, src_indices, dst_indices, npairs,
+                                             src_nslots, dst_nslots, same != 0, pad, dev_status,
+                                             (cudaStream_t)stream),
+                     "cc1d_slots_copy");
+}
+
+cc1d_status_t cc1d_slots_compact(const cc1d_slot_cache* table, int32_t ncaches,
+                                 const uint8_t* live, int64_t nslots, int32_t* remap,
+                                 int32_t* count, int32_t* moves, void* stream) {
+    if (cc1d_status_t s = check_slots(table, ncaches)) return s;
+    if (nslots < 0 || nslots > INT32_MAX / 2 - 1)
+        return fail(CC1D_ERR_INVALID, "%lld slots", (long long)nslots);
+    if (!count || !moves || (nslots > 0 && (!live || !remap)))
+        return fail(CC1D_ERR_INVALID, "a required pointer is NULL");
+    for (int32_t i = 0; i < ncaches; ++i)
+        if (table[i].src != table[i].dst || table[i].src_stride != table[i].dst_stride)
+            return fail(CC1D_ERR_INVALID, "compaction works within a cache (cache %d)", i);
+    if (cc1d_status_t s = bind_stream(stream)) return s;
+    return from_cuda(cc1d::launch_slots_compact(table, ncaches, live, nslots, remap, count, moves,
+                                                (cudaStream_t)stream),
+                     "cc1d_slots_compact");
 }
 
 cc1d_status_t cc1d_copy(void* dst, const void* src, int64_t bytes, void* stream) {

@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "../../include/cc1d.h"
+
 namespace cc1d {
 
 struct FwdArgs {
@@ -135,6 +137,16 @@ cudaError_t launch_ring(const RingArgs& a, int width, int dtype, cudaStream_t st
 cudaError_t launch_ring_convert(const RingConvArgs& a, int width, int dtype, cudaStream_t stream);
 cudaError_t launch_varlen(const VarArgs& a, int width, int dtype, cudaStream_t stream);
 cudaError_t launch_unpack(const UnpackArgs& a, int width, int dtype, cudaStream_t stream);
+cudaError_t launch_gdr_recurrent(const cc1d_gdr_args& a, bool varlen, cudaStream_t stream);
+cudaError_t launch_norm(const cc1d_norm_args& a, cudaStream_t stream);
+// same: the table's src and dst are the same caches (a source may be an earlier destination).
+cudaError_t launch_slots_copy(const cc1d_slot_cache* table, int ncaches, const int32_t* src,
+                              const int32_t* dst, int64_t npairs, int64_t src_nslots,
+                              int64_t dst_nslots, bool same, int pad, int32_t* status,
+                              cudaStream_t stream);
+cudaError_t launch_slots_compact(const cc1d_slot_cache* table, int ncaches, const uint8_t* live,
+                                 int64_t nslots, int32_t* remap, int32_t* count, int32_t* moves,
+                                 cudaStream_t stream);
 cudaError_t launch_copy(void* dst, const void* src, int64_t bytes, cudaStream_t stream);
 
 }  // namespace cc1d

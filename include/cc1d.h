@@ -47,7 +47,8 @@ enum { CC1D_BF16 = 0, CC1D_F16 = 1, CC1D_F32 = 2 };
 enum {
     CC1D_DEV_BAD_SLOT = 1,       /* a conv-state / ring slot outside [0, nslots) and != pad */
     CC1D_DEV_BAD_QSL = 2,        /* query_start_loc outside [0, ntokens] or decreasing */
-    CC1D_DEV_BAD_INTER_SLOT = 4  /* a per-step state slot outside [0, inter_nslots) */
+    CC1D_DEV_BAD_INTER_SLOT = 4, /* a per-step state slot outside [0, inter_nslots) */
+    CC1D_DEV_TIMEOUT = 8         /* a wait inside a kernel ran out; that call's results are invalid */
 };
 
 /* ABI revision; bumped on any signature change. */
@@ -215,6 +216,95 @@ cc1d_status_t cc1d_update_unpack(const void* qkvz, int64_t q_sb, const void* ba,
  * prefill's bytes timed beside every prefill kernel, benchmarks/BASELINES.md:44).
  */
 cc1d_status_t cc1d_copy(void* dst, const void* src, int64_t bytes, void* stream);
+
+/*
+ * Gated delta rule, the recurrence of a Gated DeltaNet layer. Value head h has a (dk, dv) state S
+ * and uses query/key head h / (heads_v / heads_k). For each token, in fp32:
+ *     S <- exp(g) S;   u = beta (v - S^T k);   S <- S + k u^T;   o = scale S^T q.
+ * With a_log, g and beta are raw projections: the log decay is -exp(a_log[h]) softplus(g +
+ * dt_bias[h]) and the rate is sigmoid(beta). With l2norm, q and k are first scaled by
+ * rsqrt(sum of squares + 1e-6). Log decays are expected to be <= 0; -inf clears the state.
+ *
+ * One argument block serves both entry points.
+ *   cc1d_gdr_update: `rows` batch rows of `steps` tokens each; row b, token t of q lies at
+ *     q + b*q_sb + t*q_st + head*q_sh + i*q_sd (k, v, out alike; gates: *_sb, *_st, *_sh).
+ *     Row b advances slot indices[b] (b when NULL); rows whose slot is `pad` are skipped and
+ *     their outputs left unwritten. When inter is not NULL the state after token t is written to
+ *     inter[inter_indices[b] (default: the row's slot), t]; update_states == 0 leaves the cache
+ *     itself unchanged.
+ *   cc1d_gdr_varlen: `rows` sequences packed along the token axis, sequence n spanning tokens
+ *     [query_start_loc[n], query_start_loc[n+1]) of `tokens` (the *_sb are not used). It starts
+ *     from states[indices[n]] if has_initial_state[n] != 0 and from zeros otherwise, and that slot
+ *     receives its final state; sequences of zero tokens and of slot `pad` leave the cache
+ *     untouched (those of slot `pad` leave their outputs unwritten). states may be NULL.
+ * states is (nslots, heads_v, dk, dv) of sdtype with unit stride along dv. Live slots must be
+ * distinct. dk is 1..256; sdtype is fp32 or `dtype`.
+ */
+typedef struct {
+    const void *q, *k, *v, *g, *beta, *a_log, *dt_bias;
+    void *out, *states, *inter;
+    const int32_t *indices, *inter_indices, *query_start_loc;
+    const uint8_t* has_initial_state;
+    int32_t* dev_status;
+    int64_t q_sb, q_st, q_sh, q_sd, k_sb, k_st, k_sh, k_sd, v_sb, v_st, v_sh, v_sd;
+    int64_t o_sb, o_st, o_sh, o_sd, g_sb, g_st, g_sh, b_sb, b_st, b_sh;
+    int64_t s_slot, s_sh, s_sk, i_slot, i_st, i_sh, i_sk;
+    int64_t rows, tokens, nslots, inter_nslots;
+    int32_t steps, heads_k, heads_v, dk, dv;
+    int32_t dtype, gdtype, bdtype, pdtype, sdtype; /* q k v out | g | beta | a_log dt_bias | states */
+    int32_t l2norm, update_states, pad;
+    float scale;
+} cc1d_gdr_args;
+
+cc1d_status_t cc1d_gdr_update(const cc1d_gdr_args* args, void* stream);
+cc1d_status_t cc1d_gdr_varlen(const cc1d_gdr_args* args, void* stream);
+
+/*
+ * Gated RMS norm over the last axis of (n0, n1, dim) rows: out = x rsqrt(mean(x^2) + eps) weight
+ * silu(z), statistics and products in fp32. weight (dim,) of wdtype, contiguous; z may be NULL (no
+ * gate). Unit stride along dim; strides are elements.
+ */
+typedef struct {
+    const void *x, *z, *weight;
+    void* out;
+    int64_t x_s0, x_s1, z_s0, z_s1, o_s0, o_s1;
+    int64_t n0, n1, dim;
+    int32_t dtype, wdtype;
+    float eps;
+} cc1d_norm_args;
+
+cc1d_status_t cc1d_rms_norm_gated(const cc1d_norm_args* args, void* stream);
+
+/*
+ * Slot moves between state caches. A table describes the caches of a group: slot s of cache c
+ * is row_bytes bytes at dst + s*dst_stride (src alike, in bytes).
+ *
+ * cc1d_slots_copy: for pairs i = 0..npairs-1, in that order: slot dst_indices[i] of every cache
+ * becomes a copy of slot src_indices[i] of src; a source equal to `pad` clears the slot, a
+ * destination equal to `pad` skips the pair, and a pair with another index outside the caches is
+ * skipped and reported. src may equal dst (forks within a cache) or be another group.
+ *
+ * cc1d_slots_compact: live (nslots bytes, != 0: in use). With m live slots, the i-th free slot
+ * below m receives the i-th live slot at or above m (ascending), which is the fewest moves that
+ * make slots 0..m-1 the live ones. remap[s] is the new place of slot s (-1: not live), *count is
+ * m. moves is a workspace of 2*nslots + 1 int32.
+ *
+ * At most CC1D_MAX_CACHES caches a call, nslots up to 2^31 - 1.
+ */
+#define CC1D_MAX_CACHES 64
+typedef struct {
+    void* dst;
+    const void* src;
+    int64_t dst_stride, src_stride, row_bytes;
+} cc1d_slot_cache;
+
+cc1d_status_t cc1d_slots_copy(const cc1d_slot_cache* table, int32_t ncaches,
+                              const int32_t* src_indices, const int32_t* dst_indices,
+                              int64_t npairs, int64_t src_nslots, int64_t dst_nslots,
+                              int32_t pad, int32_t* dev_status, void* stream);
+cc1d_status_t cc1d_slots_compact(const cc1d_slot_cache* table, int32_t ncaches,
+                                 const uint8_t* live, int64_t nslots, int32_t* remap,
+                                 int32_t* count, int32_t* moves, void* stream);
 
 #ifdef __cplusplus
 }

@@ -380,7 +380,10 @@ cc1d_status_t cc1d_gdr_varlen(const cc1d_gdr_args* args, void* stream) {
         return fail(CC1D_ERR_INVALID, "%lld slots for %lld sequences without indices",
                     (long long)a.nslots, (long long)a.rows);
     if (cc1d_status_t s = bind_stream(stream)) return s;
-    return from_cuda(cc1d::launch_gdr_recurrent(a, true, (cudaStream_t)stream), "cc1d_gdr_varlen");
+    return from_cuda(cc1d::gdr_chunk_serves(a)
+                         ? cc1d::launch_gdr_chunk(a, (cudaStream_t)stream)
+                         : cc1d::launch_gdr_recurrent(a, true, (cudaStream_t)stream),
+                     "cc1d_gdr_varlen");
 }
 
 cc1d_status_t cc1d_rms_norm_gated(const cc1d_norm_args* args, void* stream) {

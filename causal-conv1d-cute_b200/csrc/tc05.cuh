@@ -1,0 +1,170 @@
+// 5th-generation tensor core (tcgen05) and mbarrier primitives for sm_100a, as inline PTX.
+//
+// Shared-memory operand images are rows of 128 (or 64) bytes whose 16-byte units are permuted
+// within groups of eight rows: unit u of row r lies at u ^ (r & 7) (u ^ ((r >> 1) & 3) for 64-byte
+// rows). The same bytes serve as a K-major operand (rows along M or N) or an MN-major one (rows
+// along K), by the descriptor and the major bits of the instruction descriptor alone.
+#pragma once
+
+#include "common.cuh"
+
+namespace cc1d {
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) {
+    return (uint32_t)__cvta_generic_to_shared(p);
+}
+
+// ---------------------------------------------------------------------------------------- barriers
+
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Wait until the phase of the given parity has completed, for two seconds at most (a chunk takes
+// microseconds). When one wait of the CTA has run out, *abort is set and every later wait returns
+// at once, so that the CTA runs to its end, with wrong results that it reports, and frees its TMEM.
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+__device__ __noinline__ void mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort) {
+    unsigned long long start, now;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(start));
+    while (!*abort) {
+        for (int i = 0; i < 64; ++i)
+            if (mbar_try(bar, parity)) return;
+        asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+        if (now - start > 2000000000ull) *abort = 1;
+    }
+}
+__device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+    for (int i = 0; i < 16; ++i)
+        if (mbar_try(bar, parity)) return;
+    mbar_wait_slow(bar, parity, abort);
+}
+// Barrier of `threads` threads (whole warps) of the CTA.
+__device__ __forceinline__ void named_sync(int id, int threads) {
+    __syncwarp();
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+// Makes this thread's shared-memory writes visible to the tensor core.
+__device__ __forceinline__ void fence_async_smem() {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// -------------------------------------------------------------------------------- tensor memory
+
+__device__ __forceinline__ void tmem_alloc(uint32_t smem_result, int columns) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_result),
+                 "r"(columns)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_relinquish() {
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc(uint32_t tmem, int columns) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns)
+                 : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() {
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc_fence_after() {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+
+// 32 fp32 columns of the warp's 32 lanes: lane l of the warp gets row l. `tmem` carries the warp's
+// first lane in its upper half. The values may be used after tmem_wait_ld().
+__device__ __forceinline__ void tmem_ld32(uint32_t tmem, float* f) {
+    uint32_t r[32];
+    __syncwarp();
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+          "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+          "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(tmem)
+        : "memory");
+    // The wait stands here so that no use of the registers can be scheduled before it.
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
+}
+
+// ------------------------------------------------------------------------------------------ MMA
+
+enum : uint64_t { kSwizzle128 = 2, kSwizzle64 = 4 };
+
+// Operand descriptor: start address, byte offset between 64-element atoms along MN (MN-major
+// operands wider than one atom), byte offset between groups of eight rows, row swizzle.
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t atom, uint32_t group,
+                                            uint64_t swizzle) {
+    return (uint64_t)((addr & 0x3ffff) >> 4) | ((uint64_t)(atom >> 4) << 16) |
+           ((uint64_t)(group >> 4) << 32) | (1ull << 46) | (swizzle << 61);
+}
+
+// Instruction descriptor: bf16 x bf16 -> fp32, M = 128.
+__host__ __device__ constexpr uint32_t mma_desc(int n, bool a_mn, bool b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((a_mn ? 1u : 0u) << 15) |
+           ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+
+// D (TMEM, fp32) (+)= A B for one K step of 16; one thread issues it.
+__device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uint32_t desc,
+                                         bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(desc), "r"(accumulate ? 1u : 0u)
+        : "memory");
+}
+// Arrive on the mbarrier when all MMAs this thread has issued so far are complete.
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+        : "memory");
+}
+
+// ------------------------------------------------------------------------------- two-part bf16
+
+// (a, b) as bf16 pairs: hi rounds to nearest, lo rounds the rest, so that hi + lo is within 2^-17
+// of the value. Low halves hold a.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(b), "f"(a));
+    const float ra = a - __uint_as_float(hi << 16);
+    const float rb = b - __uint_as_float(hi & 0xffff0000u);
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(rb), "f"(ra));
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void sts16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
+                 : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
+}  // namespace cc1d

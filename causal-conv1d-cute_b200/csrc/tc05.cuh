@@ -6,6 +6,8 @@
 // along K), by the descriptor and the major bits of the instruction descriptor alone.
 #pragma once
 
+#include <cuda.h>  // CUtensorMap
+
 #include "common.cuh"
 
 namespace cc1d {
@@ -21,6 +23,11 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// The same, announcing bytes that bulk copies will bring.
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+                 : "memory");
 }
 // Wait until the phase of the given parity has completed, for two seconds at most (a chunk takes
 // microseconds). When one wait of the CTA has run out, *abort is set and every later wait returns
@@ -61,6 +68,16 @@ __device__ __forceinline__ void fence_async_smem() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+// One box of a tensor map at (x, y, z) into shared memory, counted on the mbarrier.
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
+                                         uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+
 // -------------------------------------------------------------------------------- tensor memory
 
 __device__ __forceinline__ void tmem_alloc(uint32_t smem_result, int columns) {
@@ -83,14 +100,15 @@ __device__ __forceinline__ void tc_fence_after() {
 }
 
 // 32 fp32 columns of the warp's 32 lanes: lane l of the warp gets row l. `tmem` carries the warp's
-// first lane in its upper half. The values may be used after tmem_wait_ld().
+// first lane in its upper half. 
 __device__ __forceinline__ void tmem_ld32(uint32_t tmem, float* f) {
     uint32_t r[32];
     __syncwarp();
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
         "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
           "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
           "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
@@ -98,10 +116,32 @@ __device__ __forceinline__ void tmem_ld32(uint32_t tmem, float* f) {
           "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(tmem)
         : "memory");
-    // The wait stands here so that no use of the registers can be scheduled before it.
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
     for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
+}
+
+// 16 columns from each of two places, as above.
+__device__ __forceinline__ void tmem_ld16x2(uint32_t t0, uint32_t t1, float* f, float* g) {
+    uint32_t r[16], s[16];
+    __syncwarp();
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15]), "=r"(s[0]), "=r"(s[1]), "=r"(s[2]), "=r"(s[3]), "=r"(s[4]),
+          "=r"(s[5]), "=r"(s[6]), "=r"(s[7]), "=r"(s[8]), "=r"(s[9]), "=r"(s[10]), "=r"(s[11]),
+          "=r"(s[12]), "=r"(s[13]), "=r"(s[14]), "=r"(s[15])
+        : "r"(t0), "r"(t1)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        f[i] = __uint_as_float(r[i]);
+        g[i] = __uint_as_float(s[i]);
+    }
 }
 
 // ------------------------------------------------------------------------------------------ MMA

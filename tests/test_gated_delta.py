@@ -241,6 +241,16 @@ def test_varlen_batches(lengths):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [13, 25, 60, 300])
+@pytest.mark.parametrize("sdtype", [F32, BF])
+def test_varlen_many_sequences(n, sdtype):
+    """Enough (sequence, head) pairs to fill the GPU with each width of a work tile; uneven lengths."""
+    r = torch.Generator().manual_seed(n)
+    lengths = torch.randint(0, 150, (n,), generator=r).tolist()
+    varlen_case(lengths, hk=1, hv=6, sdtype=sdtype, seed=n)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("hk,hv", [(1, 1), (1, 3), (2, 2), (4, 8), (3, 6)])
 def test_varlen_head_groups(hk, hv):
     varlen_case([100, 31, 70], hk=hk, hv=hv, seed=hk)

@@ -17,15 +17,16 @@
 //
 // Split of the work. Chunks of one sequence form a chain; heads, sequences and the columns of the
 // state are independent. A CTA takes one head of one sequence, NG tiles of VS state columns, and has
-//   - a prep warpgroup: [K;Q] K^T on the tensor core, L, its inverse, T and G = P T. Nothing of it
+//   - prep warps: [K;Q] K^T on the tensor core, L, its inverse, T and G = P T. Nothing of it
 //     depends on the state, so it runs ahead of the chain;
-//   - NG scan warpgroups, each with the chain of its own columns: [K;Q] S0, R, [T;G] R, u, K^T u, S.
-//     Two chains in a CTA fill each other's waits and share K, Q, T and G. K, Q and V come by TMA
-//     up to three chunks ahead.
+//   - NG scan groups of 256 threads (two per row), each with the chain of its own columns: [K;Q] S0,
+//     R, [T;G] R, u, K^T u, S. Two chains in a CTA fill each other's waits and share K, Q, T and G.
+// K, Q and V come by TMA, K and Q up to three chunks ahead. The state lies in TMEM.
 // Stacking K over Q and T over G makes every product M = 128, the full tensor core rate; the two
 // parts of an operand lie side by side as one operand of 2 VS columns (measured: a K step of 16
 // costs 46 cycles up to 64 columns and 66 with 128, so one wide step beats two narrow ones).
-
+// Loops over columns stay rolled where registers allow it: with all of them unrolled the warps
+// spent a quarter of their time waiting for instructions.
 #include "gdr.cuh"
 #include "kernels.h"
 #include "tc05.cuh"
@@ -45,10 +46,10 @@ struct Vectors {     // per chunk: what the scan multiplies rows by
     float pad[3];
 };
 
-// I + L in 32 x 32 blocks, fp32: the diagonal blocks (L, then their inverses in place), the block
-// below them, and L_21 inv_0 transposed.
+// I + L in 32 x 32 blocks, fp32: the diagonal blocks (L, then their inverses in place) and the
+// block below them.
 struct Blocks {
-    float diag[2][32][LPAD], low[32][LPAD], prod[32][LPAD];
+    float diag[2][32][LPAD], low[32][LPAD];
 };
 
 template <int VS, int NG>
@@ -56,26 +57,30 @@ struct Layout {
     static constexpr int kRow = VS >= 64 ? 128 : 2 * VS;  // bytes of an operand row of VS columns
     static constexpr int kS = 128 * kRow;                 // one part (hi or lo) of S
     static constexpr int kR = C * kRow;                   // one part of R or u, or one tile of V
-    static constexpr int kStages = NG == 1 ? 3 : 2;       // of K, Q, V
+    static constexpr int kStages = NG == 1 ? 3 : 2;       // of K and Q
     static constexpr int KQ = 0;                          // stages x [2 halves][128 rows][128 B]
-    static constexpr int V = KQ + kStages * 32768;        // stages x NG x [64 rows]
-    static constexpr int TG = V + kStages * NG * kR;      // [hi, lo][128 rows][128 B]
+    static constexpr int V = KQ + kStages * 32768;        // NG x [64 rows]
+    static constexpr int TG = V + NG * kR;                // [hi, lo][128 rows][128 B]
     static constexpr int SB = TG + 32768;                 // NG x (S hi, S lo); R in S hi, u in S lo
-    static constexpr int B = SB + NG * 2 * kS;            // Blocks
+    static constexpr int P = SB + NG * 2 * kS;            // [hi, lo][64 rows][128 B]
+    static constexpr int B = P + 16384;                   // Blocks
     static constexpr int VEC = B + (int)sizeof(Blocks);   // 2 stages x Vectors
     static constexpr int END = VEC + 2 * (int)sizeof(Vectors);
-    static constexpr int kTmem = 128 + NG * 2 * VS <= 256 ? 256 : 512;
-    static constexpr int kThreads = 128 * (NG + 1);
+    static constexpr int kTmem = 128 + NG * 3 * VS <= 256 ? 256 : 512;
+    static constexpr int kPrepWarps = NG == 1 ? 8 : 4;
+    static constexpr int kThreads = 256 * NG + 32 * kPrepWarps;
 };
+// P as a 128-row operand reads 8 KB behind its last row.
+static_assert(sizeof(Blocks) >= 8192, "");
 
 struct Shared {
-    uint64_t tma_full[3], kq_full[3], vec_full[2], tg_full, tg_free, prep_mma, scan_mma[2];
+    uint64_t kq_tma[3], kq_full[3], vec_full[2], v_full[2], tg_full, tg_free, prep_mma, scan_mma[2];
     uint32_t tmem;
     int abort;
     int row;  // sequence of this CTA
-    int done[3];  // per stage: scan warpgroups that are through with its K, Q and V, over all chunks
+    int done[3];  // per stage: scan groups that are through with its K and Q, over all chunks
     int len[kOrderMax];
-    alignas(16) float bh[C], bl[C], rk[C], ru[32], beta[C];
+    alignas(16) float bh[C], bl[C], rk[C], ru[32], beta[C], qq[2][C];
     double half;
 };
 
@@ -90,36 +95,36 @@ __device__ __forceinline__ uint32_t swz(int r, int u) {
 }
 
 // 8 values as two bf16 parts, one 16-byte unit each.
-__device__ __forceinline__ void store_split8(uint32_t hi, uint32_t lo, const float* f) {
+__device__ __forceinline__ void store_split8(uint32_t hi, uint32_t lo, const float2* f) {
     uint32_t h[4], l[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) split2(f[2 * i], f[2 * i + 1], h[i], l[i]);
+    for (int i = 0; i < 4; ++i) split2(f[i], h[i], l[i]);
     sts16(hi, h[0], h[1], h[2], h[3]);
     sts16(lo, l[0], l[1], l[2], l[3]);
 }
+__device__ __forceinline__ float2 mul2(float2 a, float b) {
+    return __fmul2_rn(a, make_float2(b, b));
+}
+__device__ __forceinline__ float2 bf16_pair(uint32_t v) {
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
 
-// Row i of the inverse of I + l (l strictly lower triangular, 32 x 32, zeros above) by backward
+// Row i of the inverse of I + l (l strictly lower triangular, 16 x 16, zeros above) by backward
 // substitution: y_m is final once every later y has been taken out of it, and is then taken out of
 // the earlier ones along row m of l. A lane owns a row; the rows of l come as broadcasts.
-__device__ __forceinline__ void solve_row(const float (*l)[LPAD], int i, float* y) {
-    float2 acc[16];
+__device__ __forceinline__ void solve_row16(const float (*l)[LPAD], int i, float2* y) {
 #pragma unroll
-    for (int q = 0; q < 16; ++q) acc[q] = make_float2(i == 2 * q ? 1.f : 0.f, i == 2 * q + 1 ? 1.f : 0.f);
+    for (int q = 0; q < 8; ++q) y[q] = make_float2(i == 2 * q ? 1.f : 0.f, i == 2 * q + 1 ? 1.f : 0.f);
 #pragma unroll
-    for (int m = 31; m > 0; --m) {
-        const float v = -(m % 2 ? acc[m / 2].y : acc[m / 2].x);
+    for (int m = 15; m > 0; --m) {
+        const float v = -(m % 2 ? y[m / 2].y : y[m / 2].x);
         const float2 vv = make_float2(v, v);
 #pragma unroll
         for (int r = 0; r < m; r += 4) {
             const float4 f = *reinterpret_cast<const float4*>(&l[m][r]);
-            acc[r / 2] = __ffma2_rn(make_float2(f.x, f.y), vv, acc[r / 2]);
-            if (r + 2 < m) acc[r / 2 + 1] = __ffma2_rn(make_float2(f.z, f.w), vv, acc[r / 2 + 1]);
+            y[r / 2] = __ffma2_rn(make_float2(f.x, f.y), vv, y[r / 2]);
+            if (r + 2 < m) y[r / 2 + 1] = __ffma2_rn(make_float2(f.z, f.w), vv, y[r / 2 + 1]);
         }
-    }
-#pragma unroll
-    for (int q = 0; q < 16; ++q) {
-        y[2 * q] = acc[q].x;
-        y[2 * q + 1] = acc[q].y;
     }
 }
 
@@ -131,39 +136,60 @@ __device__ __forceinline__ void mma_warp(float* d, const uint32_t* a, const uint
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
+__device__ __forceinline__ void mma_warp3(float* d, const uint32_t (*a)[4], const uint32_t (*b)[2]) {
+    mma_warp(d, a[0], b[0]);
+    mma_warp(d, a[0], b[1]);
+    mma_warp(d, a[1], b[0]);
+}
 
-// The warp's 16 x 16 tile at (r0, c0) of a 32 x 32 product a b, in two-part bf16. a is row-major;
-// b is row-major, or transposed (kBt). d: two 16 x 8 accumulator fragments.
-template <bool kBt>
-__device__ __forceinline__ void block_product(const float (*a)[LPAD], const float (*b)[LPAD], int r0,
-                                              int c0, int lane, float (*d)[4]) {
+// The 16 x 16 tile inv1[r0.., :] (low inv0)[:, c0..] of a product of K x K matrices, K = 16 or 32,
+// by one warp in two-part bf16. The inner product is formed transposed, (inv0^T low^T): its
+// accumulator fragments are then the B fragments of the outer one. d: accumulators of columns c0..
+// and c0 + 8...
+template <int K>
+__device__ __forceinline__ void merge_tile(const float (*inv1)[LPAD], const float (*low)[LPAD],
+                                           const float (*inv0)[LPAD], int r0, int c0, int lane,
+                                           float (*d)[4]) {
     const int g = lane / 4, t2 = lane % 4 * 2;
+    float m[K / 8][4];  // (low inv0)^T: rows c0.., 8 columns (rows of low) each
+#pragma unroll
+    for (int n = 0; n < K / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m[n][e] = 0.f;
+#pragma unroll
+    for (int k0 = 0; k0 < K; k0 += 16) {
+        uint32_t av[2][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int col = c0 + g + e % 2 * 8, k = k0 + t2 + e / 2 * 8;
+            split2(make_float2(inv0[k][col], inv0[k + 1][col]), av[0][e], av[1][e]);
+        }
+#pragma unroll
+        for (int n = 0; n < K / 8; ++n) {
+            uint32_t bv[2][2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                split2(*reinterpret_cast<const float2*>(&low[8 * n + g][k0 + t2 + 8 * e]), bv[0][e], bv[1][e]);
+            mma_warp3(m[n], av, bv);
+        }
+    }
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) d[n][e] = 0.f;
 #pragma unroll
-    for (int k0 = 0; k0 < 32; k0 += 16) {
-        uint32_t ah[4], al[4];
+    for (int k0 = 0; k0 < K; k0 += 16) {
+        uint32_t av[2][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 f = *reinterpret_cast<const float2*>(&a[r0 + g + e % 2 * 8][k0 + t2 + e / 2 * 8]);
-            split2(f.x, f.y, ah[e], al[e]);
-        }
+        for (int e = 0; e < 4; ++e)
+            split2(*reinterpret_cast<const float2*>(&inv1[r0 + g + e % 2 * 8][k0 + t2 + e / 2 * 8]), av[0][e], av[1][e]);
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            uint32_t bh[2], bl[2];
-            const int col = c0 + 8 * n + g;
+            uint32_t bv[2][2];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int k = k0 + t2 + 8 * e;
-                const float2 f = kBt ? *reinterpret_cast<const float2*>(&b[col][k])
-                                     : make_float2(b[k][col], b[k + 1][col]);
-                split2(f.x, f.y, bh[e], bl[e]);
-            }
-            mma_warp(d[n], ah, bh);
-            mma_warp(d[n], ah, bl);
-            mma_warp(d[n], al, bh);
+            for (int e = 0; e < 2; ++e)
+                split2(make_float2(m[k0 / 8 + e][2 * n], m[k0 / 8 + e][2 * n + 1]), bv[0][e], bv[1][e]);
+            mma_warp3(d[n], av, bv);
         }
     }
 }
@@ -186,6 +212,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
     using Lay = Layout<VS, NG>;
     constexpr uint64_t kSwz = VS >= 64 ? kSwizzle128 : kSwizzle64;
     constexpr uint32_t kGroup = 8 * Lay::kRow;  // bytes of eight rows of V columns
+    constexpr int kStages = Lay::kStages;
     extern __shared__ __align__(1024) unsigned char raw[];
     __shared__ Shared sh;
     const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
@@ -193,7 +220,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
     Vectors* vec = reinterpret_cast<Vectors*>(gen + Lay::VEC);
     Blocks& blk = *reinterpret_cast<Blocks*>(gen + Lay::B);
 
-    const int tid = threadIdx.x, warp = tid / 32, p = tid % 128;
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, p = tid % 128, w = warp % 4;
     const int vt = blockIdx.x % tiles;  // columns vt * NG * VS ..
     const int h = (int)((blockIdx.x / tiles) % a.heads_v);
     int64_t row = blockIdx.x / tiles / a.heads_v;
@@ -221,12 +248,13 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
 
     if (tid == 0) {
         for (int i = 0; i < 3; ++i) {
-            mbar_init(smem_addr(&sh.tma_full[i]), 1);
+            mbar_init(smem_addr(&sh.kq_tma[i]), 1);
             mbar_init(smem_addr(&sh.kq_full[i]), 1);
             sh.done[i] = 0;
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_addr(&sh.vec_full[i]), 1);
+            mbar_init(smem_addr(&sh.v_full[i]), 1);
             mbar_init(smem_addr(&sh.scan_mma[i]), 1);
         }
         mbar_init(smem_addr(&sh.tg_full), 1);
@@ -243,39 +271,49 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
-    const uint32_t lanes = (uint32_t)(warp % 4) << 21;  // the warp's first TMEM lane, in bits 16..
+    const uint32_t lanes = (uint32_t)w << 21;  // the warp's first TMEM lane, in bits 16..
     const uint32_t tg = base + Lay::TG;
 
-    // K, Q and V of chunk c into stage st, which must be free; one thread.
-    constexpr int kStages = Lay::kStages;
-    auto load = [&](int c, int st) {
-        const uint32_t full = smem_addr(&sh.tma_full[st]), kq = base + Lay::KQ + st * 32768;
+    // K and Q of chunk c into stage st, which must be free; one thread.
+    auto load_kq = [&](int c, int st) {
+        const uint32_t full = smem_addr(&sh.kq_tma[st]), kq = base + Lay::KQ + st * 32768;
         const int t = (int)tok0 + c * C;
-        mbar_expect(full, 32768 + NG * C * VS * 2);
+        mbar_expect(full, 32768);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             tma_load(kq + half * 16384, &mapk, half * 64, hk, t, full);
             tma_load(kq + half * 16384 + 8192, &mapq, half * 64, hk, t, full);
         }
-#pragma unroll
-        for (int g = 0; g < NG; ++g)
-            tma_load(base + Lay::V + (st * NG + g) * Lay::kR, &mapv, (vt * NG + g) * VS, h, t, full);
+    };
+    // V of chunk c for scan group g.
+    auto load_v = [&](int c, int g) {
+        const uint32_t full = smem_addr(&sh.v_full[g]);
+        mbar_expect(full, C * VS * 2);
+        tma_load(base + Lay::V + g * Lay::kR, &mapv, (vt * NG + g) * VS, h, (int)tok0 + c * C, full);
     };
     if (tid == 0) {
-        for (int c = 0; c < kStages && c < chunks; ++c) load(c, c);
+        for (int c = 0; c < kStages && c < chunks; ++c) load_kq(c, c);
+        for (int g = 0; g < NG; ++g) load_v(0, g);
     }
 
-    if (warp >= 4 * NG) {
+    if (warp >= 8 * NG) {
         // --------------------------------------------------------------------------------- prep
-        const int w = warp % 4, lane = tid % 32, i = p % C;
+        // A thread has row p of [K;Q] K^T: columns 32 half .., both halves in turn with four warps.
+        constexpr int kPrep = 32 * Lay::kPrepWarps, kHalves = kPrep / 128;
+        const int half0 = (warp - 8 * NG) / 4;
+        const int i = p % C;
+        const bool gates = p < C && half0 == 0;  // threads that also keep a token's gates
         const uint32_t D0 = tmem;  // 64 columns of [K;Q] K^T; later 128 of P [T hi | T lo]
+        const uint32_t pb = base + Lay::P;
         const int64_t g0 = tok0 * a.g_st + h * a.g_sh, b0 = tok0 * a.b_st + h * a.b_sh;
-        // T is zero above its diagonal blocks; nothing writes there again.
-        if (p < 32) {
+        // T and P are zero above their diagonal blocks; nothing writes there again.
+        if (p < 32 && half0 == 0) {
 #pragma unroll
             for (int u = 4; u < 8; ++u) {
                 sts16(tg + swz<128>(p, u), 0, 0, 0, 0);
                 sts16(tg + 16384 + swz<128>(p, u), 0, 0, 0, 0);
+                sts16(pb + swz<128>(p, u), 0, 0, 0, 0);
+                sts16(pb + 8192 + swz<128>(p, u), 0, 0, 0, 0);
             }
         }
         float rate = 0.f, dt = 0.f;
@@ -286,7 +324,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
         uint32_t g_bits = 0, b_bits = 0;
         auto load_gate_bits = [&](int c) {
             const int64_t t = (int64_t)c * C + p;
-            if (p < C && t < ntok) {
+            if (gates && t < ntok) {
                 g_bits = load_bits(a.g, g0 + t * a.g_st, a.gdtype);
                 b_bits = load_bits(a.beta, b0 + t * a.b_st, a.bdtype);
             }
@@ -295,13 +333,14 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
 
         int st = 0;
         uint32_t st_phase = 0;
+#pragma unroll 1
         for (int c = 0; c < chunks; ++c) {
             Vectors& ve = vec[c & 1];
             const uint32_t kq = base + Lay::KQ + st * 32768;
             const int left = ntok - c * C;
             // Gates of this chunk, bits of the next one's.
             float g = 0.f, beta = 0.f;
-            if (p < C && p < left) {
+            if (gates && p < left) {
                 g = bits_value(g_bits, a.gdtype);
                 beta = bits_value(b_bits, a.bdtype);
                 if (a.a_log != nullptr) {
@@ -311,37 +350,28 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
                 }
             }
             load_gate_bits(c + 1);
-            mbar_wait(smem_addr(&sh.tma_full[st]), st_phase, &sh.abort);
+            mbar_wait(smem_addr(&sh.kq_tma[st]), st_phase, &sh.abort);
             if (left < C) {
                 // The copies went on into the next sequence: zeros there, whatever it holds.
-                for (int e = p; e < (C - left) * 32; e += 128) {
+                for (int e = tid % kPrep; e < (C - left) * 32; e += kPrep) {
                     const int r = left + e / 32, u = e % 16;
                     sts16(kq + (u >> 3) * 16384 + swz<128>(r + (e & 16) * 4, u & 7), 0, 0, 0, 0);
-                }
-                for (int e = p; e < (C - left) * (NG * VS / 8); e += 128) {
-                    const int r = left + e / (NG * VS / 8), u = e % (NG * VS / 8);
-                    sts16(base + Lay::V + (st * NG + u / (VS / 8)) * Lay::kR +
-                              swz<Lay::kRow>(r, u % (VS / 8)), 0, 0, 0, 0);
                 }
                 fence_async_smem();
             }
             tc_fence_before();
-            named_sync(8, 128);
-            if (p == 0) {
+            named_sync(8, kPrep);
+            if (tid % kPrep == 0) {
                 mbar_arrive(smem_addr(&sh.kq_full[st]));
                 tc_fence_after();
-#pragma unroll
-                for (int ks = 0; ks < 8; ++ks) {
-                    const uint32_t at = kq + (ks >> 2) * 16384 + (ks & 3) * 32;
-                    mma_bf16(D0, operand(at, 16, 1024, kSwizzle128), operand(at, 16, 1024, kSwizzle128),
-                             mma_desc(64, false, false), ks > 0);
-                }
+                const uint64_t d = operand(kq, 16, 1024, kSwizzle128);
+                mma_steps(D0, d, 2, d, 2, 4, mma_desc(64, false, false), false);
+                mma_steps(D0, d + 1024, 2, d + 1024, 2, 4, mma_desc(64, false, false), true);
                 mma_commit(smem_addr(&sh.prep_mma));
             }
             // While it runs: cumulative decays (threads of K rows), query norms (Q rows).
-            float row_mul = a.scale;  // of row i of Q K^T; of K K^T below
             double total = 0;
-            if (p < C) {
+            if (gates) {
                 // -1e5 decays anything to zero, and its sums stay finite where -inf would give
                 // inf - inf below.
                 g = g < -1e5f ? -1e5f : g;
@@ -355,192 +385,209 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
                 }
                 if (p == 31) sh.half = total;
                 sh.beta[p] = beta;
-            } else if (a.l2norm) {
-                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            } else if (p >= C && a.l2norm) {
+                for (int hf = half0; hf < 2; hf += kHalves) {
+                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll 4
+                    for (int u = 0; u < 8; ++u) {
+                        const uint4 v = lds16(kq + hf * 16384 + swz<128>(p, u));
+                        const uint32_t vv[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                for (int u = 0; u < 16; ++u) {
-                    float f[8];
-                    unpack16<bf16>(lds16(kq + (u >> 3) * 16384 + swz<128>(p, u & 7)), f);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 ff = make_float2(f[2 * e], f[2 * e + 1]);
-                        sum[e % 2] = __ffma2_rn(ff, ff, sum[e % 2]);
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 f = bf16_pair(vv[e]);
+                            sum[e % 2] = __ffma2_rn(f, f, sum[e % 2]);
+                        }
                     }
+                    sh.qq[hf][i] = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 }
-                row_mul *= rsqrtf((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y) + kL2Eps);
             }
-            named_sync(8, 128);
-            float far = 0.f;  // decay between token i and the middle of the chunk
-            if (p < C) {
+            named_sync(8, kPrep);
+            float far = 0.f;  // decay between token p and the middle of the chunk, for p < 32
+            if (gates) {
                 const double mid = sh.half;
                 if (p >= 32) total += mid;
                 const float hi = (float)total;
                 sh.bh[p] = hi;
                 sh.bl[p] = (float)(total - (double)hi);
-                far = exp2_approx((float)(mid - total));  // used below 32 only
+                far = exp2_approx((float)(mid - total));
             }
             mbar_wait(smem_addr(&sh.prep_mma), 0, &sh.abort);
             tc_fence_after();
-            float x[C];
-            tmem_ld32(D0 + lanes, x);
-            tmem_ld32(D0 + lanes + 32, x + 32);
-            if (p < C) {
+            if (p < C && (w % 2 == half0 || kHalves == 1)) {
+                // |k_i|^2 is the diagonal of K K^T: element i % 16 of a group of 16 columns.
                 float d = 0.f;
 #pragma unroll
-                for (int j = 0; j < C; ++j) d = j == p ? x[j] : d;
-                const float rk = a.l2norm ? rsqrtf(d + kL2Eps) : 1.f;
-                sh.rk[p] = rk;
-                if (p < 32) sh.ru[p] = rk * far;
-                row_mul = beta * rk;
+                for (int o = 0; o < 32; o += 16) {
+                    float2 x[8];
+                    tmem_ld16(D0 + lanes + 32 * w + o, x);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        d = lane == o + 2 * e ? x[e].x : d;
+                        d = lane == o + 2 * e + 1 ? x[e].y : d;
+                    }
+                }
+                sh.rk[p] = a.l2norm ? rsqrtf(d + kL2Eps) : 1.f;
             }
-            named_sync(8, 128);
-            // Warps 0 and 1 hold rows of K K^T and make L (columns j < i), warps 2 and 3 rows of
-            // Q K^T and make P (columns j <= i). In the columns of a row's own half the decay
-            // e^(b_i - b_j) is taken element by element; for the lower left block it splits at the
-            // middle of the chunk into two factors of at most 1.
-            {
-                const float bh = sh.bh[i], bl = sh.bl[i], rk = sh.rk[i];
+            named_sync(8, kPrep);
+            // Warps 0 and 1 make L (columns j < i) of rows of K K^T, warps 2 and 3 make P (columns
+            // j <= i) of rows of Q K^T. In the columns of a row's own half the decay e^(b_i - b_j)
+            // is taken element by element; for the lower left block it splits at the middle of the
+            // chunk into two factors of at most 1.
+            const float bh = sh.bh[i], bl = sh.bl[i], rk = sh.rk[i];
+            const float mul = p < C ? sh.beta[i] * rk
+                                    : a.l2norm ? a.scale * rsqrtf(sh.qq[0][i] + sh.qq[1][i] + kL2Eps) : a.scale;
+            if (half0 == 0) {
                 const float grow = exp2_approx(bh + bl);
-                ve.in[p] = grow * (p < C ? rk : row_mul);
+                ve.in[p] = grow * (p < C ? rk : mul);
                 if (p < C) {
                     ve.out[i] = rk * exp2_approx((sh.bh[C - 1] - bh) + (sh.bl[C - 1] - bl));
+                    if (p < 32) sh.ru[p] = rk * far;
                     if (i == C - 1) ve.decay = grow;
                 }
-                const int last = p < C ? i - 1 : i;
-                const float mid = sh.bh[31], mid_l = sh.bl[31];
-                const float low_mul = row_mul * exp2_approx((bh - mid) + (bl - mid_l));
+            }
+            // ru is used by other warps than its writers.
+            named_sync(8, kPrep);
+            if (tid % kPrep == 0) mbar_arrive(smem_addr(&sh.vec_full[c & 1]));
+#pragma unroll 1
+            for (int hf = half0; hf < 2; hf += kHalves) {
+                if (hf > w % 2) continue;  // above the diagonal block
+                const bool own = hf == w % 2;
+                const float low_mul = mul * exp2_approx((bh - sh.bh[31]) + (bl - sh.bl[31]));
+                const int last = (p < C ? i - 1 : i) - 32 * hf;  // last column of this half that counts
+                float (*to)[LPAD] = own ? blk.diag[w % 2] : blk.low;
+#pragma unroll 1
+                for (int o = 0; o < 32; o += 16) {
+                    float2 x[8];
+                    tmem_ld16(D0 + lanes + 32 * hf + o, x);
+                    if (own) {
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    float* y = x + 32 * hf;
-                    if (w % 2 == hf) {
-#pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
-                            const int j = 32 * hf + e;
+                        for (int e = 0; e < 8; e += 2) {
+                            const int j = 32 * hf + o + 2 * e;
                             const float4 h4 = *reinterpret_cast<const float4*>(&sh.bh[j]);
                             const float4 l4 = *reinterpret_cast<const float4*>(&sh.bl[j]);
                             const float4 r4 = *reinterpret_cast<const float4*>(&sh.rk[j]);
-                            const float hj[4] = {h4.x, h4.y, h4.z, h4.w}, lj[4] = {l4.x, l4.y, l4.z, l4.w};
-                            const float rj[4] = {r4.x, r4.y, r4.z, r4.w};
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const float ex = exp2_approx((bh - hj[k]) + (bl - lj[k]));
-                                y[e + k] = j + k <= last ? y[e + k] * (row_mul * rj[k]) * ex : 0.f;
-                            }
-                        }
-                    } else if (hf == 0) {
-#pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
-                            const float4 r4 = *reinterpret_cast<const float4*>(&sh.ru[e]);
-                            y[e] *= low_mul * r4.x;
-                            y[e + 1] *= low_mul * r4.y;
-                            y[e + 2] *= low_mul * r4.z;
-                            y[e + 3] *= low_mul * r4.w;
+                            const int jj = o + 2 * e;
+                            x[e].x = jj <= last ? x[e].x * (mul * r4.x) * exp2_approx((bh - h4.x) + (bl - l4.x)) : 0.f;
+                            x[e].y = jj + 1 <= last ? x[e].y * (mul * r4.y) * exp2_approx((bh - h4.y) + (bl - l4.y)) : 0.f;
+                            x[e + 1].x = jj + 2 <= last ? x[e + 1].x * (mul * r4.z) * exp2_approx((bh - h4.z) + (bl - l4.z)) : 0.f;
+                            x[e + 1].y = jj + 3 <= last ? x[e + 1].y * (mul * r4.w) * exp2_approx((bh - h4.w) + (bl - l4.w)) : 0.f;
                         }
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) y[e] = 0.f;
+                        for (int e = 0; e < 8; e += 2) {
+                            const float4 r4 = *reinterpret_cast<const float4*>(&sh.ru[o + 2 * e]);
+                            x[e] = __fmul2_rn(x[e], mul2(make_float2(r4.x, r4.y), low_mul));
+                            x[e + 1] = __fmul2_rn(x[e + 1], mul2(make_float2(r4.z, r4.w), low_mul));
+                        }
+                    }
+                    if (p < C) {
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2)
+                            *reinterpret_cast<float4*>(&to[lane][o + 2 * e]) =
+                                make_float4(x[e].x, x[e].y, x[e + 1].x, x[e + 1].y);
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const uint32_t at = pb + swz<128>(i, 4 * hf + o / 8 + u);
+                            store_split8(at, at + 8192, x + 4 * u);
+                        }
                     }
                 }
             }
-            // What this thread writes into T (its row of a diagonal block) or P (its row).
-            uint32_t part[2][32];
-            if (w < 2) {
+            if (p < C && (w % 2 == half0 || kHalves == 1)) {
+                // Inverse of this warp's diagonal block: its two 16 x 16 blocks by substitution, a
+                // half warp each, then the block below them, -inv_1 (L_21 inv_0).
                 float (*dg)[LPAD] = blk.diag[w];
-#pragma unroll
-                for (int e = 0; e < 32; e += 4) {
-                    if (w == 0) {
-                        *reinterpret_cast<float4*>(&dg[lane][e]) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-                    } else {
-                        *reinterpret_cast<float4*>(&blk.low[lane][e]) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-                        *reinterpret_cast<float4*>(&dg[lane][e]) =
-                            make_float4(x[32 + e], x[33 + e], x[34 + e], x[35 + e]);
-                    }
-                }
+                const int b = lane & 16;
+                float2 y[8];
                 __syncwarp();
-                solve_row(dg, lane, x);
+                solve_row16(reinterpret_cast<const float (*)[LPAD]>(&dg[b][b]), lane & 15, y);
                 __syncwarp();
 #pragma unroll
-                for (int e = 0; e < 32; e += 4)
-                    *reinterpret_cast<float4*>(&dg[lane][e]) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+                for (int e = 0; e < 8; e += 2)
+                    *reinterpret_cast<float4*>(&dg[lane][b + 2 * e]) =
+                        make_float4(y[e].x, y[e].y, y[e + 1].x, y[e + 1].y);
+                __syncwarp();
+                float d[2][4];
+                merge_tile<16>(reinterpret_cast<const float (*)[LPAD]>(&dg[16][16]),
+                               reinterpret_cast<const float (*)[LPAD]>(&dg[16][0]), dg, 0, 0, lane, d);
+                __syncwarp();
 #pragma unroll
-                for (int e = 0; e < 32; e += 2)
-                    split2(x[e] * sh.beta[32 * w + e], x[e + 1] * sh.beta[32 * w + e + 1], part[0][e / 2], part[1][e / 2]);
-            } else {
+                for (int n = 0; n < 2; ++n)
 #pragma unroll
-                for (int e = 0; e < C; e += 2) split2(x[e], x[e + 1], part[0][e / 2], part[1][e / 2]);
+                    for (int e = 0; e < 2; ++e)
+                        *reinterpret_cast<float2*>(&dg[16 + lane / 4 + 8 * e][8 * n + lane % 4 * 2]) =
+                            make_float2(-d[n][2 * e], -d[n][2 * e + 1]);
             }
-            named_sync(8, 128);
-            if (p == 0) mbar_arrive(smem_addr(&sh.vec_full[c & 1]));
-            // The block below: -inv_1 (L_21 inv_0), a 16 x 16 tile per warp.
-            const int r0 = w / 2 * 16, c0 = w % 2 * 16, fr = r0 + lane / 4, fc = c0 + lane % 4 * 2;
-            float d[2][4];
-            block_product<false>(blk.low, blk.diag[0], r0, c0, lane, d);
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) blk.prod[fc + 8 * n + e % 2][fr + e / 2 * 8] = d[n][e];
-            named_sync(8, 128);
-            block_product<true>(blk.diag[1], blk.prod, r0, c0, lane, d);
+            named_sync(8, kPrep);
             // The chain's products with the previous T and G must be done with their memory.
             if (c > 0) mbar_wait(smem_addr(&sh.tg_free), (c - 1) & 1, &sh.abort);
+            if (half0 == 0) {
+                // The 32 x 32 block below the diagonal ones, a 16 x 16 tile per warp.
+                const int r0 = w / 2 * 16, c0 = w % 2 * 16, fr = r0 + lane / 4, fc = c0 + lane % 4 * 2;
+                float d[2][4];
+                merge_tile<32>(blk.diag[1], blk.low, blk.diag[0], r0, c0, lane, d);
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const int col = fc + 8 * n;
-                const float bt0 = -sh.beta[col], bt1 = -sh.beta[col + 1];
+                for (int n = 0; n < 2; ++n) {
+                    const int col = fc + 8 * n;
+                    const float2 bt = make_float2(-sh.beta[col], -sh.beta[col + 1]);
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    uint32_t hi, lo;
-                    split2(d[n][2 * e] * bt0, d[n][2 * e + 1] * bt1, hi, lo);
-                    const uint32_t at = tg + swz<128>(32 + fr + 8 * e, col / 8) + col % 8 * 2;
-                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(hi) : "memory");
-                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + 16384), "r"(lo) : "memory");
+                    for (int e = 0; e < 2; ++e) {
+                        uint32_t hi, lo;
+                        split2(__fmul2_rn(make_float2(d[n][2 * e], d[n][2 * e + 1]), bt), hi, lo);
+                        const uint32_t at = tg + swz<128>(32 + fr + 8 * e, col / 8) + col % 8 * 2;
+                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(hi) : "memory");
+                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + 16384), "r"(lo) : "memory");
+                    }
                 }
             }
+            if (half0 == kHalves - 1) {
+                // The diagonal blocks: row p / 2, half of its 32 columns.
+                const int r = p / 2, o = p % 2 * 16;
+#pragma unroll 1
+                for (int u = 0; u < 2; ++u) {
+                    const float* from = &blk.diag[r / 32][r % 32][o + 8 * u];
+                    const float* bt = &sh.beta[r / 32 * 32 + o + 8 * u];
+                    float2 f[4];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                if (w < 2 && u >= 4) continue;
-                const uint32_t at = tg + (w < 2 ? swz<128>(i, 4 * w + u) : swz<128>(p, u));
-                sts16(at, part[0][4 * u], part[0][4 * u + 1], part[0][4 * u + 2], part[0][4 * u + 3]);
-                sts16(at + 16384, part[1][4 * u], part[1][4 * u + 1], part[1][4 * u + 2], part[1][4 * u + 3]);
+                    for (int e = 0; e < 4; ++e)
+                        f[e] = __fmul2_rn(*reinterpret_cast<const float2*>(from + 2 * e),
+                                          *reinterpret_cast<const float2*>(bt + 2 * e));
+                    const uint32_t at = tg + swz<128>(r, r / 32 * 4 + o / 8 + u);
+                    store_split8(at, at + 16384, f);
+                }
             }
             fence_async_smem();
             tc_fence_before();
-            named_sync(8, 128);
-            if (p == 0) {
+            named_sync(8, kPrep);
+            if (tid % kPrep == 0) {
                 tc_fence_after();
-                // [T;P] T, of which the lower half is G: hi [hi | lo], then lo hi.
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks)
-                    mma_bf16(D0, operand(tg + ks * 32, 16, 1024, kSwizzle128),
-                             operand(tg + ks * 2048, 16384, 1024, kSwizzle128),
-                             mma_desc(128, false, true), ks > 0);
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks)
-                    mma_bf16(D0, operand(tg + 16384 + ks * 32, 16, 1024, kSwizzle128),
-                             operand(tg + ks * 2048, 16384, 1024, kSwizzle128),
-                             mma_desc(64, false, true), true);
+                // G = P T in rows 0..63: hi [hi | lo], then lo hi. Rows 64.. are of no use.
+                const uint64_t t = operand(tg, 16384, 1024, kSwizzle128);
+                mma_steps(D0, operand(pb, 16, 1024, kSwizzle128), 2, t, 128, 4, mma_desc(128, false, true), false);
+                mma_steps(D0, operand(pb + 8192, 16, 1024, kSwizzle128), 2, t, 128, 4, mma_desc(64, false, true), true);
                 mma_commit(smem_addr(&sh.prep_mma));
             }
             mbar_wait(smem_addr(&sh.prep_mma), 1, &sh.abort);
             tc_fence_after();
-            if (w >= 2) {
+            if (p < C) {
+#pragma unroll 1
+                for (int o = 16 * half0; o < C; o += 16 * kHalves) {
+                    float2 x[8], y[8];
+                    tmem_ld16(D0 + lanes + o, D0 + lanes + 64 + o, x, y);
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    tmem_ld32(D0 + lanes + 32 * hf, x);
-                    tmem_ld32(D0 + lanes + 64 + 32 * hf, x + 32);
+                    for (int e = 0; e < 8; ++e) x[e] = __fadd2_rn(x[e], y[e]);
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) x[8 * u + e] += x[32 + 8 * u + e];
-                        const uint32_t at = tg + swz<128>(p, 4 * hf + u);
-                        store_split8(at, at + 16384, x + 8 * u);
+                    for (int u = 0; u < 2; ++u) {
+                        const uint32_t at = tg + swz<128>(C + p, o / 8 + u);
+                        store_split8(at, at + 16384, x + 4 * u);
                     }
                 }
                 fence_async_smem();
             }
             tc_fence_before();
-            named_sync(8, 128);
-            if (p == 0) mbar_arrive(smem_addr(&sh.tg_full));
+            named_sync(8, kPrep);
+            if (tid % kPrep == 0) mbar_arrive(smem_addr(&sh.tg_full));
             if (++st == kStages) {
                 st = 0;
                 st_phase ^= 1;
@@ -548,140 +595,170 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
         }
     } else {
         // -------------------------------------------------------------------------------- scan
-        const int grp = warp / 4;
+        // A thread has row p and columns first .. first + W of its group's tile.
+        constexpr int W = VS / 2;
+        const int grp = warp / 8, first = warp / 4 % 2 * W;
         const int bar = 1 + grp;
-        const uint32_t D = tmem + 128 + grp * 2 * VS;  // [product with hi parts | with lo parts]
+        const bool lead = tid % 256 == 0;
+        const uint32_t D = tmem + 128 + grp * 3 * VS;  // [product with hi parts | with lo parts]
+        const uint32_t Dh = D + lanes + first, Dl = Dh + VS, TS = Dl + VS;  // TS: the state
         const uint32_t mma = smem_addr(&sh.scan_mma[grp]);
         const uint32_t s_hi = base + Lay::SB + grp * 2 * Lay::kS, s_lo = s_hi + Lay::kS;
         const uint32_t r_hi = s_hi, r_lo = r_hi + Lay::kR, u_hi = s_lo, u_lo = u_hi + Lay::kR;
-        const int col = (vt * NG + grp) * VS;
+        const uint32_t vb = base + Lay::V + grp * Lay::kR;
+        const int col = (vt * NG + grp) * VS + first;
         const bool initial = a.states != nullptr && a.has_initial_state != nullptr && a.has_initial_state[row];
         ST* sp = nullptr;
         if (a.states != nullptr)
             sp = static_cast<ST*>(a.states) + slot * a.s_slot + h * a.s_sh + p * a.s_sk + col;
-        float S[VS];  // row p of the state
         constexpr int SV = Vec<ST>::V;
-#pragma unroll
-        for (int j = 0; j < VS; j += SV) {
-            if (initial) {
-                unpack16<ST>(ld16(sp + j), S + j);
-            } else {
-#pragma unroll
-                for (int e = 0; e < SV; ++e) S[j + e] = 0.f;
-            }
-        }
         bf16* op = static_cast<bf16*>(a.out) + tok0 * a.o_st + h * a.o_sh + col;
 
         int st = 0;
         uint32_t phase = 0, st_phase = 0;
-        for (int c = 0; c < chunks; ++c) {
-            const uint32_t kq = base + Lay::KQ + st * 32768;
+        float decay = 0.f;
+#pragma unroll 1
+        for (int c = 0;; ++c) {
+            // The state after the chunk before, into TMEM, and as an operand if there is another.
+#pragma unroll 1
+            for (int o = 0; o < W; o += 16) {
+                float2 s[8];
+                if (c == 0) {
 #pragma unroll
-            for (int u = 0; u < VS / 8; ++u) {
-                const uint32_t at = swz<Lay::kRow>(p, u);
-                store_split8(s_hi + at, s_lo + at, S + 8 * u);
+                    for (int e = 0; e < 8; ++e) s[e] = make_float2(0.f, 0.f);
+                    if (initial) {
+#pragma unroll
+                        for (int e = 0; e < 16; e += SV) unpack16<ST>(ld16(sp + o + e), &s[0].x + e);
+                    }
+                } else {
+                    float2 d[8], e[8];
+                    tmem_ld16(Dh + o, Dl + o, TS + o, d, e, s);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        s[k] = __ffma2_rn(make_float2(decay, decay), s[k], __fadd2_rn(d[k], e[k]));
+                }
+                if (c == chunks) {
+                    if (sp != nullptr) {
+#pragma unroll
+                        for (int e = 0; e < 16; e += SV) st16(sp + o + e, pack16<ST>(&s[0].x + e));
+                    }
+                } else {
+                    tmem_st16(TS + o, s);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const uint32_t at = swz<Lay::kRow>(p, (first + o) / 8 + u);
+                        store_split8(s_hi + at, s_lo + at, s + 4 * u);
+                    }
+                }
             }
+            if (c == chunks) break;
+            tmem_wait_st();
+            const uint32_t kq = base + Lay::KQ + st * 32768;
             fence_async_smem();
             tc_fence_before();
-            named_sync(bar, 128);
-            if (p == 0) {
+            named_sync(bar, 256);
+            if (lead) {
                 mbar_wait(smem_addr(&sh.kq_full[st]), st_phase, &sh.abort);
                 tc_fence_after();
                 // [K;Q] S
-#pragma unroll
-                for (int ks = 0; ks < 8; ++ks)
-                    mma_bf16(D, operand(kq + (ks >> 2) * 16384 + (ks & 3) * 32, 16, 1024, kSwizzle128),
-                             operand(s_hi + ks * 2 * kGroup, Lay::kS, kGroup, kSwz),
-                             mma_desc(2 * VS, false, true), ks > 0);
+                const uint64_t k = operand(kq, 16, 1024, kSwizzle128), s = operand(s_hi, Lay::kS, kGroup, kSwz);
+                mma_steps(D, k, 2, s, kGroup / 8, 4, mma_desc(2 * VS, false, true), false);
+                mma_steps(D, k + 1024, 2, s + kGroup / 2, kGroup / 8, 4, mma_desc(2 * VS, false, true), true);
                 mma_commit(mma);
             }
             mbar_wait(smem_addr(&sh.vec_full[c & 1]), (c >> 1) & 1, &sh.abort);
-            const float in = vec[c & 1].in[p], decay = vec[c & 1].decay, out = vec[c & 1].out[p % C];
-            float o[VS];  // rows of Q: their outputs
+            const float in = vec[c & 1].in[p], out = vec[c & 1].out[p % C];
+            decay = vec[c & 1].decay;
+            float2 q[W / 2];  // rows of Q: their outputs
+            if (p < C) mbar_wait(smem_addr(&sh.v_full[grp]), c & 1, &sh.abort);
             mbar_wait(mma, phase, &sh.abort);
             phase ^= 1;
             tc_fence_after();
-            const uint32_t vb = base + Lay::V + (st * NG + grp) * Lay::kR;
-#pragma unroll
-            for (int g = 0; g < VS / 16; ++g) {
-                float d[16], e[16];
-                tmem_ld16x2(D + lanes + 16 * g, D + lanes + VS + 16 * g, d, e);
-                if (p < C) {
-                    // R = V - r e^b (K S)
+            if (p < C) {
+                // R = V - r e^b (K S), zero behind the sequence's end, whatever V holds there
+                const bool live = c * C + p < ntok;
+#pragma unroll 1
+                for (int o = 0; o < W; o += 16) {
+                    float2 d[8], e[8];
+                    tmem_ld16(Dh + o, Dl + o, d, e);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        float f[8];
-                        unpack16<bf16>(lds16(vb + swz<Lay::kRow>(p, 2 * g + u)), f);
+                        const uint32_t at = swz<Lay::kRow>(p, (first + o) / 8 + u);
+                        const uint4 v = lds16(vb + at);
+                        const uint32_t vv[4] = {v.x, v.y, v.z, v.w};
+                        float2 f[4];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) f[k] = fmaf(-in, d[8 * u + k] + e[8 * u + k], f[k]);
-                        const uint32_t at = swz<Lay::kRow>(p, 2 * g + u);
+                        for (int k = 0; k < 4; ++k)
+                            f[k] = __ffma2_rn(make_float2(-in, -in), __fadd2_rn(d[4 * u + k], e[4 * u + k]),
+                                              bf16_pair(live ? vv[k] : 0u));
                         store_split8(r_hi + at, r_lo + at, f);
                     }
-                } else {
+                }
+                fence_async_smem();
+            } else {
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) o[16 * g + k] = in * (d[k] + e[k]);
+                for (int o = 0; o < W; o += 16) {
+                    float2 d[8], e[8];
+                    tmem_ld16(Dh + o, Dl + o, d, e);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) q[o / 2 + k] = mul2(__fadd2_rn(d[k], e[k]), in);
                 }
             }
-            fence_async_smem();
             tc_fence_before();
-            named_sync(bar, 128);
-            if (p == 0) {
+            named_sync(bar, 256);
+            if (lead) {
+                if (c + 1 < chunks) load_v(c + 1, grp);
                 mbar_wait(smem_addr(&sh.tg_full), c & 1, &sh.abort);
                 tc_fence_after();
                 // [T;G] R: hi [hi | lo], then lo hi
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks)
-                    mma_bf16(D, operand(tg + ks * 32, 16, 1024, kSwizzle128),
-                             operand(r_hi + ks * 2 * kGroup, Lay::kR, kGroup, kSwz),
-                             mma_desc(2 * VS, false, true), ks > 0);
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks)
-                    mma_bf16(D, operand(tg + 16384 + ks * 32, 16, 1024, kSwizzle128),
-                             operand(r_hi + ks * 2 * kGroup, Lay::kR, kGroup, kSwz),
-                             mma_desc(VS, false, true), true);
+                const uint64_t r = operand(r_hi, Lay::kR, kGroup, kSwz);
+                mma_steps(D, operand(tg, 16, 1024, kSwizzle128), 2, r, kGroup / 8, 4, mma_desc(2 * VS, false, true), false);
+                mma_steps(D, operand(tg + 16384, 16, 1024, kSwizzle128), 2, r, kGroup / 8, 4, mma_desc(VS, false, true), true);
                 mma_commit(mma);
                 mma_commit(smem_addr(&sh.tg_free));
             }
             mbar_wait(mma, phase, &sh.abort);
             phase ^= 1;
             tc_fence_after();
+            if (p < C) {
+#pragma unroll 1
+                for (int o = 0; o < W; o += 16) {
+                    float2 d[8], e[8];
+                    tmem_ld16(Dh + o, Dl + o, d, e);
 #pragma unroll
-            for (int g = 0; g < VS / 16; ++g) {
-                float d[16], e[16];
-                tmem_ld16x2(D + lanes + 16 * g, D + lanes + VS + 16 * g, d, e);
-                if (p < C) {
+                    for (int k = 0; k < 8; ++k) d[k] = mul2(__fadd2_rn(d[k], e[k]), out);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        float f[8];
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) f[k] = out * (d[8 * u + k] + e[8 * u + k]);
-                        const uint32_t at = swz<Lay::kRow>(p, 2 * g + u);
-                        store_split8(u_hi + at, u_lo + at, f);
+                        const uint32_t at = swz<Lay::kRow>(p, (first + o) / 8 + u);
+                        store_split8(u_hi + at, u_lo + at, d + 4 * u);
                     }
-                } else {
+                }
+                fence_async_smem();
+            } else {
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) o[16 * g + k] += d[k] + e[k];
+                for (int o = 0; o < W; o += 16) {
+                    float2 d[8], e[8];
+                    tmem_ld16(Dh + o, Dl + o, d, e);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        q[o / 2 + k] = __fadd2_rn(q[o / 2 + k], __fadd2_rn(d[k], e[k]));
                 }
             }
-            fence_async_smem();
             tc_fence_before();
-            named_sync(bar, 128);
-            if (p == 0) {
+            named_sync(bar, 256);
+            if (lead) {
                 tc_fence_after();
                 // K^T u
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks)
-                    mma_bf16(D, operand(kq + ks * 2048, 16384, 1024, kSwizzle128),
-                             operand(u_hi + ks * 2 * kGroup, Lay::kR, kGroup, kSwz),
-                             mma_desc(2 * VS, true, true), ks > 0);
+                mma_steps(D, operand(kq, 16384, 1024, kSwizzle128), 128, operand(u_hi, Lay::kR, kGroup, kSwz),
+                          kGroup / 8, 4, mma_desc(2 * VS, true, true), false);
                 mma_commit(mma);
             }
             const int t = c * C + p - C;
             if (p >= C && t < ntok) {
                 bf16* to = op + (int64_t)t * a.o_st;
 #pragma unroll
-                for (int k = 0; k < VS; k += 16) {
-                    const uint4 lo = pack16<bf16>(o + k), hi = pack16<bf16>(o + k + 8);
+                for (int k = 0; k < W; k += 16) {
+                    const uint4 lo = pack16<bf16>(&q[k / 2].x), hi = pack16<bf16>(&q[k / 2 + 4].x);
                     if (out32) {
                         st32_stream(to + k, lo, hi);
                     } else {
@@ -693,29 +770,18 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
             mbar_wait(mma, phase, &sh.abort);
             phase ^= 1;
             tc_fence_after();
-            if (p == 0 && c + kStages < chunks) {
-                // The last scan warpgroup through with the chunk refills its stage.
+            if (lead && c + kStages < chunks) {
+                // The last scan group through with the chunk refills its stage.
                 __threadfence_block();
                 if (atomicAdd(&sh.done[st], 1) % NG == NG - 1) {
                     __threadfence_block();
-                    load(c + kStages, st);
+                    load_kq(c + kStages, st);
                 }
-            }
-#pragma unroll
-            for (int g = 0; g < VS / 16; ++g) {
-                float d[16], e[16];
-                tmem_ld16x2(D + lanes + 16 * g, D + lanes + VS + 16 * g, d, e);
-#pragma unroll
-                for (int k = 0; k < 16; ++k) S[16 * g + k] = fmaf(decay, S[16 * g + k], d[k] + e[k]);
             }
             if (++st == kStages) {
                 st = 0;
                 st_phase ^= 1;
             }
-        }
-        if (sp != nullptr) {
-#pragma unroll
-            for (int j = 0; j < VS; j += SV) st16(sp + j, pack16<ST>(S + j));
         }
     }
     tc_fence_before();

@@ -99,49 +99,55 @@ __device__ __forceinline__ void tc_fence_after() {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
 
-// 32 fp32 columns of the warp's 32 lanes: lane l of the warp gets row l. `tmem` carries the warp's
-// first lane in its upper half. 
-__device__ __forceinline__ void tmem_ld32(uint32_t tmem, float* f) {
-    uint32_t r[32];
-    __syncwarp();
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-          "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
-          "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(tmem)
-        : "memory");
-#pragma unroll
-    for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
-}
+// 16 fp32 columns of the warp's 32 lanes, from each of one, two or three places: lane l of the warp
+// gets row l. Addresses carry the warp's first lane in their upper half. The loads and their wait
+// are one statement, so that no use of the registers can come before it.
+#define CC1D_LD16(first, addr)                                                                \
+    "tcgen05.ld.sync.aligned.32x32b.x16.b32 {" first "}, [" addr "];\n\t"
+#define CC1D_16REGS(r)                                                                           \
+    "=f"((r)[0].x), "=f"((r)[0].y), "=f"((r)[1].x), "=f"((r)[1].y), "=f"((r)[2].x),              \
+        "=f"((r)[2].y), "=f"((r)[3].x), "=f"((r)[3].y), "=f"((r)[4].x), "=f"((r)[4].y),          \
+        "=f"((r)[5].x), "=f"((r)[5].y), "=f"((r)[6].x), "=f"((r)[6].y), "=f"((r)[7].x),          \
+        "=f"((r)[7].y)
+#define CC1D_R0 "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15"
+#define CC1D_R1 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31"
+#define CC1D_R2 "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47"
 
-// 16 columns from each of two places, as above.
-__device__ __forceinline__ void tmem_ld16x2(uint32_t t0, uint32_t t1, float* f, float* g) {
-    uint32_t r[16], s[16];
+__device__ __forceinline__ void tmem_ld16(uint32_t t0, float2* f) {
+    __syncwarp();
+    asm volatile(CC1D_LD16(CC1D_R0, "%16") "tcgen05.wait::ld.sync.aligned;"
+                 : CC1D_16REGS(f)
+                 : "r"(t0)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t t0, uint32_t t1, float2* f, float2* g) {
+    __syncwarp();
+    asm volatile(CC1D_LD16(CC1D_R0, "%32") CC1D_LD16(CC1D_R1, "%33") "tcgen05.wait::ld.sync.aligned;"
+                 : CC1D_16REGS(f), CC1D_16REGS(g)
+                 : "r"(t0), "r"(t1)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t t0, uint32_t t1, uint32_t t2, float2* f, float2* g,
+                                          float2* h) {
+    __syncwarp();
+    asm volatile(CC1D_LD16(CC1D_R0, "%48") CC1D_LD16(CC1D_R1, "%49") CC1D_LD16(CC1D_R2, "%50")
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : CC1D_16REGS(f), CC1D_16REGS(g), CC1D_16REGS(h)
+                 : "r"(t0), "r"(t1), "r"(t2)
+                 : "memory");
+}
+// The reverse; tmem_wait_st() before another load of the same columns.
+__device__ __forceinline__ void tmem_st16(uint32_t t0, const float2* f) {
     __syncwarp();
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n\t"
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-          "=r"(r[14]), "=r"(r[15]), "=r"(s[0]), "=r"(s[1]), "=r"(s[2]), "=r"(s[3]), "=r"(s[4]),
-          "=r"(s[5]), "=r"(s[6]), "=r"(s[7]), "=r"(s[8]), "=r"(s[9]), "=r"(s[10]), "=r"(s[11]),
-          "=r"(s[12]), "=r"(s[13]), "=r"(s[14]), "=r"(s[15])
-        : "r"(t0), "r"(t1)
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {" CC1D_R0 "};" ::"f"(f[0].x), "f"(f[0].y),
+        "f"(f[1].x), "f"(f[1].y), "f"(f[2].x), "f"(f[2].y), "f"(f[3].x), "f"(f[3].y), "f"(f[4].x),
+        "f"(f[4].y), "f"(f[5].x), "f"(f[5].y), "f"(f[6].x), "f"(f[6].y), "f"(f[7].x), "f"(f[7].y),
+        "r"(t0)
         : "memory");
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        f[i] = __uint_as_float(r[i]);
-        g[i] = __uint_as_float(s[i]);
-    }
+}
+__device__ __forceinline__ void tmem_wait_st() {
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
 // ------------------------------------------------------------------------------------------ MMA
@@ -172,6 +178,18 @@ __device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uin
         ::"r"(d), "l"(a), "l"(b), "r"(desc), "r"(accumulate ? 1u : 0u)
         : "memory");
 }
+// `steps` K steps, the operands' descriptors moving on by a_step and b_step 16-byte units. A loop
+// on purpose: the tensor core takes 46 cycles and more a step, and the code stays small.
+__device__ __forceinline__ void mma_steps(uint32_t d, uint64_t a, int a_step, uint64_t b, int b_step,
+                                          int steps, uint32_t desc, bool accumulate) {
+#pragma unroll 1
+    for (int i = 0; i < steps; ++i) {
+        mma_bf16(d, a, b, desc, accumulate);
+        a += a_step;
+        b += b_step;
+        accumulate = true;
+    }
+}
 // Arrive on the mbarrier when all MMAs this thread has issued so far are complete.
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile(
@@ -181,13 +199,13 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
 
 // ------------------------------------------------------------------------------- two-part bf16
 
-// (a, b) as bf16 pairs: hi rounds to nearest, lo rounds the rest, so that hi + lo is within 2^-17
-// of the value. Low halves hold a.
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(b), "f"(a));
-    const float ra = a - __uint_as_float(hi << 16);
-    const float rb = b - __uint_as_float(hi & 0xffff0000u);
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(rb), "f"(ra));
+// Two values as bf16 pairs: hi rounds to nearest, lo rounds the rest, so that hi + lo is within
+// 2^-17 of the value. The low halves hold f.x.
+__device__ __forceinline__ void split2(float2 f, uint32_t& hi, uint32_t& lo) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(f.y), "f"(f.x));
+    const float2 h = make_float2(__uint_as_float(hi << 16), __uint_as_float(hi & 0xffff0000u));
+    const float2 r = __ffma2_rn(h, make_float2(-1.f, -1.f), f);
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(r.y), "f"(r.x));
 }
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;

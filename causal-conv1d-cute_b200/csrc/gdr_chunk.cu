@@ -73,6 +73,12 @@ struct Layout {
 // P as a 128-row operand reads 8 KB behind its last row.
 static_assert(sizeof(Blocks) >= 8192, "");
 
+// What a chunk's gates give: cumulative log2 decays b, negated, in two parts each; rates; decays
+// e^(b_i), e^(b_C - b_j) and, below 32, e^(b_31 - b_j).
+struct Gates {
+    alignas(16) float nbh[C], nbl[C], beta[C], grow[C], out[C], far[32];
+};
+
 struct Shared {
     uint64_t kq_tma[3], kq_full[3], vec_full[2], v_full[2], tg_full, tg_free, prep_mma, scan_mma[2];
     uint32_t tmem;
@@ -80,8 +86,8 @@ struct Shared {
     int row;  // sequence of this CTA
     int done[3];  // per stage: scan groups that are through with its K and Q, over all chunks
     int len[kOrderMax];
-    alignas(16) float bh[C], bl[C], rk[C], ru[32], beta[C], qq[2][C];
-    double half;
+    alignas(16) float rk[C], ru[32], qq[2][2 * C];
+    Gates gates[2];
 };
 
 // Row r, 16-byte unit u of an operand image of ROW-byte rows.
@@ -151,47 +157,53 @@ __device__ __forceinline__ void merge_tile(const float (*inv1)[LPAD], const floa
                                            const float (*inv0)[LPAD], int r0, int c0, int lane,
                                            float (*d)[4]) {
     const int g = lane / 4, t2 = lane % 4 * 2;
-    float m[K / 8][4];  // (low inv0)^T: rows c0.., 8 columns (rows of low) each
+    // The two halves of a sum over 32 go to accumulators of their own: shorter chains of products.
+    float m[K / 16][K / 8][4];  // (low inv0)^T: rows c0.., 8 columns (rows of low) each
 #pragma unroll
-    for (int n = 0; n < K / 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) m[n][e] = 0.f;
-#pragma unroll
-    for (int k0 = 0; k0 < K; k0 += 16) {
+    for (int k = 0; k < K / 16; ++k) {
         uint32_t av[2][4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int col = c0 + g + e % 2 * 8, k = k0 + t2 + e / 2 * 8;
-            split2(make_float2(inv0[k][col], inv0[k + 1][col]), av[0][e], av[1][e]);
+            const int col = c0 + g + e % 2 * 8, r = 16 * k + t2 + e / 2 * 8;
+            split2(make_float2(inv0[r][col], inv0[r + 1][col]), av[0][e], av[1][e]);
         }
 #pragma unroll
         for (int n = 0; n < K / 8; ++n) {
             uint32_t bv[2][2];
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-                split2(*reinterpret_cast<const float2*>(&low[8 * n + g][k0 + t2 + 8 * e]), bv[0][e], bv[1][e]);
-            mma_warp3(m[n], av, bv);
+                split2(*reinterpret_cast<const float2*>(&low[8 * n + g][16 * k + t2 + 8 * e]), bv[0][e], bv[1][e]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m[k][n][e] = 0.f;
+            mma_warp3(m[k][n], av, bv);
+        }
+    }
+    float s[K / 16][2][4];
+#pragma unroll
+    for (int k = 0; k < K / 16; ++k) {
+        uint32_t av[2][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            split2(*reinterpret_cast<const float2*>(&inv1[r0 + g + e % 2 * 8][16 * k + t2 + e / 2 * 8]), av[0][e], av[1][e]);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            uint32_t bv[2][2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float2 f = make_float2(m[0][2 * k + e][2 * n], m[0][2 * k + e][2 * n + 1]);
+                if (K > 16)
+                    f = __fadd2_rn(f, make_float2(m[K / 16 - 1][2 * k + e][2 * n], m[K / 16 - 1][2 * k + e][2 * n + 1]));
+                split2(f, bv[0][e], bv[1][e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[k][n][e] = 0.f;
+            mma_warp3(s[k][n], av, bv);
         }
     }
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) d[n][e] = 0.f;
-#pragma unroll
-    for (int k0 = 0; k0 < K; k0 += 16) {
-        uint32_t av[2][4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            split2(*reinterpret_cast<const float2*>(&inv1[r0 + g + e % 2 * 8][k0 + t2 + e / 2 * 8]), av[0][e], av[1][e]);
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            uint32_t bv[2][2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-                split2(make_float2(m[k0 / 8 + e][2 * n], m[k0 / 8 + e][2 * n + 1]), bv[0][e], bv[1][e]);
-            mma_warp3(d[n], av, bv);
-        }
-    }
+        for (int e = 0; e < 4; ++e) d[n][e] = K > 16 ? s[0][n][e] + s[K / 16 - 1][n][e] : s[0][n][e];
 }
 
 // Bits of element i of a gate tensor, and its value: the load and its use can lie far apart.
@@ -302,10 +314,11 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
         constexpr int kPrep = 32 * Lay::kPrepWarps, kHalves = kPrep / 128;
         const int half0 = (warp - 8 * NG) / 4;
         const int i = p % C;
-        const bool gates = p < C && half0 == 0;  // threads that also keep a token's gates
+        const int pt = tid - 256 * NG;
+        const bool lead = pt == kPrep - 32;          // issues the products
+        const bool gate_warp = pt / 32 == kPrep / 32 - 4 + (kHalves == 1 ? 2 : 0);  // idle while others solve
         const uint32_t D0 = tmem;  // 64 columns of [K;Q] K^T; later 128 of P [T hi | T lo]
         const uint32_t pb = base + Lay::P;
-        const int64_t g0 = tok0 * a.g_st + h * a.g_sh, b0 = tok0 * a.b_st + h * a.b_sh;
         // T and P are zero above their diagonal blocks; nothing writes there again.
         if (p < 32 && half0 == 0) {
 #pragma unroll
@@ -316,44 +329,86 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
                 sts16(pb + 8192 + swz<128>(p, u), 0, 0, 0, 0);
             }
         }
+        // Gates of a chunk, by one warp, two tokens a lane. The raw values of the next chunk are
+        // loaded here a chunk before they are used.
         float rate = 0.f, dt = 0.f;
-        if (a.a_log != nullptr) {
-            rate = -expf(load_any(a.a_log, h, a.pdtype));
-            dt = load_any(a.dt_bias, h, a.pdtype);
-        }
-        uint32_t g_bits = 0, b_bits = 0;
+        uint32_t g_bits[2] = {0, 0}, b_bits[2] = {0, 0};
+        const int64_t g0 = tok0 * a.g_st + h * a.g_sh, b0 = tok0 * a.b_st + h * a.b_sh;
         auto load_gate_bits = [&](int c) {
-            const int64_t t = (int64_t)c * C + p;
-            if (gates && t < ntok) {
-                g_bits = load_bits(a.g, g0 + t * a.g_st, a.gdtype);
-                b_bits = load_bits(a.beta, b0 + t * a.b_st, a.bdtype);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int64_t t = (int64_t)c * C + 2 * lane + e;
+                if (t < ntok) {
+                    g_bits[e] = load_bits(a.g, g0 + t * a.g_st, a.gdtype);
+                    b_bits[e] = load_bits(a.beta, b0 + t * a.b_st, a.bdtype);
+                }
             }
         };
-        load_gate_bits(0);
+        auto make_gates = [&](int c) {
+            Gates& to = sh.gates[c & 1];
+            double sum[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float g = 0.f, beta = 0.f;
+                if (c * C + 2 * lane + e < ntok) {
+                    g = bits_value(g_bits[e], a.gdtype);
+                    beta = bits_value(b_bits[e], a.bdtype);
+                    if (a.a_log != nullptr) {
+                        const float z = g + dt;
+                        g = rate * (z > 20.f ? z : log1pf(expf(z)));
+                        beta = 1.f / (1.f + expf(-beta));
+                    }
+                    // -1e5 decays anything to zero, and its sums stay finite where -inf would give
+                    // inf - inf below.
+                    g = g < -1e5f ? -1e5f : g;
+                }
+                to.beta[2 * lane + e] = beta;
+                // The sums are carried in 64 bits and kept as two fp32 parts: their differences
+                // are exponents, where fp32 sums of strong decays would lose the weak ones.
+                sum[e] = (double)g * 1.4426950408889634;
+            }
+            load_gate_bits(c + 1);
+            sum[1] += sum[0];
+            double total = sum[1];
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const double below = __shfl_up_sync(~0u, total, o);
+                if (lane >= o) total += below;
+            }
+            const double mid = __shfl_sync(~0u, total, 15), end = __shfl_sync(~0u, total, 31);
+            const double b[2] = {total - sum[1] + sum[0], total};
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int t = 2 * lane + e;
+                const float hi = (float)b[e];
+                to.nbh[t] = -hi;
+                to.nbl[t] = (float)((double)hi - b[e]);
+                to.grow[t] = exp2_approx(hi);
+                to.out[t] = exp2_approx((float)(end - b[e]));
+                if (t < 32) to.far[t] = exp2_approx((float)(mid - b[e]));
+            }
+        };
+        if (gate_warp) {
+            if (a.a_log != nullptr) {
+                rate = -expf(load_any(a.a_log, h, a.pdtype));
+                dt = load_any(a.dt_bias, h, a.pdtype);
+            }
+            load_gate_bits(0);
+            make_gates(0);
+        }
 
         int st = 0;
         uint32_t st_phase = 0;
 #pragma unroll 1
         for (int c = 0; c < chunks; ++c) {
             Vectors& ve = vec[c & 1];
+            const Gates& ga = sh.gates[c & 1];
             const uint32_t kq = base + Lay::KQ + st * 32768;
             const int left = ntok - c * C;
-            // Gates of this chunk, bits of the next one's.
-            float g = 0.f, beta = 0.f;
-            if (gates && p < left) {
-                g = bits_value(g_bits, a.gdtype);
-                beta = bits_value(b_bits, a.bdtype);
-                if (a.a_log != nullptr) {
-                    const float z = g + dt;
-                    g = rate * (z > 20.f ? z : log1pf(expf(z)));
-                    beta = 1.f / (1.f + expf(-beta));
-                }
-            }
-            load_gate_bits(c + 1);
             mbar_wait(smem_addr(&sh.kq_tma[st]), st_phase, &sh.abort);
             if (left < C) {
                 // The copies went on into the next sequence: zeros there, whatever it holds.
-                for (int e = tid % kPrep; e < (C - left) * 32; e += kPrep) {
+                for (int e = pt; e < (C - left) * 32; e += kPrep) {
                     const int r = left + e / 32, u = e % 16;
                     sts16(kq + (u >> 3) * 16384 + swz<128>(r + (e & 16) * 4, u & 7), 0, 0, 0, 0);
                 }
@@ -361,98 +416,55 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
             }
             tc_fence_before();
             named_sync(8, kPrep);
-            if (tid % kPrep == 0) {
+            if (lead) {
                 mbar_arrive(smem_addr(&sh.kq_full[st]));
                 tc_fence_after();
                 const uint64_t d = operand(kq, 16, 1024, kSwizzle128);
-                mma_steps(D0, d, 2, d, 2, 4, mma_desc(64, false, false), false);
-                mma_steps(D0, d + 1024, 2, d + 1024, 2, 4, mma_desc(64, false, false), true);
+                mma_steps<4, 2, 2>(D0, d, d, mma_desc(64, false, false), false);
+                mma_steps<4, 2, 2>(D0, d + 1024, d + 1024, mma_desc(64, false, false), true);
                 mma_commit(smem_addr(&sh.prep_mma));
             }
-            // While it runs: cumulative decays (threads of K rows), query norms (Q rows).
-            double total = 0;
-            if (gates) {
-                // -1e5 decays anything to zero, and its sums stay finite where -inf would give
-                // inf - inf below.
-                g = g < -1e5f ? -1e5f : g;
-                // The sums are carried in 64 bits and kept as two fp32 parts: their differences
-                // are exponents, where fp32 sums of strong decays would lose the weak ones.
-                total = (double)g * 1.4426950408889634;
-#pragma unroll
-                for (int o = 1; o < 32; o *= 2) {
-                    const double below = __shfl_up_sync(~0u, total, o);
-                    if (lane >= o) total += below;
-                }
-                if (p == 31) sh.half = total;
-                sh.beta[p] = beta;
-            } else if (p >= C && a.l2norm) {
-                for (int hf = half0; hf < 2; hf += kHalves) {
-                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            // While it runs: the norms of its rows.
+            for (int hf = half0; hf < 2; hf += kHalves) {
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll 4
-                    for (int u = 0; u < 8; ++u) {
-                        const uint4 v = lds16(kq + hf * 16384 + swz<128>(p, u));
-                        const uint32_t vv[4] = {v.x, v.y, v.z, v.w};
+                for (int u = 0; u < 8; ++u) {
+                    const uint4 v = lds16(kq + hf * 16384 + swz<128>(p, u));
+                    const uint32_t vv[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float2 f = bf16_pair(vv[e]);
-                            sum[e % 2] = __ffma2_rn(f, f, sum[e % 2]);
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 f = bf16_pair(vv[e]);
+                        sum[e % 2] = __ffma2_rn(f, f, sum[e % 2]);
                     }
-                    sh.qq[hf][i] = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                }
+                sh.qq[hf][p] = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+            }
+            named_sync(8, kPrep);
+            const float norm = a.l2norm ? rsqrtf(sh.qq[0][p] + sh.qq[1][p] + kL2Eps) : 1.f;
+            const float mul = norm * (p < C ? ga.beta[i] : a.scale);  // of row i of L or P
+            if (half0 == 0) {
+                ve.in[p] = ga.grow[i] * (p < C ? norm : mul);
+                if (p < C) {
+                    sh.rk[p] = norm;
+                    ve.out[i] = norm * ga.out[i];
+                    if (p < 32) sh.ru[p] = norm * ga.far[p];
+                    if (i == C - 1) ve.decay = ga.grow[i];
                 }
             }
             named_sync(8, kPrep);
-            float far = 0.f;  // decay between token p and the middle of the chunk, for p < 32
-            if (gates) {
-                const double mid = sh.half;
-                if (p >= 32) total += mid;
-                const float hi = (float)total;
-                sh.bh[p] = hi;
-                sh.bl[p] = (float)(total - (double)hi);
-                far = exp2_approx((float)(mid - total));
-            }
+            if (pt == 0) mbar_arrive(smem_addr(&sh.vec_full[c & 1]));
             mbar_wait(smem_addr(&sh.prep_mma), 0, &sh.abort);
             tc_fence_after();
-            if (p < C && (w % 2 == half0 || kHalves == 1)) {
-                // |k_i|^2 is the diagonal of K K^T: element i % 16 of a group of 16 columns.
-                float d = 0.f;
-#pragma unroll
-                for (int o = 0; o < 32; o += 16) {
-                    float2 x[8];
-                    tmem_ld16(D0 + lanes + 32 * w + o, x);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        d = lane == o + 2 * e ? x[e].x : d;
-                        d = lane == o + 2 * e + 1 ? x[e].y : d;
-                    }
-                }
-                sh.rk[p] = a.l2norm ? rsqrtf(d + kL2Eps) : 1.f;
-            }
-            named_sync(8, kPrep);
             // Warps 0 and 1 make L (columns j < i) of rows of K K^T, warps 2 and 3 make P (columns
             // j <= i) of rows of Q K^T. In the columns of a row's own half the decay e^(b_i - b_j)
             // is taken element by element; for the lower left block it splits at the middle of the
             // chunk into two factors of at most 1.
-            const float bh = sh.bh[i], bl = sh.bl[i], rk = sh.rk[i];
-            const float mul = p < C ? sh.beta[i] * rk
-                                    : a.l2norm ? a.scale * rsqrtf(sh.qq[0][i] + sh.qq[1][i] + kL2Eps) : a.scale;
-            if (half0 == 0) {
-                const float grow = exp2_approx(bh + bl);
-                ve.in[p] = grow * (p < C ? rk : mul);
-                if (p < C) {
-                    ve.out[i] = rk * exp2_approx((sh.bh[C - 1] - bh) + (sh.bl[C - 1] - bl));
-                    if (p < 32) sh.ru[p] = rk * far;
-                    if (i == C - 1) ve.decay = grow;
-                }
-            }
-            // ru is used by other warps than its writers.
-            named_sync(8, kPrep);
-            if (tid % kPrep == 0) mbar_arrive(smem_addr(&sh.vec_full[c & 1]));
 #pragma unroll 1
             for (int hf = half0; hf < 2; hf += kHalves) {
                 if (hf > w % 2) continue;  // above the diagonal block
                 const bool own = hf == w % 2;
-                const float low_mul = mul * exp2_approx((bh - sh.bh[31]) + (bl - sh.bl[31]));
+                const float2 bh = make_float2(-ga.nbh[i], -ga.nbh[i]), bl = make_float2(-ga.nbl[i], -ga.nbl[i]);
+                const float low_mul = mul * exp2_approx((bh.x + ga.nbh[31]) + (bl.x + ga.nbl[31]));
                 const int last = (p < C ? i - 1 : i) - 32 * hf;  // last column of this half that counts
                 float (*to)[LPAD] = own ? blk.diag[w % 2] : blk.low;
 #pragma unroll 1
@@ -462,15 +474,23 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
                     if (own) {
 #pragma unroll
                         for (int e = 0; e < 8; e += 2) {
-                            const int j = 32 * hf + o + 2 * e;
-                            const float4 h4 = *reinterpret_cast<const float4*>(&sh.bh[j]);
-                            const float4 l4 = *reinterpret_cast<const float4*>(&sh.bl[j]);
+                            const int jj = o + 2 * e, j = 32 * hf + jj;
+                            const float4 h4 = *reinterpret_cast<const float4*>(&ga.nbh[j]);
+                            const float4 l4 = *reinterpret_cast<const float4*>(&ga.nbl[j]);
                             const float4 r4 = *reinterpret_cast<const float4*>(&sh.rk[j]);
-                            const int jj = o + 2 * e;
-                            x[e].x = jj <= last ? x[e].x * (mul * r4.x) * exp2_approx((bh - h4.x) + (bl - l4.x)) : 0.f;
-                            x[e].y = jj + 1 <= last ? x[e].y * (mul * r4.y) * exp2_approx((bh - h4.y) + (bl - l4.y)) : 0.f;
-                            x[e + 1].x = jj + 2 <= last ? x[e + 1].x * (mul * r4.z) * exp2_approx((bh - h4.z) + (bl - l4.z)) : 0.f;
-                            x[e + 1].y = jj + 3 <= last ? x[e + 1].y * (mul * r4.w) * exp2_approx((bh - h4.w) + (bl - l4.w)) : 0.f;
+                            const float2 e0 = __fadd2_rn(__fadd2_rn(bh, make_float2(h4.x, h4.y)),
+                                                         __fadd2_rn(bl, make_float2(l4.x, l4.y)));
+                            const float2 e1 = __fadd2_rn(__fadd2_rn(bh, make_float2(h4.z, h4.w)),
+                                                         __fadd2_rn(bl, make_float2(l4.z, l4.w)));
+                            x[e] = __fmul2_rn(__fmul2_rn(x[e], mul2(make_float2(r4.x, r4.y), mul)),
+                                              make_float2(exp2_approx(e0.x), exp2_approx(e0.y)));
+                            x[e + 1] = __fmul2_rn(__fmul2_rn(x[e + 1], mul2(make_float2(r4.z, r4.w), mul)),
+                                                  make_float2(exp2_approx(e1.x), exp2_approx(e1.y)));
+                            // Columns behind the last one: their decay may be inf, their value is 0.
+                            x[e].x = jj <= last ? x[e].x : 0.f;
+                            x[e].y = jj + 1 <= last ? x[e].y : 0.f;
+                            x[e + 1].x = jj + 2 <= last ? x[e + 1].x : 0.f;
+                            x[e + 1].y = jj + 3 <= last ? x[e + 1].y : 0.f;
                         }
                     } else {
 #pragma unroll
@@ -494,6 +514,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
                     }
                 }
             }
+            if (gate_warp && c + 1 < chunks) make_gates(c + 1);
             if (p < C && (w % 2 == half0 || kHalves == 1)) {
                 // Inverse of this warp's diagonal block: its two 16 x 16 blocks by substitution, a
                 // half warp each, then the block below them, -inv_1 (L_21 inv_0).
@@ -530,7 +551,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
                     const int col = fc + 8 * n;
-                    const float2 bt = make_float2(-sh.beta[col], -sh.beta[col + 1]);
+                    const float2 bt = make_float2(-ga.beta[col], -ga.beta[col + 1]);
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         uint32_t hi, lo;
@@ -547,7 +568,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
 #pragma unroll 1
                 for (int u = 0; u < 2; ++u) {
                     const float* from = &blk.diag[r / 32][r % 32][o + 8 * u];
-                    const float* bt = &sh.beta[r / 32 * 32 + o + 8 * u];
+                    const float* bt = &ga.beta[r / 32 * 32 + o + 8 * u];
                     float2 f[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
@@ -560,12 +581,12 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
             fence_async_smem();
             tc_fence_before();
             named_sync(8, kPrep);
-            if (tid % kPrep == 0) {
+            if (lead) {
                 tc_fence_after();
                 // G = P T in rows 0..63: hi [hi | lo], then lo hi. Rows 64.. are of no use.
                 const uint64_t t = operand(tg, 16384, 1024, kSwizzle128);
-                mma_steps(D0, operand(pb, 16, 1024, kSwizzle128), 2, t, 128, 4, mma_desc(128, false, true), false);
-                mma_steps(D0, operand(pb + 8192, 16, 1024, kSwizzle128), 2, t, 128, 4, mma_desc(64, false, true), true);
+                mma_steps<4, 2, 128>(D0, operand(pb, 16, 1024, kSwizzle128), t, mma_desc(128, false, true), false);
+                mma_steps<4, 2, 128>(D0, operand(pb + 8192, 16, 1024, kSwizzle128), t, mma_desc(64, false, true), true);
                 mma_commit(smem_addr(&sh.prep_mma));
             }
             mbar_wait(smem_addr(&sh.prep_mma), 1, &sh.abort);
@@ -587,7 +608,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
             }
             tc_fence_before();
             named_sync(8, kPrep);
-            if (tid % kPrep == 0) mbar_arrive(smem_addr(&sh.tg_full));
+            if (pt == 0) mbar_arrive(smem_addr(&sh.tg_full));
             if (++st == kStages) {
                 st = 0;
                 st_phase ^= 1;
@@ -662,8 +683,8 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
                 tc_fence_after();
                 // [K;Q] S
                 const uint64_t k = operand(kq, 16, 1024, kSwizzle128), s = operand(s_hi, Lay::kS, kGroup, kSwz);
-                mma_steps(D, k, 2, s, kGroup / 8, 4, mma_desc(2 * VS, false, true), false);
-                mma_steps(D, k + 1024, 2, s + kGroup / 2, kGroup / 8, 4, mma_desc(2 * VS, false, true), true);
+                mma_steps<4, 2, kGroup / 8>(D, k, s, mma_desc(2 * VS, false, true), false);
+                mma_steps<4, 2, kGroup / 8>(D, k + 1024, s + kGroup / 2, mma_desc(2 * VS, false, true), true);
                 mma_commit(mma);
             }
             mbar_wait(smem_addr(&sh.vec_full[c & 1]), (c >> 1) & 1, &sh.abort);
@@ -712,8 +733,8 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
                 tc_fence_after();
                 // [T;G] R: hi [hi | lo], then lo hi
                 const uint64_t r = operand(r_hi, Lay::kR, kGroup, kSwz);
-                mma_steps(D, operand(tg, 16, 1024, kSwizzle128), 2, r, kGroup / 8, 4, mma_desc(2 * VS, false, true), false);
-                mma_steps(D, operand(tg + 16384, 16, 1024, kSwizzle128), 2, r, kGroup / 8, 4, mma_desc(VS, false, true), true);
+                mma_steps<4, 2, kGroup / 8>(D, operand(tg, 16, 1024, kSwizzle128), r, mma_desc(2 * VS, false, true), false);
+                mma_steps<4, 2, kGroup / 8>(D, operand(tg + 16384, 16, 1024, kSwizzle128), r, mma_desc(VS, false, true), true);
                 mma_commit(mma);
                 mma_commit(smem_addr(&sh.tg_free));
             }
@@ -749,8 +770,9 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
             if (lead) {
                 tc_fence_after();
                 // K^T u
-                mma_steps(D, operand(kq, 16384, 1024, kSwizzle128), 128, operand(u_hi, Lay::kR, kGroup, kSwz),
-                          kGroup / 8, 4, mma_desc(2 * VS, true, true), false);
+                mma_steps<4, 128, kGroup / 8>(D, operand(kq, 16384, 1024, kSwizzle128),
+                                              operand(u_hi, Lay::kR, kGroup, kSwz),
+                                              mma_desc(2 * VS, true, true), false);
                 mma_commit(mma);
             }
             const int t = c * C + p - C;

@@ -40,6 +40,7 @@ SIGNATURES = {
                     _p, _p, _p, _i64, _i64, _i64, _i64, _i32, _i64, _i32, _i32, _i32, _p, _p],
     "cc1d_update_unpack": [_p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _i32,
                            _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _p],
+    "cc1d_gdr_workspace": [_p, _p],
     "cc1d_gdr_update": [_p, _p],
     "cc1d_gdr_varlen": [_p, _p],
     "cc1d_rms_norm_gated": [_p, _p],
@@ -50,7 +51,7 @@ SIGNATURES = {
 
 # Argument blocks (cc1d_gdr_args, cc1d_norm_args) are packed by struct in one call, which costs the
 # host less than setting the fields of a ctypes structure: pointers, then int64, int32 and float.
-GDR_ARGS = struct.Struct("15P33q13if")
+GDR_ARGS = struct.Struct("16P34q13if")
 NORM_ARGS = struct.Struct("4P9q2if4x")
 
 EXPORTS = ("cc1d_abi_version", "cc1d_status_string", "cc1d_last_error", *SIGNATURES)

@@ -14,6 +14,8 @@ outside the state cache, sequence bounds outside the packed tokens). device_stat
 clears it. Checks are off by default so that no call allocates anything.
 """
 
+import ctypes
+
 import torch
 
 from . import _lib
@@ -217,7 +219,7 @@ def _update_unpack_impl(qkvz, ba, state, weight, bias, out, z, b, a, idx, heads,
 
 
 def _gdr_args(q, k, v, g, beta, a_log, dt_bias, out, states, inter, idx, iidx, qsl, hinit, rows,
-              tokens, steps, scale, l2norm, update, pad):
+              tokens, steps, scale, l2norm, update, pad, workspace=None):
     """The packed cc1d_gdr_args; the token-major tensors are (rows, steps, ...) or (tokens, ...)."""
     zero = (0,) if q.dim() == 3 else ()
     ss, nslots = ((0, 0, 0), 0) if states is None else (states.stride()[:3], states.shape[0])
@@ -229,10 +231,10 @@ def _gdr_args(q, k, v, g, beta, a_log, dt_bias, out, states, inter, idx, iidx, q
         0 if inter is None else inter.data_ptr(),
         0 if idx is None else idx.data_ptr(), 0 if iidx is None else iidx.data_ptr(),
         0 if qsl is None else qsl.data_ptr(), 0 if hinit is None else hinit.data_ptr(),
-        _status_ptr(q.device) or 0,
+        _status_ptr(q.device) or 0, 0 if workspace is None else workspace.data_ptr(),
         *zero, *q.stride(), *zero, *k.stride(), *zero, *v.stride(), *zero, *out.stride(),
         *zero, *g.stride(), *zero, *beta.stride(), *ss, *si,
-        rows, tokens, nslots, ni,
+        rows, tokens, nslots, ni, 0 if workspace is None else workspace.numel(),
         steps, q.shape[-2], v.shape[-2], q.shape[-1], v.shape[-1],
         dtype_code(q.dtype), dtype_code(g.dtype), dtype_code(beta.dtype),
         F32 if a_log is None else dtype_code(a_log.dtype),
@@ -255,9 +257,15 @@ def _gdr_update_impl(q, k, v, g, beta, a_log, dt_bias, out, states, idx, inter, 
 def _gdr_varlen_impl(q, k, v, g, beta, a_log, dt_bias, out, states, qsl, idx, hinit, scale,
                      l2norm, pad):
     """Gated delta rule over packed sequences (cc1d_gdr_varlen): (tokens, heads, dim)."""
-    args = _gdr_args(q, k, v, g, beta, a_log, dt_bias, out, states, None, idx, None, qsl, hinit,
-                     qsl.numel() - 1, q.shape[0], 0, scale, l2norm, True, pad)
-    check(load().cc1d_gdr_varlen(args, _stream(q.device)))
+    lib = load()
+    call = (q, k, v, g, beta, a_log, dt_bias, out, states, None, idx, None, qsl, hinit,
+            qsl.numel() - 1, q.shape[0], 0, scale, l2norm, True, pad)
+    args, need = _gdr_args(*call), ctypes.c_int64()
+    check(lib.cc1d_gdr_workspace(args, ctypes.byref(need)))
+    if need.value:
+        # From the caching allocator, on the current stream: reused by the stream's later work only.
+        args = _gdr_args(*call, torch.empty(need.value, dtype=torch.uint8, device=q.device))
+    check(lib.cc1d_gdr_varlen(args, _stream(q.device)))
 
 
 def _rms_norm_gated_impl(x, z, weight, eps, out):

@@ -352,6 +352,15 @@ cc1d_status_t cc1d_update_unpack(const void* qkvz, int64_t q_sb, const void* ba,
                      "cc1d_update_unpack");
 }
 
+cc1d_status_t cc1d_gdr_workspace(const cc1d_gdr_args* args, int64_t* bytes) {
+    if (args == nullptr || bytes == nullptr) return fail(CC1D_ERR_INVALID, "a required pointer is NULL");
+    if (cc1d_status_t s = check_gdr(*args)) return s;
+    *bytes = args->rows > 0 && args->tokens > 0 && cc1d::gdr_chunk_serves(*args)
+                 ? cc1d::gdr_chunk_workspace(*args)
+                 : 0;
+    return ok();
+}
+
 cc1d_status_t cc1d_gdr_update(const cc1d_gdr_args* args, void* stream) {
     if (args == nullptr) return fail(CC1D_ERR_INVALID, "args is NULL");
     const cc1d_gdr_args& a = *args;
@@ -380,7 +389,10 @@ cc1d_status_t cc1d_gdr_varlen(const cc1d_gdr_args* args, void* stream) {
         return fail(CC1D_ERR_INVALID, "%lld slots for %lld sequences without indices",
                     (long long)a.nslots, (long long)a.rows);
     if (cc1d_status_t s = bind_stream(stream)) return s;
-    return from_cuda(cc1d::gdr_chunk_serves(a)
+    const bool chunked = a.workspace != nullptr && (uintptr_t)a.workspace % 128 == 0 &&
+                         cc1d::gdr_chunk_serves(a) &&
+                         a.workspace_bytes >= cc1d::gdr_chunk_workspace(a);
+    return from_cuda(chunked
                          ? cc1d::launch_gdr_chunk(a, (cudaStream_t)stream)
                          : cc1d::launch_gdr_recurrent(a, true, (cudaStream_t)stream),
                      "cc1d_gdr_varlen");

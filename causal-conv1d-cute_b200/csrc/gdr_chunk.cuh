@@ -1,0 +1,67 @@
+// What the two kernels of the chunked gated delta rule share: the image of a chunk in the workspace,
+// operand images in shared memory, tensor maps.
+#pragma once
+
+#include "gdr.cuh"
+#include "kernels.h"
+#include "tc05.cuh"
+
+namespace cc1d {
+
+constexpr int C = 64;    // tokens per chunk
+constexpr int DK = 128;  // key head dim
+
+// What the prep kernel leaves of a chunk and value head for the scan kernel.
+struct ChunkImage {
+    unsigned char tg[2][128 * 128];  // [T;G], hi and lo bf16 parts, 128-byte rows, swizzled
+    float in[2 * C];                 // r_i e^(b_i) (rows of K), s_i e^(b_i) (rows of Q)
+    float out[C];                    // r_j e^(b_C - b_j)
+    float decay;                     // e^(b_C)
+    float pad[3];
+};
+constexpr int kVectorBytes = (int)sizeof(ChunkImage) - 32768;  // what follows tg
+
+// Image slots: the chunks of sequence n start at slot floor(first token / 64) + n, which leaves
+// every sequence room for its chunks without a prefix sum over the lengths.
+__device__ __forceinline__ int64_t chunk_base(int64_t first_token, int64_t n) {
+    return first_token / C + n;
+}
+__host__ __device__ inline int64_t chunk_slots(int64_t tokens, int64_t rows) {
+    return tokens / C + rows;
+}
+
+// Row r, 16-byte unit u of an operand image of ROW-byte rows.
+template <int ROW>
+__device__ __forceinline__ uint32_t swz(int r, int u) {
+    if constexpr (ROW == 128) {
+        return r * 128 + ((u ^ (r & 7)) << 4);
+    } else {
+        return r * 64 + ((u ^ ((r >> 1) & 3)) << 4);
+    }
+}
+
+// 8 values as two bf16 parts, one 16-byte unit each.
+__device__ __forceinline__ void store_split8(uint32_t hi, uint32_t lo, const float2* f) {
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) split2(f[i], h[i], l[i]);
+    sts16(hi, h[0], h[1], h[2], h[3]);
+    sts16(lo, l[0], l[1], l[2], l[3]);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float b) {
+    return __fmul2_rn(a, make_float2(b, b));
+}
+__device__ __forceinline__ float2 bf16_pair(uint32_t v) {
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+
+// One box (cols x 64 tokens of a head) of the tensor map of a (tokens, heads, dim) bf16 view.
+bool make_map(CUtensorMap* map, const void* p, int64_t tokens, int heads, int dim, int64_t st,
+              int64_t sh, int cols);
+// Whether the driver offers tensor maps.
+bool have_maps();
+
+cudaError_t launch_gdr_prep(const cc1d_gdr_args& a, const CUtensorMap& q, const CUtensorMap& k,
+                            cudaStream_t stream);
+
+}  // namespace cc1d

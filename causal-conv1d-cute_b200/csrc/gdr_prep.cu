@@ -1,0 +1,507 @@
+// Gated delta rule in chunks, first kernel: everything of a chunk that does not depend on the state.
+// gdr_chunk.cu has the mathematics; here, per chunk of 64 tokens and value head,
+//     L_ij = beta_i r_i r_j e^(b_i - b_j) k_i.k_j  (j < i),   T = (I + L)^-1 diag(beta),
+//     P_ij = s_i r_j e^(b_i - b_j) q_i.k_j         (j <= i),  G = P T,
+// and the row factors of the scan. The chunks are independent, so latency is hidden by four CTAs
+// per SM rather than inside one.
+//
+// A CTA of four warps takes one chunk of one query/key head: K and Q by TMA, [K;Q] K^T on the tensor
+// core and the norms once, then the value heads of the group one after another. The inverse goes in
+// blocks: 16 x 16 by substitution in registers (a lane owns a row, rows of L come as broadcasts),
+// the blocks below the diagonal by -inv_1 (L_21 inv_0) in two-part bf16 on the warp-level tensor
+// core (120 dependent fp32 steps a row instead of the 2016 of plain substitution). G is a product on
+// the tensor core again. T leaves by a bulk copy, G from registers.
+//
+// Bound: instruction issue and latency (about 2200 warp instructions per chunk and value head) next
+// to 33.6 KB written.
+#include "gdr_chunk.cuh"
+
+namespace cc1d {
+namespace {
+
+constexpr int LPAD = 36;  // fp32 row of a 32 x 32 block: 16-byte accesses of 8 rows hit 8 bank groups
+constexpr int kHeads = 4;  // value heads whose gates are made at a time, one warp each
+
+// I + L in 32 x 32 blocks, fp32: the diagonal blocks (L, then their inverses in place) and the
+// block below them.
+struct Blocks {
+    float diag[2][32][LPAD], low[32][LPAD];
+};
+// P as a 128-row operand reads 8 KB behind its last row.
+static_assert(sizeof(Blocks) >= 8192, "");
+
+// What a chunk's gates give: cumulative log2 decays b, negated, in two parts each; rates; decays
+// e^(b_i), e^(b_C - b_j) and, below 32, e^(b_31 - b_j).
+struct Gates {
+    alignas(16) float nbh[C], nbl[C], beta[C], grow[C], out[C], far[32];
+};
+
+struct Smem {
+    unsigned char kq[32768];  // [2 halves][K 64 rows, Q 64 rows][128 B]; later T hi, T lo, P hi, P lo
+    Blocks blk;
+    Gates gates[kHeads];
+    alignas(16) float rk[C], ru[C];
+    uint64_t full, mma;
+    uint32_t tmem;
+    int abort, seq;
+};
+
+// Row i of the inverse of I + l (l strictly lower triangular, 16 x 16, zeros above) by backward
+// substitution: y_m is final once every later y has been taken out of it, and is then taken out of
+// the earlier ones along row m of l. A lane owns a row; the rows of l come as broadcasts.
+__device__ __forceinline__ void solve_row16(const float (*l)[LPAD], int i, float2* y) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) y[q] = make_float2(i == 2 * q ? 1.f : 0.f, i == 2 * q + 1 ? 1.f : 0.f);
+#pragma unroll
+    for (int m = 15; m > 0; --m) {
+        const float v = -(m % 2 ? y[m / 2].y : y[m / 2].x);
+        const float2 vv = make_float2(v, v);
+#pragma unroll
+        for (int r = 0; r < m; r += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(&l[m][r]);
+            y[r / 2] = __ffma2_rn(make_float2(f.x, f.y), vv, y[r / 2]);
+            if (r + 2 < m) y[r / 2 + 1] = __ffma2_rn(make_float2(f.z, f.w), vv, y[r / 2 + 1]);
+        }
+    }
+}
+
+// d (16 x 8) += a (16 x 16) b (16 x 8), bf16 operands, fp32 sums, within a warp.
+__device__ __forceinline__ void mma_warp(float* d, const uint32_t* a, const uint32_t* b) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+__device__ __forceinline__ void mma_warp3(float* d, const uint32_t (*a)[4], const uint32_t (*b)[2]) {
+    mma_warp(d, a[0], b[0]);
+    mma_warp(d, a[0], b[1]);
+    mma_warp(d, a[1], b[0]);
+}
+
+// The 16 x 16 tile inv1[r0.., :] (low inv0)[:, c0..] of a product of K x K matrices, K = 16 or 32,
+// by one warp in two-part bf16. The inner product is formed transposed, (inv0^T low^T): its
+// accumulator fragments are then the B fragments of the outer one. d: accumulators of columns c0..
+// and c0 + 8...
+template <int K>
+__device__ __forceinline__ void merge_tile(const float (*inv1)[LPAD], const float (*low)[LPAD],
+                                           const float (*inv0)[LPAD], int r0, int c0, int lane,
+                                           float (*d)[4]) {
+    const int g = lane / 4, t2 = lane % 4 * 2;
+    // The two halves of a sum over 32 go to accumulators of their own: shorter chains of products.
+    float m[K / 16][K / 8][4];  // (low inv0)^T: rows c0.., 8 columns (rows of low) each
+#pragma unroll
+    for (int k = 0; k < K / 16; ++k) {
+        uint32_t av[2][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int col = c0 + g + e % 2 * 8, r = 16 * k + t2 + e / 2 * 8;
+            split2(make_float2(inv0[r][col], inv0[r + 1][col]), av[0][e], av[1][e]);
+        }
+#pragma unroll
+        for (int n = 0; n < K / 8; ++n) {
+            uint32_t bv[2][2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                split2(*reinterpret_cast<const float2*>(&low[8 * n + g][16 * k + t2 + 8 * e]), bv[0][e], bv[1][e]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m[k][n][e] = 0.f;
+            mma_warp3(m[k][n], av, bv);
+        }
+    }
+    float s[K / 16][2][4];
+#pragma unroll
+    for (int k = 0; k < K / 16; ++k) {
+        uint32_t av[2][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            split2(*reinterpret_cast<const float2*>(&inv1[r0 + g + e % 2 * 8][16 * k + t2 + e / 2 * 8]), av[0][e], av[1][e]);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            uint32_t bv[2][2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float2 f = make_float2(m[0][2 * k + e][2 * n], m[0][2 * k + e][2 * n + 1]);
+                if (K > 16)
+                    f = __fadd2_rn(f, make_float2(m[K / 16 - 1][2 * k + e][2 * n], m[K / 16 - 1][2 * k + e][2 * n + 1]));
+                split2(f, bv[0][e], bv[1][e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[k][n][e] = 0.f;
+            mma_warp3(s[k][n], av, bv);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[n][e] = K > 16 ? s[0][n][e] + s[K / 16 - 1][n][e] : s[0][n][e];
+}
+
+// Bits of element i of a gate tensor, and its value: the load and its use can lie far apart.
+__device__ __forceinline__ uint32_t load_bits(const void* p, int64_t i, int dtype) {
+    return dtype == CC1D_F32 ? static_cast<const uint32_t*>(p)[i] : static_cast<const uint16_t*>(p)[i];
+}
+__device__ __forceinline__ float bits_value(uint32_t b, int dtype) {
+    if (dtype == CC1D_BF16) return __uint_as_float(b << 16);
+    if (dtype == CC1D_F16) return __half2float(__ushort_as_half((unsigned short)b));
+    return __uint_as_float(b);
+}
+
+__global__ void __launch_bounds__(128, 4)
+gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__ CUtensorMap mapq,
+                const __grid_constant__ CUtensorMap mapk) {
+    extern __shared__ __align__(1024) unsigned char raw[];
+    Smem& sh = *reinterpret_cast<Smem*>(raw + ((1024 - (smem_addr(raw) & 1023)) & 1023));
+    const uint32_t kq = smem_addr(sh.kq), tb = kq, pb = kq + 16384;
+    const int p = threadIdx.x, w = p / 32, lane = p % 32, i = p % C;
+    const int hk = blockIdx.x % a.heads_k;
+    const int64_t image = blockIdx.x / a.heads_k;
+
+    // The sequence whose chunk this is.
+    if (p == 0) sh.seq = -1;
+    __syncthreads();
+    for (int64_t n = p; n < a.rows; n += 128) {
+        const int64_t t0 = a.query_start_loc[n], t1 = a.query_start_loc[n + 1];
+        if (t0 < 0 || t1 <= t0 || t1 > a.tokens) continue;
+        const int64_t first = chunk_base(t0, n);
+        if (image >= first && image < first + (t1 - t0 + C - 1) / C) sh.seq = (int)n;
+    }
+    __syncthreads();
+    const int64_t row = sh.seq;
+    int64_t tok0, slot;
+    int ntok;
+    if (row < 0 || !gdr_row(a, true, row, tok0, ntok, slot, false)) return;
+    const int c = (int)(image - chunk_base(tok0, row));
+    tok0 += c * C;
+    const int left = ntok - c * C;
+
+    if (p == 0) {
+        mbar_init(smem_addr(&sh.full), 1);
+        mbar_init(smem_addr(&sh.mma), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        sh.abort = 0;
+    }
+    if (w == 0) {
+        tmem_alloc(smem_addr(&sh.tmem), 128);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t D0 = sh.tmem, DG = D0 + 64;  // [K;Q] K^T; G
+    const uint32_t lanes = (uint32_t)w << 21;   // the warp's first TMEM lane, in bits 16..
+    if (p == 0) {
+        const uint32_t full = smem_addr(&sh.full);
+        mbar_expect(full, 32768);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            tma_load(kq + half * 16384, &mapk, half * 64, hk, (int)tok0, full);
+            tma_load(kq + half * 16384 + 8192, &mapq, half * 64, hk, (int)tok0, full);
+        }
+    }
+
+    // Gates of one value head by one warp, two tokens a lane.
+    const int group = a.heads_v / a.heads_k;
+    auto make_gates = [&](int h, Gates& to) {
+        float rate = 0.f, dt = 0.f;
+        if (a.a_log != nullptr) {
+            rate = -expf(load_any(a.a_log, h, a.pdtype));
+            dt = load_any(a.dt_bias, h, a.pdtype);
+        }
+        uint32_t g_bits[2] = {0, 0}, b_bits[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int64_t t = tok0 + 2 * lane + e;
+            if (2 * lane + e < left) {
+                g_bits[e] = load_bits(a.g, t * a.g_st + h * a.g_sh, a.gdtype);
+                b_bits[e] = load_bits(a.beta, t * a.b_st + h * a.b_sh, a.bdtype);
+            }
+        }
+        double sum[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float g = 0.f, beta = 0.f;
+            if (2 * lane + e < left) {
+                g = bits_value(g_bits[e], a.gdtype);
+                beta = bits_value(b_bits[e], a.bdtype);
+                if (a.a_log != nullptr) {
+                    const float z = g + dt;
+                    g = rate * (z > 20.f ? z : log1pf(expf(z)));
+                    beta = 1.f / (1.f + expf(-beta));
+                }
+                // -1e5 decays anything to zero, and its sums stay finite where -inf would give
+                // inf - inf below.
+                g = g < -1e5f ? -1e5f : g;
+            }
+            to.beta[2 * lane + e] = beta;
+            // The sums are carried in 64 bits and kept as two fp32 parts: their differences are
+            // exponents, where fp32 sums of strong decays would lose the weak ones.
+            sum[e] = (double)g * 1.4426950408889634;
+        }
+        sum[1] += sum[0];
+        double total = sum[1];
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const double below = __shfl_up_sync(~0u, total, o);
+            if (lane >= o) total += below;
+        }
+        const double mid = __shfl_sync(~0u, total, 15), end = __shfl_sync(~0u, total, 31);
+        const double b[2] = {total - sum[1] + sum[0], total};
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int t = 2 * lane + e;
+            const float hi = (float)b[e];
+            to.nbh[t] = -hi;
+            to.nbl[t] = (float)((double)hi - b[e]);
+            to.grow[t] = exp2_approx(hi);
+            to.out[t] = exp2_approx((float)(end - b[e]));
+            if (t < 32) to.far[t] = exp2_approx((float)(mid - b[e]));
+        }
+    };
+    if (w < group) make_gates(hk * group + w, sh.gates[w]);
+
+    mbar_wait(smem_addr(&sh.full), 0, &sh.abort);
+    if (left < C) {
+        // The copies went on into the next sequence: zeros there, whatever it holds.
+        for (int e = p; e < (C - left) * 32; e += 128) {
+            const int r = left + e / 32, u = e % 16;
+            sts16(kq + (u >> 3) * 16384 + swz<128>(r + (e & 16) * 4, u & 7), 0, 0, 0, 0);
+        }
+        fence_async_smem();
+    }
+    __syncthreads();
+    uint32_t phase = 0;
+    if (p == 0) {
+        tc_fence_after();
+        const uint64_t d = operand(kq, 16, 1024, kSwizzle128);
+        mma_steps<4, 2, 2>(D0, d, d, mma_desc(64, false, false), false);
+        mma_steps<4, 2, 2>(D0, d + 1024, d + 1024, mma_desc(64, false, false), true);
+        mma_commit(smem_addr(&sh.mma));
+    }
+    // Norm of row p of [K;Q].
+    float norm = 1.f;
+    if (a.l2norm) {
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll 4
+        for (int u = 0; u < 16; ++u) {
+            const uint4 v = lds16(kq + (u >> 3) * 16384 + swz<128>(p, u & 7));
+            const uint32_t vv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = bf16_pair(vv[e]);
+                sum[e % 2] = __ffma2_rn(f, f, sum[e % 2]);
+            }
+        }
+        norm = rsqrtf((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y) + kL2Eps);
+    }
+    if (p < C) sh.rk[p] = norm;
+    mbar_wait(smem_addr(&sh.mma), phase, &sh.abort);
+    phase ^= 1;
+    __syncthreads();
+    // K and Q are through; T and P are zero above their diagonal blocks from here on.
+    if (p < 32) {
+#pragma unroll
+        for (int u = 4; u < 8; ++u) {
+#pragma unroll
+            for (int m = 0; m < 4; ++m) sts16(kq + m * 8192 + swz<128>(p, u), 0, 0, 0, 0);
+        }
+    }
+
+    Blocks& blk = sh.blk;
+#pragma unroll 1
+    for (int v = 0; v < group; ++v) {
+        const int h = hk * group + v;
+        if (v > 0 && v % kHeads == 0) {
+            __syncthreads();
+            if (v + w < group) make_gates(h + w, sh.gates[w]);
+            __syncthreads();
+        }
+        const Gates& ga = sh.gates[v % kHeads];
+        ChunkImage* out = static_cast<ChunkImage*>(a.workspace) + image * a.heads_v + h;
+        const float mul = norm * (p < C ? ga.beta[i] : a.scale);  // of row i of L or P
+        out->in[p] = ga.grow[i] * (p < C ? norm : mul);
+        if (p < C) out->out[i] = norm * ga.out[i];
+        if (p == C - 1) out->decay = ga.grow[i];
+        if (p < 32) sh.ru[p] = norm * ga.far[p];
+        __syncthreads();
+        tc_fence_after();
+        // Warps 0 and 1 make L (columns j < i) of rows of K K^T, warps 2 and 3 make P (columns
+        // j <= i) of rows of Q K^T. In the columns of a row's own half the decay e^(b_i - b_j) is
+        // taken element by element; for the lower left block it splits at the middle of the chunk
+        // into two factors of at most 1.
+        const float2 bh = make_float2(-ga.nbh[i], -ga.nbh[i]), bl = make_float2(-ga.nbl[i], -ga.nbl[i]);
+        const float low_mul = mul * exp2_approx((bh.x + ga.nbh[31]) + (bl.x + ga.nbl[31]));
+#pragma unroll 1
+        for (int hf = 0; hf <= w % 2; ++hf) {
+            const bool own = hf == w % 2;
+            const int last = (p < C ? i - 1 : i) - 32 * hf;  // last column of this half that counts
+            float (*to)[LPAD] = own ? blk.diag[w % 2] : blk.low;
+#pragma unroll 1
+            for (int o = 0; o < 32; o += 16) {
+                float2 x[8];
+                tmem_ld16(D0 + lanes + 32 * hf + o, x);
+                if (own) {
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        const int jj = o + 2 * e, j = 32 * hf + jj;
+                        const float4 h4 = *reinterpret_cast<const float4*>(&ga.nbh[j]);
+                        const float4 l4 = *reinterpret_cast<const float4*>(&ga.nbl[j]);
+                        const float4 r4 = *reinterpret_cast<const float4*>(&sh.rk[j]);
+                        const float2 e0 = __fadd2_rn(__fadd2_rn(bh, make_float2(h4.x, h4.y)),
+                                                     __fadd2_rn(bl, make_float2(l4.x, l4.y)));
+                        const float2 e1 = __fadd2_rn(__fadd2_rn(bh, make_float2(h4.z, h4.w)),
+                                                     __fadd2_rn(bl, make_float2(l4.z, l4.w)));
+                        x[e] = __fmul2_rn(__fmul2_rn(x[e], mul2(make_float2(r4.x, r4.y), mul)),
+                                          make_float2(exp2_approx(e0.x), exp2_approx(e0.y)));
+                        x[e + 1] = __fmul2_rn(__fmul2_rn(x[e + 1], mul2(make_float2(r4.z, r4.w), mul)),
+                                              make_float2(exp2_approx(e1.x), exp2_approx(e1.y)));
+                        // Columns behind the last one: their decay may be inf, their value is 0.
+                        x[e].x = jj <= last ? x[e].x : 0.f;
+                        x[e].y = jj + 1 <= last ? x[e].y : 0.f;
+                        x[e + 1].x = jj + 2 <= last ? x[e + 1].x : 0.f;
+                        x[e + 1].y = jj + 3 <= last ? x[e + 1].y : 0.f;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        const float4 r4 = *reinterpret_cast<const float4*>(&sh.ru[o + 2 * e]);
+                        x[e] = __fmul2_rn(x[e], mul2(make_float2(r4.x, r4.y), low_mul));
+                        x[e + 1] = __fmul2_rn(x[e + 1], mul2(make_float2(r4.z, r4.w), low_mul));
+                    }
+                }
+                if (p < C) {
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2)
+                        *reinterpret_cast<float4*>(&to[lane][o + 2 * e]) =
+                            make_float4(x[e].x, x[e].y, x[e + 1].x, x[e + 1].y);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const uint32_t at = pb + swz<128>(i, 4 * hf + o / 8 + u);
+                        store_split8(at, at + 8192, x + 4 * u);
+                    }
+                }
+            }
+        }
+        if (p < C) {
+            // Inverse of this warp's diagonal block: its two 16 x 16 blocks by substitution, a half
+            // warp each, then the block below them, -inv_1 (L_21 inv_0).
+            float (*dg)[LPAD] = blk.diag[w];
+            const int b = lane & 16;
+            float2 y[8];
+            __syncwarp();
+            solve_row16(reinterpret_cast<const float (*)[LPAD]>(&dg[b][b]), lane & 15, y);
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < 8; e += 2)
+                *reinterpret_cast<float4*>(&dg[lane][b + 2 * e]) =
+                    make_float4(y[e].x, y[e].y, y[e + 1].x, y[e + 1].y);
+            __syncwarp();
+            float d[2][4];
+            merge_tile<16>(reinterpret_cast<const float (*)[LPAD]>(&dg[16][16]),
+                           reinterpret_cast<const float (*)[LPAD]>(&dg[16][0]), dg, 0, 0, lane, d);
+            __syncwarp();
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    *reinterpret_cast<float2*>(&dg[16 + lane / 4 + 8 * e][8 * n + lane % 4 * 2]) =
+                        make_float2(-d[n][2 * e], -d[n][2 * e + 1]);
+        }
+        // The bulk copies of the T before have read it.
+        if (p == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncthreads();
+        {
+            // The 32 x 32 block below the diagonal ones, a 16 x 16 tile per warp.
+            const int r0 = w / 2 * 16, c0 = w % 2 * 16, fr = r0 + lane / 4, fc = c0 + lane % 4 * 2;
+            float d[2][4];
+            merge_tile<32>(blk.diag[1], blk.low, blk.diag[0], r0, c0, lane, d);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const int col = fc + 8 * n;
+                const float2 bt = make_float2(-ga.beta[col], -ga.beta[col + 1]);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    uint32_t hi, lo;
+                    split2(__fmul2_rn(make_float2(d[n][2 * e], d[n][2 * e + 1]), bt), hi, lo);
+                    const uint32_t at = tb + swz<128>(32 + fr + 8 * e, col / 8) + col % 8 * 2;
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(hi) : "memory");
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + 8192), "r"(lo) : "memory");
+                }
+            }
+            // The diagonal blocks: row p / 2, half of its 32 columns.
+            const int r = p / 2, o = p % 2 * 16;
+#pragma unroll 1
+            for (int u = 0; u < 2; ++u) {
+                const float* from = &blk.diag[r / 32][r % 32][o + 8 * u];
+                const float* bt = &ga.beta[r / 32 * 32 + o + 8 * u];
+                float2 f[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    f[e] = __fmul2_rn(*reinterpret_cast<const float2*>(from + 2 * e),
+                                      *reinterpret_cast<const float2*>(bt + 2 * e));
+                const uint32_t at = tb + swz<128>(r, r / 32 * 4 + o / 8 + u);
+                store_split8(at, at + 8192, f);
+            }
+        }
+        fence_async_smem();
+        tc_fence_before();
+        __syncthreads();
+        if (p == 0) {
+            tc_fence_after();
+            // G = P T in rows 0..63: hi hi, hi lo, lo hi. Rows 64.. are of no use.
+            const uint64_t P = operand(pb, 16, 1024, kSwizzle128), T = operand(tb, 16384, 1024, kSwizzle128);
+            mma_steps<4, 2, 128>(DG, P, T, mma_desc(64, false, true), false);
+            mma_steps<4, 2, 128>(DG, P, T + 512, mma_desc(64, false, true), true);
+            mma_steps<4, 2, 128>(DG, P + 512, T, mma_desc(64, false, true), true);
+            mma_commit(smem_addr(&sh.mma));
+#pragma unroll
+            for (int part = 0; part < 2; ++part)
+                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], 8192;" ::"l"(
+                                 out->tg[part]), "r"(tb + part * 8192)
+                             : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+        mbar_wait(smem_addr(&sh.mma), phase, &sh.abort);
+        phase ^= 1;
+        tc_fence_after();
+        if (p < C) {
+#pragma unroll 1
+            for (int o = 0; o < C; o += 16) {
+                float2 x[8];
+                tmem_ld16(DG + lanes + o, x);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) split2(x[4 * u + e], hi[e], lo[e]);
+                    const uint32_t at = swz<128>(C + p, o / 8 + u);
+                    st16(out->tg[0] + at, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+                    st16(out->tg[1] + at, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+                }
+            }
+        }
+        tc_fence_before();
+    }
+    if (p == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncthreads();
+    tc_fence_after();
+    if (w == 0) tmem_dealloc(sh.tmem, 128);
+    if (p == 0 && sh.abort) flag_status(a.dev_status, CC1D_DEV_TIMEOUT);
+}
+
+}  // namespace
+
+cudaError_t launch_gdr_prep(const cc1d_gdr_args& a, const CUtensorMap& q, const CUtensorMap& k,
+                            cudaStream_t stream) {
+    constexpr int smem = (int)sizeof(Smem) + 1024;
+    const cudaError_t err =
+        cudaFuncSetAttribute(gdr_prep_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (err != cudaSuccess) return err;
+    const int64_t grid = chunk_slots(a.tokens, a.rows) * a.heads_k;
+    if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
+    gdr_prep_kernel<<<(unsigned)grid, 128, smem, stream>>>(a, q, k);
+    return cudaGetLastError();
+}
+
+}  // namespace cc1d

@@ -140,6 +140,7 @@ cudaError_t launch_unpack(const UnpackArgs& a, int width, int dtype, cudaStream_
 cudaError_t launch_gdr_recurrent(const cc1d_gdr_args& a, bool varlen, cudaStream_t stream);
 // Packed prefill chunk by chunk on the tensor cores, where it serves the types and layout.
 bool gdr_chunk_serves(const cc1d_gdr_args& a);
+int64_t gdr_chunk_workspace(const cc1d_gdr_args& a);
 cudaError_t launch_gdr_chunk(const cc1d_gdr_args& a, cudaStream_t stream);
 cudaError_t launch_norm(const cc1d_norm_args& a, cudaStream_t stream);
 // same: the table's src and dst are the same caches (a source may be an earlier destination).

@@ -246,15 +246,24 @@ typedef struct {
     const int32_t *indices, *inter_indices, *query_start_loc;
     const uint8_t* has_initial_state;
     int32_t* dev_status;
+    void* workspace;
     int64_t q_sb, q_st, q_sh, q_sd, k_sb, k_st, k_sh, k_sd, v_sb, v_st, v_sh, v_sd;
     int64_t o_sb, o_st, o_sh, o_sd, g_sb, g_st, g_sh, b_sb, b_st, b_sh;
     int64_t s_slot, s_sh, s_sk, i_slot, i_st, i_sh, i_sk;
-    int64_t rows, tokens, nslots, inter_nslots;
+    int64_t rows, tokens, nslots, inter_nslots, workspace_bytes;
     int32_t steps, heads_k, heads_v, dk, dv;
     int32_t dtype, gdtype, bdtype, pdtype, sdtype; /* q k v out | g | beta | a_log dt_bias | states */
     int32_t l2norm, update_states, pad;
     float scale;
 } cc1d_gdr_args;
+
+/*
+ * Bytes of workspace (128-byte aligned) with which cc1d_gdr_varlen runs chunk by chunk on the
+ * tensor cores; 0 where it does not (other types or layouts, short sequences). It depends on the
+ * sizes, strides, pointers' alignment and types of args alone. With less, or NULL, the call runs token
+ * by token. The workspace holds nothing between calls.
+ */
+cc1d_status_t cc1d_gdr_workspace(const cc1d_gdr_args* args, int64_t* bytes);
 
 cc1d_status_t cc1d_gdr_update(const cc1d_gdr_args* args, void* stream);
 cc1d_status_t cc1d_gdr_varlen(const cc1d_gdr_args* args, void* stream);

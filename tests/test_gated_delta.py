@@ -186,8 +186,8 @@ def test_c_abi_refuses_before_launch():
         """An argument block with made-up pointers; everything refused here is refused on the host."""
         f = dict(dict(states=1, nslots=4, rows=2, tokens=8, steps=1, hk=2, hv=4, dk=16, dv=16, dtype=2, sdtype=2,
                       a_log=0, dt=0, q=1, inter=0), **kw)
-        return _lib.GDR_ARGS.pack(f["q"], 1, 1, 1, 1, f["a_log"], f["dt"], 1, f["states"], f["inter"], 0, 0, 1, 0, 0,
-                                  *[0] * 29, f["rows"], f["tokens"], f["nslots"], 0, f["steps"], f["hk"], f["hv"],
+        return _lib.GDR_ARGS.pack(f["q"], 1, 1, 1, 1, f["a_log"], f["dt"], 1, f["states"], f["inter"], 0, 0, 1, 0, 0, 0,
+                                  *[0] * 29, f["rows"], f["tokens"], f["nslots"], 0, 0, f["steps"], f["hk"], f["hv"],
                                   f["dk"], f["dv"], f["dtype"], 2, 2, 2, f["sdtype"], 0, 1, -1, 1.0)
 
     up, var = lib.cc1d_gdr_update, lib.cc1d_gdr_varlen

@@ -182,22 +182,29 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
         int st = 0;
         uint32_t phase = 0, st_phase = 0;
         float decay = 0.f;
+        mbar_wait(smem_addr(&sh.full[0]), 0, &sh.abort);
 #pragma unroll 1
         for (int c = 0;; ++c) {
             // The state after the chunk before, into TMEM, and as an operand if there is another.
-#pragma unroll 1
-            for (int o = 0; o < W; o += 16) {
+#pragma unroll
+            for (int g = 0; g < W / 16; ++g) {
                 float2 s[8];
                 if (c == 0) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) s[e] = make_float2(0.f, 0.f);
+                    for (int k = 0; k < 8; ++k) s[k] = make_float2(0.f, 0.f);
                     if (initial) {
 #pragma unroll
-                        for (int e = 0; e < 16; e += SV) unpack16<ST>(ld16(sp + o + e), &s[0].x + e);
+                        for (int k = 0; k < 16; k += SV) unpack16<ST>(ld16(sp + 16 * g + k), &s[0].x + k);
                     }
                 } else {
                     float2 d[8], e[8];
-                    tmem_ld16(Dh + o, Dl + o, TS + o, d, e, s);
+                    tmem_ld16_async(Dh + 16 * g, d);
+                    tmem_ld16_async(Dl + 16 * g, e);
+                    tmem_ld16_async(TS + 16 * g, s);
+                    tmem_wait_ld();
+                    tmem_ready(d);
+                    tmem_ready(e);
+                    tmem_ready(s);
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
                         s[k] = __ffma2_rn(make_float2(decay, decay), s[k], __fadd2_rn(d[k], e[k]));
@@ -205,13 +212,13 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
                 if (c == chunks) {
                     if (sp != nullptr) {
 #pragma unroll
-                        for (int e = 0; e < 16; e += SV) st16(sp + o + e, pack16<ST>(&s[0].x + e));
+                        for (int k = 0; k < 16; k += SV) st16(sp + 16 * g + k, pack16<ST>(&s[0].x + k));
                     }
                 } else {
-                    tmem_st16(TS + o, s);
+                    tmem_st16(TS + 16 * g, s);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const uint32_t at = swz<Lay::kRow>(p, (first + o) / 8 + u);
+                        const uint32_t at = swz<Lay::kRow>(p, first / 8 + 2 * g + u);
                         store_split8(s_hi + at, s_lo + at, s + 4 * u);
                     }
                 }
@@ -223,14 +230,12 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
             if (left < C) {
                 // The copies of K went on into the next sequence: zeros there, whatever it holds
                 // (rows of Q there make outputs that are not stored).
-                mbar_wait(smem_addr(&sh.full[st]), st_phase, &sh.abort);
                 for (int e = tid % 256; e < (C - left) * 16; e += 256)
                     sts16(kq + (e % 16 >> 3) * 16384 + swz<128>(left + e / 16, e % 8), 0, 0, 0, 0);
             }
             fence_async_smem();
             tc_fence_before();
             named_sync(bar, 256);
-            mbar_wait(smem_addr(&sh.full[st]), st_phase, &sh.abort);
             if (lead) {
                 tc_fence_after();
                 // [K;Q] S
@@ -238,6 +243,16 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
                 mma_steps<4, 2, kGroup / 8>(D, k, s, mma_desc(2 * VS, false, true), false);
                 mma_steps<4, 2, kGroup / 8>(D, k + 1024, s + kGroup / 2, mma_desc(2 * VS, false, true), true);
                 mma_commit(mma);
+                // While it runs: the last scan group through with the chunk before refills its
+                // stage.
+                if (c > 0 && c - 1 + kStages < chunks) {
+                    const int before = st > 0 ? st - 1 : kStages - 1;
+                    __threadfence_block();
+                    if (atomicAdd(&sh.done[before], 1) % NG == NG - 1) {
+                        __threadfence_block();
+                        load(c - 1 + kStages, before);
+                    }
+                }
             }
             const float in = vec[st].in[p], out = vec[st].out[p % C];
             decay = vec[st].decay;
@@ -246,73 +261,89 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
             mbar_wait(mma, phase, &sh.abort);
             phase ^= 1;
             tc_fence_after();
-            if (p < C) {
-                // R = V - r e^b (K S), zero behind the sequence's end, whatever V holds there
-                const bool live = c * C + p < ntok;
-#pragma unroll 1
-                for (int o = 0; o < W; o += 16) {
-                    float2 d[8], e[8];
-                    tmem_ld16(Dh + o, Dl + o, d, e);
+            {
+                float2 d[W / 16][8], e[W / 16][8];
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const uint32_t at = swz<Lay::kRow>(p, (first + o) / 8 + u);
-                        const uint4 v = lds16(vb + at);
-                        const uint32_t vv[4] = {v.x, v.y, v.z, v.w};
-                        float2 f[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            f[k] = __ffma2_rn(make_float2(-in, -in), __fadd2_rn(d[4 * u + k], e[4 * u + k]),
-                                              bf16_pair(live ? vv[k] : 0u));
-                        store_split8(r_hi + at, r_lo + at, f);
-                    }
+                for (int g = 0; g < W / 16; ++g) {
+                    tmem_ld16_async(Dh + 16 * g, d[g]);
+                    tmem_ld16_async(Dl + 16 * g, e[g]);
                 }
-                fence_async_smem();
-            } else {
+                if (p < C) {
+                    // R = V - r e^b (K S), zero behind the sequence's end, whatever V holds there
+                    const bool live = p < left;
+                    uint4 v[W / 8];
 #pragma unroll
-                for (int o = 0; o < W; o += 16) {
-                    float2 d[8], e[8];
-                    tmem_ld16(Dh + o, Dl + o, d, e);
+                    for (int u = 0; u < W / 8; ++u) v[u] = lds16(vb + swz<Lay::kRow>(p, first / 8 + u));
+                    tmem_wait_ld();
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) q[o / 2 + k] = mul2(__fadd2_rn(d[k], e[k]), in);
+                    for (int g = 0; g < W / 16; ++g) {
+                        tmem_ready(d[g]);
+                        tmem_ready(e[g]);
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const uint32_t vv[4] = {v[2 * g + u].x, v[2 * g + u].y, v[2 * g + u].z, v[2 * g + u].w};
+                            float2 f[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                f[k] = __ffma2_rn(make_float2(-in, -in), __fadd2_rn(d[g][4 * u + k], e[g][4 * u + k]),
+                                                  bf16_pair(live ? vv[k] : 0u));
+                            const uint32_t at = swz<Lay::kRow>(p, first / 8 + 2 * g + u);
+                            store_split8(r_hi + at, r_lo + at, f);
+                        }
+                    }
+                    fence_async_smem();
+                } else {
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int g = 0; g < W / 16; ++g) {
+                        tmem_ready(d[g]);
+                        tmem_ready(e[g]);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) q[8 * g + k] = mul2(__fadd2_rn(d[g][k], e[g][k]), in);
+                    }
                 }
             }
             tc_fence_before();
             named_sync(bar, 256);
             if (lead) {
-                if (c + 1 < chunks) load_v(c + 1, grp);
                 tc_fence_after();
                 // [T;G] R: hi [hi | lo], then lo hi
                 const uint64_t r = operand(r_hi, Lay::kR, kGroup, kSwz);
                 mma_steps<4, 2, kGroup / 8>(D, operand(tg, 16, 1024, kSwizzle128), r, mma_desc(2 * VS, false, true), false);
                 mma_steps<4, 2, kGroup / 8>(D, operand(tg + 16384, 16, 1024, kSwizzle128), r, mma_desc(VS, false, true), true);
                 mma_commit(mma);
+                if (c + 1 < chunks) load_v(c + 1, grp);
             }
             mbar_wait(mma, phase, &sh.abort);
             phase ^= 1;
             tc_fence_after();
-            if (p < C) {
-#pragma unroll 1
-                for (int o = 0; o < W; o += 16) {
-                    float2 d[8], e[8];
-                    tmem_ld16(Dh + o, Dl + o, d, e);
+            {
+                float2 d[W / 16][8], e[W / 16][8];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) d[k] = mul2(__fadd2_rn(d[k], e[k]), out);
+                for (int g = 0; g < W / 16; ++g) {
+                    tmem_ld16_async(Dh + 16 * g, d[g]);
+                    tmem_ld16_async(Dl + 16 * g, e[g]);
+                }
+                tmem_wait_ld();
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const uint32_t at = swz<Lay::kRow>(p, (first + o) / 8 + u);
-                        store_split8(u_hi + at, u_lo + at, d + 4 * u);
+                for (int g = 0; g < W / 16; ++g) {
+                    tmem_ready(d[g]);
+                    tmem_ready(e[g]);
+                    if (p < C) {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) d[g][k] = mul2(__fadd2_rn(d[g][k], e[g][k]), out);
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const uint32_t at = swz<Lay::kRow>(p, first / 8 + 2 * g + u);
+                            store_split8(u_hi + at, u_lo + at, d[g] + 4 * u);
+                        }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            q[8 * g + k] = __fadd2_rn(q[8 * g + k], __fadd2_rn(d[g][k], e[g][k]));
                     }
                 }
-                fence_async_smem();
-            } else {
-#pragma unroll
-                for (int o = 0; o < W; o += 16) {
-                    float2 d[8], e[8];
-                    tmem_ld16(Dh + o, Dl + o, d, e);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        q[o / 2 + k] = __fadd2_rn(q[o / 2 + k], __fadd2_rn(d[k], e[k]));
-                }
+                if (p < C) fence_async_smem();
             }
             tc_fence_before();
             named_sync(bar, 256);
@@ -338,21 +369,15 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
                     }
                 }
             }
-            mbar_wait(mma, phase, &sh.abort);
-            phase ^= 1;
-            tc_fence_after();
-            if (lead && c + kStages < chunks) {
-                // The last scan group through with the chunk refills its stage.
-                __threadfence_block();
-                if (atomicAdd(&sh.done[st], 1) % NG == NG - 1) {
-                    __threadfence_block();
-                    load(c + kStages, st);
-                }
-            }
             if (++st == kStages) {
                 st = 0;
                 st_phase ^= 1;
             }
+            // The next chunk's K, Q, T, G: there by now, and the look costs less here.
+            if (c + 1 < chunks) mbar_wait(smem_addr(&sh.full[st]), st_phase, &sh.abort);
+            mbar_wait(mma, phase, &sh.abort);
+            phase ^= 1;
+            tc_fence_after();
         }
     }
     tc_fence_before();

@@ -107,9 +107,9 @@ __device__ __forceinline__ void tc_fence_after() {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
 
-// 16 fp32 columns of the warp's 32 lanes, from each of one, two or three places: lane l of the warp
-// gets row l. Addresses carry the warp's first lane in their upper half. The loads and their wait
-// are one statement, so that no use of the registers can come before it.
+// 16 fp32 columns of the warp's 32 lanes: lane l of the warp gets row l. The address carries the
+// warp's first lane in its upper half. The load and its wait are one statement, so that no use of
+// the registers can come before it.
 #define CC1D_LD16(first, addr)                                                                \
     "tcgen05.ld.sync.aligned.32x32b.x16.b32 {" first "}, [" addr "];\n\t"
 #define CC1D_16REGS(r)                                                                           \
@@ -118,8 +118,6 @@ __device__ __forceinline__ void tc_fence_after() {
         "=f"((r)[5].x), "=f"((r)[5].y), "=f"((r)[6].x), "=f"((r)[6].y), "=f"((r)[7].x),          \
         "=f"((r)[7].y)
 #define CC1D_R0 "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15"
-#define CC1D_R1 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31"
-#define CC1D_R2 "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47"
 
 __device__ __forceinline__ void tmem_ld16(uint32_t t0, float2* f) {
     __syncwarp();
@@ -128,21 +126,18 @@ __device__ __forceinline__ void tmem_ld16(uint32_t t0, float2* f) {
                  : "r"(t0)
                  : "memory");
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t t0, uint32_t t1, float2* f, float2* g) {
+// The same without the wait: after tmem_wait_ld() and tmem_ready() of each the values may be used.
+__device__ __forceinline__ void tmem_ld16_async(uint32_t t0, float2* f) {
     __syncwarp();
-    asm volatile(CC1D_LD16(CC1D_R0, "%32") CC1D_LD16(CC1D_R1, "%33") "tcgen05.wait::ld.sync.aligned;"
-                 : CC1D_16REGS(f), CC1D_16REGS(g)
-                 : "r"(t0), "r"(t1)
-                 : "memory");
+    asm volatile(CC1D_LD16(CC1D_R0, "%16") : CC1D_16REGS(f) : "r"(t0) : "memory");
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t t0, uint32_t t1, uint32_t t2, float2* f, float2* g,
-                                          float2* h) {
-    __syncwarp();
-    asm volatile(CC1D_LD16(CC1D_R0, "%48") CC1D_LD16(CC1D_R1, "%49") CC1D_LD16(CC1D_R2, "%50")
-                 "tcgen05.wait::ld.sync.aligned;"
-                 : CC1D_16REGS(f), CC1D_16REGS(g), CC1D_16REGS(h)
-                 : "r"(t0), "r"(t1), "r"(t2)
-                 : "memory");
+__device__ __forceinline__ void tmem_wait_ld() {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// Keeps uses of the registers behind the wait that stands before it.
+__device__ __forceinline__ void tmem_ready(float2* f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) asm volatile("" : "+f"(f[i].x), "+f"(f[i].y));
 }
 // The reverse; tmem_wait_st() before another load of the same columns.
 __device__ __forceinline__ void tmem_st16(uint32_t t0, const float2* f) {

@@ -21,9 +21,9 @@
 // chunk and head. (One kernel with warps for either part was tried first: a chunk's T and G take
 // longer than its step of the chain, and shared memory has no room for more of them in flight.)
 // The kernel here walks the chain: [K;Q] S0, R, [T;G] R, u, K^T u, S. A CTA takes one head of one
-// sequence and NG tiles of VS state columns, each with a group of 256 threads (two per row); two
-// chains in a CTA fill each other's waits and share K, Q, T and G, which come by TMA and bulk copies
-// a chunk or two ahead. The state lies in TMEM.
+// sequence and VS state columns; K, Q, T and G come by TMA and bulk copies a chunk or two ahead. The
+// state lies in TMEM. (Two chains of 64 columns in one CTA took 7700 cycles a chunk and one of 128
+// columns takes XXXX: tensor memory serves the products of one and the loads of the other in turn.)
 // Stacking K over Q and T over G makes every product M = 128, the full tensor core rate; the two
 // parts of an operand lie side by side as one operand of 2 VS columns (measured: a K step of 16
 // costs 46 cycles up to 64 columns and 66 with 128, so one wide step beats two narrow ones).
@@ -36,20 +36,21 @@ namespace {
 
 constexpr int kOrderMax = 256;  // batches up to this many sequences start with the longest
 
-template <int VS, int NG>
+template <int VS>
 struct Layout {
-    static constexpr int kRow = VS >= 64 ? 128 : 2 * VS;  // bytes of an operand row of VS columns
-    static constexpr int kS = 128 * kRow;                 // one part (hi or lo) of S
-    static constexpr int kR = C * kRow;                   // one part of R or u, or one tile of V
-    static constexpr int kStages = VS * NG <= 32 ? 3 : 2;
+    static constexpr int kRow = VS >= 64 ? 128 : 2 * VS;  // bytes of a row of an operand's column atom
+    static constexpr int kAtoms = VS >= 64 ? VS / 64 : 1;
+    static constexpr int kS = 128 * kRow * kAtoms;        // one part (hi or lo) of S
+    static constexpr int kR = C * kRow * kAtoms;          // one part of R or u, or V
+    static constexpr int kStages = VS <= 32 ? 3 : 2;
     static constexpr int KQ = 0;                          // stages x [2 halves][128 rows][128 B]
     static constexpr int TG = KQ + kStages * 32768;       // stages x [hi, lo][128 rows][128 B]
-    static constexpr int SB = TG + kStages * 32768;       // NG x (S hi, S lo); R in S hi, u in S lo
-    static constexpr int V = SB + NG * 2 * kS;            // NG x [64 rows]
-    static constexpr int VEC = V + NG * kR;               // stages x row factors
+    static constexpr int SB = TG + kStages * 32768;       // S hi, S lo; R in S hi, u in S lo
+    static constexpr int V = SB + 2 * kS;                 // [atoms][64 rows]
+    static constexpr int VEC = V + kR;                    // stages x row factors
     static constexpr int END = VEC + kStages * kVectorBytes;
-    static constexpr int kTmem = NG * 3 * VS <= 128 ? 128 : NG * 3 * VS <= 256 ? 256 : 512;
-    static constexpr int kThreads = 256 * NG;
+    static constexpr int kTmem = VS == 32 ? 128 : VS == 64 ? 256 : 512;  // of 3 VS columns
+    static constexpr int kThreads = VS == 128 ? 512 : 256;
 };
 
 // The row factors of a ChunkImage, as they follow its T and G.
@@ -59,19 +60,28 @@ struct Vectors {
 static_assert(sizeof(Vectors) == kVectorBytes, "");
 
 struct Shared {
-    uint64_t full[3], v_full[2], scan_mma[2];
+    uint64_t full[3], v_full, mma;
     uint32_t tmem;
     int abort;
-    int row;      // sequence of this CTA
-    int done[3];  // per stage: scan groups that are through with it, over all chunks
+    int row;  // sequence of this CTA
 };
 
-template <typename ST, int VS, int NG>
-__global__ void __launch_bounds__(Layout<VS, NG>::kThreads, 1)
+// Row r, unit u of a row of columns whose 64-column atoms lie `rows` rows apart.
+template <int VS>
+__device__ __forceinline__ uint32_t swz_cols(int rows, int r, int u) {
+    if constexpr (VS > 64) {
+        return (u >> 3) * rows * 128 + swz<128>(r, u & 7);
+    } else {
+        return swz<Layout<VS>::kRow>(r, u);
+    }
+}
+
+template <typename ST, int VS>
+__global__ void __launch_bounds__(Layout<VS>::kThreads, 1)
 gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__ CUtensorMap mapq,
                  const __grid_constant__ CUtensorMap mapk, const __grid_constant__ CUtensorMap mapv,
                  int tiles, bool out32) {
-    using Lay = Layout<VS, NG>;
+    using Lay = Layout<VS>;
     constexpr uint64_t kSwz = VS >= 64 ? kSwizzle128 : kSwizzle64;
     constexpr uint32_t kGroup = 8 * Lay::kRow;  // bytes of eight rows of V columns
     constexpr int kStages = Lay::kStages;
@@ -82,7 +92,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
     const Vectors* vec = reinterpret_cast<const Vectors*>(gen + Lay::VEC);
 
     const int tid = threadIdx.x, warp = tid / 32, p = tid % 128, w = warp % 4;
-    const int vt = blockIdx.x % tiles;  // columns vt * NG * VS ..
+    const int vt = blockIdx.x % tiles;  // columns vt * VS ..
     const int h = (int)((blockIdx.x / tiles) % a.heads_v);
     int64_t row = blockIdx.x / tiles / a.heads_v;
     const int hk = h / (a.heads_v / a.heads_k);
@@ -110,14 +120,9 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
         static_cast<const ChunkImage*>(a.workspace) + chunk_base(tok0, row) * a.heads_v + h;
 
     if (tid == 0) {
-        for (int i = 0; i < 3; ++i) {
-            mbar_init(smem_addr(&sh.full[i]), 1);
-            sh.done[i] = 0;
-        }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(smem_addr(&sh.v_full[i]), 1);
-            mbar_init(smem_addr(&sh.scan_mma[i]), 1);
-        }
+        for (int i = 0; i < 3; ++i) mbar_init(smem_addr(&sh.full[i]), 1);
+        mbar_init(smem_addr(&sh.v_full), 1);
+        mbar_init(smem_addr(&sh.mma), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         sh.abort = 0;
     }
@@ -147,238 +152,239 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
         bulk_load(base + Lay::VEC + st * kVectorBytes, from->in, kVectorBytes, full);
         bulk_load(base + Lay::TG + st * 32768, from->tg, 32768, full);
     };
-    // V of chunk c for scan group g.
-    auto load_v = [&](int c, int g) {
-        const uint32_t full = smem_addr(&sh.v_full[g]);
+    // V of chunk c.
+    auto load_v = [&](int c) {
+        const uint32_t full = smem_addr(&sh.v_full);
         mbar_expect(full, C * VS * 2);
-        tma_load(base + Lay::V + g * Lay::kR, &mapv, (vt * NG + g) * VS, h, (int)tok0 + c * C, full);
+#pragma unroll
+        for (int at = 0; at < Lay::kAtoms; ++at)
+            tma_load(base + Lay::V + at * C * Lay::kRow, &mapv, vt * VS + at * 64, h, (int)tok0 + c * C, full);
     };
     if (tid == 0) {
         for (int c = 0; c < kStages && c < chunks; ++c) load(c, c);
-        for (int g = 0; g < NG; ++g) load_v(0, g);
+        load_v(0);
     }
 
-    {
-        // -------------------------------------------------------------------------------- scan
-        // A thread has row p and columns first .. first + W of its group's tile.
-        constexpr int W = VS / 2;
-        const int grp = warp / 8, first = warp / 4 % 2 * W;
-        const int bar = 1 + grp;
-        const bool lead = tid % 256 == 0;
-        const uint32_t D = tmem + grp * 3 * VS;  // [product with hi parts | with lo parts]
-        const uint32_t Dh = D + lanes + first, Dl = Dh + VS, TS = Dl + VS;  // TS: the state
-        const uint32_t mma = smem_addr(&sh.scan_mma[grp]);
-        const uint32_t s_hi = base + Lay::SB + grp * 2 * Lay::kS, s_lo = s_hi + Lay::kS;
-        const uint32_t r_hi = s_hi, r_lo = r_hi + Lay::kR, u_hi = s_lo, u_lo = u_hi + Lay::kR;
-        const uint32_t vb = base + Lay::V + grp * Lay::kR;
-        const int col = (vt * NG + grp) * VS + first;
-        const bool initial = a.states != nullptr && a.has_initial_state != nullptr && a.has_initial_state[row];
-        ST* sp = nullptr;
-        if (a.states != nullptr)
-            sp = static_cast<ST*>(a.states) + slot * a.s_slot + h * a.s_sh + p * a.s_sk + col;
-        constexpr int SV = Vec<ST>::V;
-        bf16* op = static_cast<bf16*>(a.out) + tok0 * a.o_st + h * a.o_sh + col;
+    // A thread has row p and columns first .. first + W of the tile.
+    constexpr int W = VS * 128 / Lay::kThreads;
+    const int first = warp / 4 * W;
+    const bool lead = tid == 0;
+    const uint32_t D = tmem;  // [product with hi parts | with lo parts]
+    const uint32_t Dh = D + lanes + first, Dl = Dh + VS, TS = Dl + VS;  // TS: the state
+    const uint32_t mma = smem_addr(&sh.mma);
+    const uint32_t s_hi = base + Lay::SB, s_lo = s_hi + Lay::kS;
+    const uint32_t r_hi = s_hi, r_lo = r_hi + Lay::kR, u_hi = s_lo, u_lo = u_hi + Lay::kR;
+    const uint32_t vb = base + Lay::V;
+    const int col = vt * VS + first;
+    const bool initial = a.states != nullptr && a.has_initial_state != nullptr && a.has_initial_state[row];
+    ST* sp = nullptr;
+    if (a.states != nullptr)
+        sp = static_cast<ST*>(a.states) + slot * a.s_slot + h * a.s_sh + p * a.s_sk + col;
+    constexpr int SV = Vec<ST>::V;
+    bf16* op = static_cast<bf16*>(a.out) + tok0 * a.o_st + h * a.o_sh + col;
 
-        int st = 0;
-        uint32_t phase = 0, st_phase = 0;
-        float decay = 0.f;
-        mbar_wait(smem_addr(&sh.full[0]), 0, &sh.abort);
+    // The loop below starts with S <- decay S + product; before the first chunk that is S0 + 0.
+#pragma unroll
+    for (int g = 0; g < W / 16; ++g) {
+        float2 s[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s[k] = make_float2(0.f, 0.f);
+        tmem_st16(Dh + 16 * g, s);
+        tmem_st16(Dl + 16 * g, s);
+        if (initial) {
+#pragma unroll
+            for (int k = 0; k < 16; k += SV) unpack16<ST>(ld16(sp + 16 * g + k), &s[0].x + k);
+        }
+        tmem_st16(TS + 16 * g, s);
+    }
+    tmem_wait_st();
+    int st = 0;
+    uint32_t phase = 0, st_phase = 0;
+    float decay = 1.f;
+    mbar_wait(smem_addr(&sh.full[0]), 0, &sh.abort);
 #pragma unroll 1
-        for (int c = 0;; ++c) {
-            // The state after the chunk before, into TMEM, and as an operand if there is another.
+    for (int c = 0;; ++c) {
+        // The state after the chunk before, into TMEM, and as an operand if there is another.
+        {
+            float2 d[W / 16][8], e[W / 16][8], s[W / 16][8];
 #pragma unroll
             for (int g = 0; g < W / 16; ++g) {
-                float2 s[8];
-                if (c == 0) {
+                tmem_ld16_async(Dh + 16 * g, d[g]);
+                tmem_ld16_async(Dl + 16 * g, e[g]);
+                tmem_ld16_async(TS + 16 * g, s[g]);
+            }
+            tmem_wait_ld();
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) s[k] = make_float2(0.f, 0.f);
-                    if (initial) {
+            for (int g = 0; g < W / 16; ++g) {
+                tmem_ready(d[g]);
+                tmem_ready(e[g]);
+                tmem_ready(s[g]);
 #pragma unroll
-                        for (int k = 0; k < 16; k += SV) unpack16<ST>(ld16(sp + 16 * g + k), &s[0].x + k);
-                    }
-                } else {
-                    float2 d[8], e[8];
-                    tmem_ld16_async(Dh + 16 * g, d);
-                    tmem_ld16_async(Dl + 16 * g, e);
-                    tmem_ld16_async(TS + 16 * g, s);
-                    tmem_wait_ld();
-                    tmem_ready(d);
-                    tmem_ready(e);
-                    tmem_ready(s);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        s[k] = __ffma2_rn(make_float2(decay, decay), s[k], __fadd2_rn(d[k], e[k]));
-                }
+                for (int k = 0; k < 8; ++k)
+                    s[g][k] = __ffma2_rn(make_float2(decay, decay), s[g][k], __fadd2_rn(d[g][k], e[g][k]));
                 if (c == chunks) {
                     if (sp != nullptr) {
 #pragma unroll
-                        for (int k = 0; k < 16; k += SV) st16(sp + 16 * g + k, pack16<ST>(&s[0].x + k));
+                        for (int k = 0; k < 16; k += SV) st16(sp + 16 * g + k, pack16<ST>(&s[g][0].x + k));
                     }
                 } else {
-                    tmem_st16(TS + 16 * g, s);
+                    tmem_st16(TS + 16 * g, s[g]);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const uint32_t at = swz<Lay::kRow>(p, first / 8 + 2 * g + u);
-                        store_split8(s_hi + at, s_lo + at, s + 4 * u);
+                        const uint32_t at = swz_cols<VS>(128, p, first / 8 + 2 * g + u);
+                        store_split8(s_hi + at, s_lo + at, s[g] + 4 * u);
                     }
                 }
             }
-            if (c == chunks) break;
-            tmem_wait_st();
-            const uint32_t kq = base + Lay::KQ + st * 32768, tg = base + Lay::TG + st * 32768;
-            const int left = ntok - c * C;
-            if (left < C) {
-                // The copies of K went on into the next sequence: zeros there, whatever it holds
-                // (rows of Q there make outputs that are not stored).
-                for (int e = tid % 256; e < (C - left) * 16; e += 256)
-                    sts16(kq + (e % 16 >> 3) * 16384 + swz<128>(left + e / 16, e % 8), 0, 0, 0, 0);
-            }
-            fence_async_smem();
-            tc_fence_before();
-            named_sync(bar, 256);
-            if (lead) {
-                tc_fence_after();
-                // [K;Q] S
-                const uint64_t k = operand(kq, 16, 1024, kSwizzle128), s = operand(s_hi, Lay::kS, kGroup, kSwz);
-                mma_steps<4, 2, kGroup / 8>(D, k, s, mma_desc(2 * VS, false, true), false);
-                mma_steps<4, 2, kGroup / 8>(D, k + 1024, s + kGroup / 2, mma_desc(2 * VS, false, true), true);
-                mma_commit(mma);
-                // While it runs: the last scan group through with the chunk before refills its
-                // stage.
-                if (c > 0 && c - 1 + kStages < chunks) {
-                    const int before = st > 0 ? st - 1 : kStages - 1;
-                    __threadfence_block();
-                    if (atomicAdd(&sh.done[before], 1) % NG == NG - 1) {
-                        __threadfence_block();
-                        load(c - 1 + kStages, before);
-                    }
-                }
-            }
-            const float in = vec[st].in[p], out = vec[st].out[p % C];
-            decay = vec[st].decay;
-            float2 q[W / 2];  // rows of Q: their outputs
-            if (p < C) mbar_wait(smem_addr(&sh.v_full[grp]), c & 1, &sh.abort);
-            mbar_wait(mma, phase, &sh.abort);
-            phase ^= 1;
+        }
+        if (c == chunks) break;
+        tmem_wait_st();
+        const uint32_t kq = base + Lay::KQ + st * 32768, tg = base + Lay::TG + st * 32768;
+        const int left = ntok - c * C;
+        if (left < C) {
+            // The copies of K went on into the next sequence: zeros there, whatever it holds
+            // (rows of Q there make outputs that are not stored).
+            for (int e = tid; e < (C - left) * 16; e += Lay::kThreads)
+                sts16(kq + (e % 16 >> 3) * 16384 + swz<128>(left + e / 16, e % 8), 0, 0, 0, 0);
+        }
+        fence_async_smem();
+        tc_fence_before();
+        __syncthreads();
+        if (lead) {
             tc_fence_after();
-            {
-                float2 d[W / 16][8], e[W / 16][8];
+            // [K;Q] S
+            const uint64_t k = operand(kq, 16, 1024, kSwizzle128), s = operand(s_hi, 128 * Lay::kRow, kGroup, kSwz);
+            mma_steps<4, 2, kGroup / 8>(D, k, s, mma_desc(2 * VS, false, true), false);
+            mma_steps<4, 2, kGroup / 8>(D, k + 1024, s + kGroup / 2, mma_desc(2 * VS, false, true), true);
+            mma_commit(mma);
+        }
+        // While it runs, a thread with little else to do (six copies take 560 cycles to issue) refills
+        // the stage of the chunk before.
+        if (tid == 64 && c > 0 && c - 1 + kStages < chunks) load(c - 1 + kStages, st > 0 ? st - 1 : kStages - 1);
+        const float in = vec[st].in[p], out = vec[st].out[p % C];
+        decay = vec[st].decay;
+        float2 q[W / 2];  // rows of Q: their outputs
+        if (p < C) mbar_wait(smem_addr(&sh.v_full), c & 1, &sh.abort);
+        mbar_wait(mma, phase, &sh.abort);
+        phase ^= 1;
+        tc_fence_after();
+        {
+            float2 d[W / 16][8], e[W / 16][8];
 #pragma unroll
-                for (int g = 0; g < W / 16; ++g) {
-                    tmem_ld16_async(Dh + 16 * g, d[g]);
-                    tmem_ld16_async(Dl + 16 * g, e[g]);
-                }
-                if (p < C) {
-                    // R = V - r e^b (K S), zero behind the sequence's end, whatever V holds there
-                    const bool live = p < left;
-                    uint4 v[W / 8];
-#pragma unroll
-                    for (int u = 0; u < W / 8; ++u) v[u] = lds16(vb + swz<Lay::kRow>(p, first / 8 + u));
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int g = 0; g < W / 16; ++g) {
-                        tmem_ready(d[g]);
-                        tmem_ready(e[g]);
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const uint32_t vv[4] = {v[2 * g + u].x, v[2 * g + u].y, v[2 * g + u].z, v[2 * g + u].w};
-                            float2 f[4];
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                f[k] = __ffma2_rn(make_float2(-in, -in), __fadd2_rn(d[g][4 * u + k], e[g][4 * u + k]),
-                                                  bf16_pair(live ? vv[k] : 0u));
-                            const uint32_t at = swz<Lay::kRow>(p, first / 8 + 2 * g + u);
-                            store_split8(r_hi + at, r_lo + at, f);
-                        }
-                    }
-                    fence_async_smem();
-                } else {
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int g = 0; g < W / 16; ++g) {
-                        tmem_ready(d[g]);
-                        tmem_ready(e[g]);
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) q[8 * g + k] = mul2(__fadd2_rn(d[g][k], e[g][k]), in);
-                    }
-                }
+            for (int g = 0; g < W / 16; ++g) {
+                tmem_ld16_async(Dh + 16 * g, d[g]);
+                tmem_ld16_async(Dl + 16 * g, e[g]);
             }
-            tc_fence_before();
-            named_sync(bar, 256);
-            if (lead) {
-                tc_fence_after();
-                // [T;G] R: hi [hi | lo], then lo hi
-                const uint64_t r = operand(r_hi, Lay::kR, kGroup, kSwz);
-                mma_steps<4, 2, kGroup / 8>(D, operand(tg, 16, 1024, kSwizzle128), r, mma_desc(2 * VS, false, true), false);
-                mma_steps<4, 2, kGroup / 8>(D, operand(tg + 16384, 16, 1024, kSwizzle128), r, mma_desc(VS, false, true), true);
-                mma_commit(mma);
-                if (c + 1 < chunks) load_v(c + 1, grp);
-            }
-            mbar_wait(mma, phase, &sh.abort);
-            phase ^= 1;
-            tc_fence_after();
-            {
-                float2 d[W / 16][8], e[W / 16][8];
+            if (p < C) {
+                // R = V - r e^b (K S), zero behind the sequence's end, whatever V holds there
+                const bool live = p < left;
+                uint4 v[W / 8];
 #pragma unroll
-                for (int g = 0; g < W / 16; ++g) {
-                    tmem_ld16_async(Dh + 16 * g, d[g]);
-                    tmem_ld16_async(Dl + 16 * g, e[g]);
-                }
+                for (int u = 0; u < W / 8; ++u) v[u] = lds16(vb + swz_cols<VS>(C, p, first / 8 + u));
                 tmem_wait_ld();
 #pragma unroll
                 for (int g = 0; g < W / 16; ++g) {
                     tmem_ready(d[g]);
                     tmem_ready(e[g]);
-                    if (p < C) {
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) d[g][k] = mul2(__fadd2_rn(d[g][k], e[g][k]), out);
+                    for (int u = 0; u < 2; ++u) {
+                        const uint32_t vv[4] = {v[2 * g + u].x, v[2 * g + u].y, v[2 * g + u].z, v[2 * g + u].w};
+                        float2 f[4];
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const uint32_t at = swz<Lay::kRow>(p, first / 8 + 2 * g + u);
-                            store_split8(u_hi + at, u_lo + at, d[g] + 4 * u);
-                        }
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 8; ++k)
-                            q[8 * g + k] = __fadd2_rn(q[8 * g + k], __fadd2_rn(d[g][k], e[g][k]));
+                        for (int k = 0; k < 4; ++k)
+                            f[k] = __ffma2_rn(make_float2(-in, -in), __fadd2_rn(d[g][4 * u + k], e[g][4 * u + k]),
+                                              bf16_pair(live ? vv[k] : 0u));
+                        const uint32_t at = swz_cols<VS>(C, p, first / 8 + 2 * g + u);
+                        store_split8(r_hi + at, r_lo + at, f);
                     }
                 }
-                if (p < C) fence_async_smem();
-            }
-            tc_fence_before();
-            named_sync(bar, 256);
-            if (lead) {
-                tc_fence_after();
-                // K^T u
-                mma_steps<4, 128, kGroup / 8>(D, operand(kq, 16384, 1024, kSwizzle128),
-                                              operand(u_hi, Lay::kR, kGroup, kSwz),
-                                              mma_desc(2 * VS, true, true), false);
-                mma_commit(mma);
-            }
-            const int t = c * C + p - C;
-            if (p >= C && t < ntok) {
-                bf16* to = op + (int64_t)t * a.o_st;
+                fence_async_smem();
+            } else {
+                tmem_wait_ld();
 #pragma unroll
-                for (int k = 0; k < W; k += 16) {
-                    const uint4 lo = pack16<bf16>(&q[k / 2].x), hi = pack16<bf16>(&q[k / 2 + 4].x);
-                    if (out32) {
-                        st32_stream(to + k, lo, hi);
-                    } else {
-                        st16(to + k, lo);
-                        st16(to + k + 8, hi);
-                    }
+                for (int g = 0; g < W / 16; ++g) {
+                    tmem_ready(d[g]);
+                    tmem_ready(e[g]);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) q[8 * g + k] = mul2(__fadd2_rn(d[g][k], e[g][k]), in);
                 }
             }
-            if (++st == kStages) {
-                st = 0;
-                st_phase ^= 1;
-            }
-            // The next chunk's K, Q, T, G: there by now, and the look costs less here.
-            if (c + 1 < chunks) mbar_wait(smem_addr(&sh.full[st]), st_phase, &sh.abort);
-            mbar_wait(mma, phase, &sh.abort);
-            phase ^= 1;
-            tc_fence_after();
         }
+        tc_fence_before();
+        __syncthreads();
+        if (lead) {
+            tc_fence_after();
+            // [T;G] R: hi [hi | lo], then lo hi
+            const uint64_t r = operand(r_hi, C * Lay::kRow, kGroup, kSwz);
+            mma_steps<4, 2, kGroup / 8>(D, operand(tg, 16, 1024, kSwizzle128), r, mma_desc(2 * VS, false, true), false);
+            mma_steps<4, 2, kGroup / 8>(D, operand(tg + 16384, 16, 1024, kSwizzle128), r, mma_desc(VS, false, true), true);
+            mma_commit(mma);
+            if (c + 1 < chunks) load_v(c + 1);
+        }
+        mbar_wait(mma, phase, &sh.abort);
+        phase ^= 1;
+        tc_fence_after();
+        {
+            float2 d[W / 16][8], e[W / 16][8];
+#pragma unroll
+            for (int g = 0; g < W / 16; ++g) {
+                tmem_ld16_async(Dh + 16 * g, d[g]);
+                tmem_ld16_async(Dl + 16 * g, e[g]);
+            }
+            tmem_wait_ld();
+#pragma unroll
+            for (int g = 0; g < W / 16; ++g) {
+                tmem_ready(d[g]);
+                tmem_ready(e[g]);
+                if (p < C) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) d[g][k] = mul2(__fadd2_rn(d[g][k], e[g][k]), out);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const uint32_t at = swz_cols<VS>(C, p, first / 8 + 2 * g + u);
+                        store_split8(u_hi + at, u_lo + at, d[g] + 4 * u);
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        q[8 * g + k] = __fadd2_rn(q[8 * g + k], __fadd2_rn(d[g][k], e[g][k]));
+                }
+            }
+            if (p < C) fence_async_smem();
+        }
+        tc_fence_before();
+        __syncthreads();
+        if (lead) {
+            tc_fence_after();
+            // K^T u
+            mma_steps<4, 128, kGroup / 8>(D, operand(kq, 16384, 1024, kSwizzle128),
+                                          operand(u_hi, C * Lay::kRow, kGroup, kSwz),
+                                          mma_desc(2 * VS, true, true), false);
+            mma_commit(mma);
+        }
+        const int t = c * C + p - C;
+        if (p >= C && t < ntok) {
+            bf16* to = op + (int64_t)t * a.o_st;
+#pragma unroll
+            for (int k = 0; k < W; k += 16) {
+                const uint4 lo = pack16<bf16>(&q[k / 2].x), hi = pack16<bf16>(&q[k / 2 + 4].x);
+                if (out32) {
+                    st32_stream(to + k, lo, hi);
+                } else {
+                    st16(to + k, lo);
+                    st16(to + k + 8, hi);
+                }
+            }
+        }
+        if (++st == kStages) {
+            st = 0;
+            st_phase ^= 1;
+        }
+        // The next chunk's K, Q, T, G: there by now, and the look costs less here.
+        if (c + 1 < chunks) mbar_wait(smem_addr(&sh.full[st]), st_phase, &sh.abort);
+        mbar_wait(mma, phase, &sh.abort);
+        phase ^= 1;
+        tc_fence_after();
     }
     tc_fence_before();
     __syncthreads();
@@ -404,32 +410,32 @@ Encode encoder() {
     return f;
 }
 
-template <typename ST, int VS, int NG>
+template <typename ST, int VS>
 cudaError_t go(const cc1d_gdr_args& a, bool out32, cudaStream_t stream) {
-    using Lay = Layout<VS, NG>;
+    using Lay = Layout<VS>;
     constexpr int smem = Lay::END + 1024;
-    const int tiles = a.dv / (VS * NG);
+    const int tiles = a.dv / VS;
     const int64_t grid = a.rows * a.heads_v * tiles;
     if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
     CUtensorMap q, k, v;
     if (!make_map(&q, a.q, a.tokens, a.heads_k, a.dk, a.q_st, a.q_sh, 64) ||
         !make_map(&k, a.k, a.tokens, a.heads_k, a.dk, a.k_st, a.k_sh, 64) ||
-        !make_map(&v, a.v, a.tokens, a.heads_v, a.dv, a.v_st, a.v_sh, VS))
+        !make_map(&v, a.v, a.tokens, a.heads_v, a.dv, a.v_st, a.v_sh, VS < 64 ? VS : 64))
         return cudaErrorInvalidValue;
     cudaError_t err = launch_gdr_prep(a, q, k, stream);
     if (err != cudaSuccess) return err;
-    err = cudaFuncSetAttribute(gdr_chunk_kernel<ST, VS, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    err = cudaFuncSetAttribute(gdr_chunk_kernel<ST, VS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (err != cudaSuccess) return err;
-    gdr_chunk_kernel<ST, VS, NG><<<(unsigned)grid, Lay::kThreads, smem, stream>>>(a, q, k, v, tiles, out32);
+    gdr_chunk_kernel<ST, VS><<<(unsigned)grid, Lay::kThreads, smem, stream>>>(a, q, k, v, tiles, out32);
     return cudaGetLastError();
 }
 
 template <typename ST>
 cudaError_t pick(const cc1d_gdr_args& a, bool out32, cudaStream_t stream) {
     const int64_t heads = a.rows * a.heads_v;
-    if (a.dv % 128 == 0 && heads * (a.dv / 128) >= 148) return go<ST, 64, 2>(a, out32, stream);
-    if (a.dv % 64 == 0 && heads * (a.dv / 64) >= 148) return go<ST, 64, 1>(a, out32, stream);
-    return go<ST, 32, 1>(a, out32, stream);
+    if (a.dv % 128 == 0 && heads * (a.dv / 128) >= 148) return go<ST, 128>(a, out32, stream);
+    if (a.dv % 64 == 0 && heads * (a.dv / 64) >= 148) return go<ST, 64>(a, out32, stream);
+    return go<ST, 32>(a, out32, stream);
 }
 
 }  // namespace

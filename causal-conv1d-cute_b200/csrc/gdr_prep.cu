@@ -27,9 +27,6 @@ constexpr int kHeads = 4;  // value heads whose gates are made at a time, one wa
 struct Blocks {
     float diag[2][32][LPAD], low[32][LPAD];
 };
-// P as a 128-row operand reads 8 KB behind its last row.
-static_assert(sizeof(Blocks) >= 8192, "");
-
 // What a chunk's gates give: cumulative log2 decays b, negated, in two parts each; rates; decays
 // e^(b_i), e^(b_C - b_j) and, below 32, e^(b_31 - b_j).
 struct Gates {
@@ -308,6 +305,28 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
     }
 
     Blocks& blk = sh.blk;
+    // G of value head h, once its product is there: rows 64.. of the product, by warps 2 and 3.
+    auto store_g = [&](int h) {
+        ChunkImage* out = static_cast<ChunkImage*>(a.workspace) + image * a.heads_v + h;
+        mbar_wait(smem_addr(&sh.mma), phase, &sh.abort);
+        phase ^= 1;
+        tc_fence_after();
+#pragma unroll 1
+        for (int o = 0; o < C; o += 16) {
+            float2 x[8];
+            tmem_ld16(DG + lanes + o, x);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) split2(x[4 * u + e], hi[e], lo[e]);
+                const uint32_t at = swz<128>(p, o / 8 + u);
+                st16(out->tg[0] + at, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+                st16(out->tg[1] + at, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+            }
+        }
+        tc_fence_before();
+    };
 #pragma unroll 1
     for (int v = 0; v < group; ++v) {
         const int h = hk * group + v;
@@ -325,6 +344,8 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
         if (p < 32) sh.ru[p] = norm * ga.far[p];
         __syncthreads();
         tc_fence_after();
+        // The head before: its G, while warps 0 and 1 are at L and its inverse.
+        if (p >= C && v > 0) store_g(h - 1);
         // Warps 0 and 1 make L (columns j < i) of rows of K K^T, warps 2 and 3 make P (columns
         // j <= i) of rows of Q K^T. In the columns of a row's own half the decay e^(b_i - b_j) is
         // taken element by element; for the lower left block it splits at the middle of the chunk
@@ -449,8 +470,9 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
         __syncthreads();
         if (p == 0) {
             tc_fence_after();
-            // G = P T in rows 0..63: hi hi, hi lo, lo hi. Rows 64.. are of no use.
-            const uint64_t P = operand(pb, 16, 1024, kSwizzle128), T = operand(tb, 16384, 1024, kSwizzle128);
+            // G = P T in rows 64..: hi hi, hi lo, lo hi. The 8 KB before either part of P are other
+            // parts of T or P; the rows 0..63 they make are of no use.
+            const uint64_t P = operand(pb - 8192, 16, 1024, kSwizzle128), T = operand(tb, 16384, 1024, kSwizzle128);
             mma_steps<4, 2, 128>(DG, P, T, mma_desc(64, false, true), false);
             mma_steps<4, 2, 128>(DG, P, T + 512, mma_desc(64, false, true), true);
             mma_steps<4, 2, 128>(DG, P + 512, T, mma_desc(64, false, true), true);
@@ -462,27 +484,8 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
                              : "memory");
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
-        mbar_wait(smem_addr(&sh.mma), phase, &sh.abort);
-        phase ^= 1;
-        tc_fence_after();
-        if (p < C) {
-#pragma unroll 1
-            for (int o = 0; o < C; o += 16) {
-                float2 x[8];
-                tmem_ld16(DG + lanes + o, x);
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    uint32_t hi[4], lo[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) split2(x[4 * u + e], hi[e], lo[e]);
-                    const uint32_t at = swz<128>(C + p, o / 8 + u);
-                    st16(out->tg[0] + at, make_uint4(hi[0], hi[1], hi[2], hi[3]));
-                    st16(out->tg[1] + at, make_uint4(lo[0], lo[1], lo[2], lo[3]));
-                }
-            }
-        }
-        tc_fence_before();
     }
+    if (p >= C) store_g(hk * group + group - 1);
     if (p == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     __syncthreads();
     tc_fence_after();

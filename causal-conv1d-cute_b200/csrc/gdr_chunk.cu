@@ -26,7 +26,8 @@
 // columns takes XXXX: tensor memory serves the products of one and the loads of the other in turn.)
 // Stacking K over Q and T over G makes every product M = 128, the full tensor core rate; the two
 // parts of an operand lie side by side as one operand of 2 VS columns (measured: a K step of 16
-// costs 46 cycles up to 64 columns and 66 with 128, so one wide step beats two narrow ones).
+// costs 46 cycles up to 64 columns, 66 with 128 and 137 with 256, so one wide step beats two narrow
+// ones up to VS = 64).
 // Loops over columns stay rolled where registers allow it: with all of them unrolled the warps
 // spent a quarter of their time waiting for instructions.
 #include "gdr_chunk.cuh"
@@ -49,7 +50,11 @@ struct Layout {
     static constexpr int V = SB + 2 * kS;                 // [atoms][64 rows]
     static constexpr int VEC = V + kR;                    // stages x row factors
     static constexpr int END = VEC + kStages * kVectorBytes;
-    static constexpr int kTmem = VS == 32 ? 128 : VS == 64 ? 256 : 512;  // of 3 VS columns
+    // The products with the two parts of an operand: side by side, and added on the way out of
+    // TMEM, while that is the faster way (see above); on top of each other with 128 columns, where
+    // a step costs the same per column either way.
+    static constexpr bool kWide = VS < 128;
+    static constexpr int kTmem = VS == 32 ? 128 : 256;  // of 3 VS columns, or 2
     static constexpr int kThreads = VS == 128 ? 512 : 256;
 };
 
@@ -73,6 +78,20 @@ __device__ __forceinline__ uint32_t swz_cols(int rows, int r, int u) {
         return (u >> 3) * rows * 128 + swz<128>(r, u & 7);
     } else {
         return swz<Layout<VS>::kRow>(r, u);
+    }
+}
+
+// One thread: D (+)= A B over kSteps K steps, B in two parts: side by side as one operand of 2 VS
+// columns, or, with 128 columns, one after the other (`lo` units apart) onto the same columns.
+template <int VS, int kSteps, int kA, bool kTransposedA>
+__device__ __forceinline__ void two_part_product(uint32_t d, uint64_t a, uint64_t b, uint32_t lo,
+                                                 bool accumulate) {
+    constexpr int kB = 8 * Layout<VS>::kRow / 8;
+    if constexpr (Layout<VS>::kWide) {
+        mma_steps<kSteps, kA, kB>(d, a, b, mma_desc(2 * VS, kTransposedA, true), accumulate);
+    } else {
+        mma_steps<kSteps, kA, kB>(d, a, b, mma_desc(VS, kTransposedA, true), accumulate);
+        mma_steps<kSteps, kA, kB>(d, a, b + lo, mma_desc(VS, kTransposedA, true), true);
     }
 }
 
@@ -169,8 +188,8 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
     constexpr int W = VS * 128 / Lay::kThreads;
     const int first = warp / 4 * W;
     const bool lead = tid == 0;
-    const uint32_t D = tmem;  // [product with hi parts | with lo parts]
-    const uint32_t Dh = D + lanes + first, Dl = Dh + VS, TS = Dl + VS;  // TS: the state
+    const uint32_t D = tmem;  // the product, or [product with hi parts | with lo parts]
+    const uint32_t Dh = D + lanes + first, Dl = Dh + VS, TS = Lay::kWide ? Dl + VS : Dl;  // TS: the state
     const uint32_t mma = smem_addr(&sh.mma);
     const uint32_t s_hi = base + Lay::SB, s_lo = s_hi + Lay::kS;
     const uint32_t r_hi = s_hi, r_lo = r_hi + Lay::kR, u_hi = s_lo, u_lo = u_hi + Lay::kR;
@@ -180,6 +199,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
     ST* sp = nullptr;
     if (a.states != nullptr)
         sp = static_cast<ST*>(a.states) + slot * a.s_slot + h * a.s_sh + p * a.s_sk + col;
+    auto sum = [](float2 x, float2 y) { return Lay::kWide ? __fadd2_rn(x, y) : x; };
     constexpr int SV = Vec<ST>::V;
     bf16* op = static_cast<bf16*>(a.out) + tok0 * a.o_st + h * a.o_sh + col;
 
@@ -190,7 +210,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
 #pragma unroll
         for (int k = 0; k < 8; ++k) s[k] = make_float2(0.f, 0.f);
         tmem_st16(Dh + 16 * g, s);
-        tmem_st16(Dl + 16 * g, s);
+        if (Lay::kWide) tmem_st16(Dl + 16 * g, s);
         if (initial) {
 #pragma unroll
             for (int k = 0; k < 16; k += SV) unpack16<ST>(ld16(sp + 16 * g + k), &s[0].x + k);
@@ -210,18 +230,18 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
 #pragma unroll
             for (int g = 0; g < W / 16; ++g) {
                 tmem_ld16_async(Dh + 16 * g, d[g]);
-                tmem_ld16_async(Dl + 16 * g, e[g]);
+                if (Lay::kWide) tmem_ld16_async(Dl + 16 * g, e[g]);
                 tmem_ld16_async(TS + 16 * g, s[g]);
             }
             tmem_wait_ld();
 #pragma unroll
             for (int g = 0; g < W / 16; ++g) {
                 tmem_ready(d[g]);
-                tmem_ready(e[g]);
+                if (Lay::kWide) tmem_ready(e[g]);
                 tmem_ready(s[g]);
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
-                    s[g][k] = __ffma2_rn(make_float2(decay, decay), s[g][k], __fadd2_rn(d[g][k], e[g][k]));
+                    s[g][k] = __ffma2_rn(make_float2(decay, decay), s[g][k], sum(d[g][k], e[g][k]));
                 if (c == chunks) {
                     if (sp != nullptr) {
 #pragma unroll
@@ -254,8 +274,8 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
             tc_fence_after();
             // [K;Q] S
             const uint64_t k = operand(kq, 16, 1024, kSwizzle128), s = operand(s_hi, 128 * Lay::kRow, kGroup, kSwz);
-            mma_steps<4, 2, kGroup / 8>(D, k, s, mma_desc(2 * VS, false, true), false);
-            mma_steps<4, 2, kGroup / 8>(D, k + 1024, s + kGroup / 2, mma_desc(2 * VS, false, true), true);
+            two_part_product<VS, 4, 2, false>(D, k, s, Lay::kS / 16, false);
+            two_part_product<VS, 4, 2, false>(D, k + 1024, s + kGroup / 2, Lay::kS / 16, true);
             mma_commit(mma);
         }
         // While it runs, a thread with little else to do (six copies take 560 cycles to issue) refills
@@ -273,7 +293,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
 #pragma unroll
             for (int g = 0; g < W / 16; ++g) {
                 tmem_ld16_async(Dh + 16 * g, d[g]);
-                tmem_ld16_async(Dl + 16 * g, e[g]);
+                if (Lay::kWide) tmem_ld16_async(Dl + 16 * g, e[g]);
             }
             if (p < C) {
                 // R = V - r e^b (K S), zero behind the sequence's end, whatever V holds there
@@ -285,15 +305,14 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
 #pragma unroll
                 for (int g = 0; g < W / 16; ++g) {
                     tmem_ready(d[g]);
-                    tmem_ready(e[g]);
+                    if (Lay::kWide) tmem_ready(e[g]);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         const uint32_t vv[4] = {v[2 * g + u].x, v[2 * g + u].y, v[2 * g + u].z, v[2 * g + u].w};
                         float2 f[4];
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            f[k] = __ffma2_rn(make_float2(-in, -in), __fadd2_rn(d[g][4 * u + k], e[g][4 * u + k]),
-                                              bf16_pair(live ? vv[k] : 0u));
+                            f[k] = add_bf16(live ? vv[k] : 0u, mul2(sum(d[g][4 * u + k], e[g][4 * u + k]), -in));
                         const uint32_t at = swz_cols<VS>(C, p, first / 8 + 2 * g + u);
                         store_split8(r_hi + at, r_lo + at, f);
                     }
@@ -304,9 +323,9 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
 #pragma unroll
                 for (int g = 0; g < W / 16; ++g) {
                     tmem_ready(d[g]);
-                    tmem_ready(e[g]);
+                    if (Lay::kWide) tmem_ready(e[g]);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) q[8 * g + k] = mul2(__fadd2_rn(d[g][k], e[g][k]), in);
+                    for (int k = 0; k < 8; ++k) q[8 * g + k] = mul2(sum(d[g][k], e[g][k]), in);
                 }
             }
         }
@@ -316,7 +335,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
             tc_fence_after();
             // [T;G] R: hi [hi | lo], then lo hi
             const uint64_t r = operand(r_hi, C * Lay::kRow, kGroup, kSwz);
-            mma_steps<4, 2, kGroup / 8>(D, operand(tg, 16, 1024, kSwizzle128), r, mma_desc(2 * VS, false, true), false);
+            two_part_product<VS, 4, 2, false>(D, operand(tg, 16, 1024, kSwizzle128), r, Lay::kR / 16, false);
             mma_steps<4, 2, kGroup / 8>(D, operand(tg + 16384, 16, 1024, kSwizzle128), r, mma_desc(VS, false, true), true);
             mma_commit(mma);
             if (c + 1 < chunks) load_v(c + 1);
@@ -329,16 +348,16 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
 #pragma unroll
             for (int g = 0; g < W / 16; ++g) {
                 tmem_ld16_async(Dh + 16 * g, d[g]);
-                tmem_ld16_async(Dl + 16 * g, e[g]);
+                if (Lay::kWide) tmem_ld16_async(Dl + 16 * g, e[g]);
             }
             tmem_wait_ld();
 #pragma unroll
             for (int g = 0; g < W / 16; ++g) {
                 tmem_ready(d[g]);
-                tmem_ready(e[g]);
+                if (Lay::kWide) tmem_ready(e[g]);
                 if (p < C) {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) d[g][k] = mul2(__fadd2_rn(d[g][k], e[g][k]), out);
+                    for (int k = 0; k < 8; ++k) d[g][k] = mul2(sum(d[g][k], e[g][k]), out);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         const uint32_t at = swz_cols<VS>(C, p, first / 8 + 2 * g + u);
@@ -347,7 +366,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
                 } else {
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
-                        q[8 * g + k] = __fadd2_rn(q[8 * g + k], __fadd2_rn(d[g][k], e[g][k]));
+                        q[8 * g + k] = __fadd2_rn(q[8 * g + k], sum(d[g][k], e[g][k]));
                 }
             }
             if (p < C) fence_async_smem();
@@ -357,9 +376,8 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
         if (lead) {
             tc_fence_after();
             // K^T u
-            mma_steps<4, 128, kGroup / 8>(D, operand(kq, 16384, 1024, kSwizzle128),
-                                          operand(u_hi, C * Lay::kRow, kGroup, kSwz),
-                                          mma_desc(2 * VS, true, true), false);
+            two_part_product<VS, 4, 128, true>(D, operand(kq, 16384, 1024, kSwizzle128),
+                                               operand(u_hi, C * Lay::kRow, kGroup, kSwz), Lay::kR / 16, false);
             mma_commit(mma);
         }
         const int t = c * C + p - C;

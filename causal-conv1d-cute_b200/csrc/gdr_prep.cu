@@ -37,7 +37,7 @@ struct Smem {
     unsigned char kq[32768];  // [2 halves][K 64 rows, Q 64 rows][128 B]; later T hi, T lo, P hi, P lo
     Blocks blk;
     Gates gates[kHeads];
-    alignas(16) float rk[C], ru[C];
+    alignas(16) float rk[C], ru[kHeads][32];  // inverse norms of the keys; with e^(b_31 - b_j)
     uint64_t full, mma;
     uint32_t tmem;
     int abort, seq;
@@ -197,15 +197,14 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
         }
     }
 
-    // Gates of one value head by one warp, two tokens a lane.
+    // Gates of one value head by one warp, two tokens a lane: the loads, all at once, and the rest.
     const int group = a.heads_v / a.heads_k;
-    auto make_gates = [&](int h, Gates& to) {
-        float rate = 0.f, dt = 0.f;
+    uint32_t g_bits[2] = {0, 0}, b_bits[2] = {0, 0}, rate_bits = 0, dt_bits = 0;
+    auto load_gates = [&](int h) {
         if (a.a_log != nullptr) {
-            rate = -expf(load_any(a.a_log, h, a.pdtype));
-            dt = load_any(a.dt_bias, h, a.pdtype);
+            rate_bits = load_bits(a.a_log, h, a.pdtype);
+            dt_bits = load_bits(a.dt_bias, h, a.pdtype);
         }
-        uint32_t g_bits[2] = {0, 0}, b_bits[2] = {0, 0};
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int64_t t = tok0 + 2 * lane + e;
@@ -214,6 +213,9 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
                 b_bits[e] = load_bits(a.beta, t * a.b_st + h * a.b_sh, a.bdtype);
             }
         }
+    };
+    auto make_gates = [&](Gates& to) {
+        const float rate = -expf(bits_value(rate_bits, a.pdtype)), dt = bits_value(dt_bits, a.pdtype);
         double sum[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -255,7 +257,8 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
             if (t < 32) to.far[t] = exp2_approx((float)(mid - b[e]));
         }
     };
-    if (w < group) make_gates(hk * group + w, sh.gates[w]);
+    if (w < group) load_gates(hk * group + w);
+    if (w < group) make_gates(sh.gates[w]);
 
     mbar_wait(smem_addr(&sh.full), 0, &sh.abort);
     if (left < C) {
@@ -292,9 +295,10 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
         norm = rsqrtf((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y) + kL2Eps);
     }
     if (p < C) sh.rk[p] = norm;
+    __syncthreads();
+    sh.ru[w][lane] = sh.rk[lane] * sh.gates[w].far[lane];
     mbar_wait(smem_addr(&sh.mma), phase, &sh.abort);
     phase ^= 1;
-    __syncthreads();
     // K and Q are through; T and P are zero above their diagonal blocks from here on.
     if (p < 32) {
 #pragma unroll
@@ -303,6 +307,8 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
             for (int m = 0; m < 4; ++m) sts16(kq + m * 8192 + swz<128>(p, u), 0, 0, 0, 0);
         }
     }
+    __syncthreads();
+    tc_fence_after();
 
     Blocks& blk = sh.blk;
     // G of value head h, once its product is there: rows 64.. of the product, by warps 2 and 3.
@@ -331,8 +337,12 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
     for (int v = 0; v < group; ++v) {
         const int h = hk * group + v;
         if (v > 0 && v % kHeads == 0) {
-            __syncthreads();
-            if (v + w < group) make_gates(h + w, sh.gates[w]);
+            if (v + w < group) {
+                load_gates(h + w);
+                make_gates(sh.gates[w]);
+            }
+            __syncwarp();
+            sh.ru[w][lane] = sh.rk[lane] * sh.gates[w].far[lane];
             __syncthreads();
         }
         const Gates& ga = sh.gates[v % kHeads];
@@ -341,9 +351,6 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
         out->in[p] = ga.grow[i] * (p < C ? norm : mul);
         if (p < C) out->out[i] = norm * ga.out[i];
         if (p == C - 1) out->decay = ga.grow[i];
-        if (p < 32) sh.ru[p] = norm * ga.far[p];
-        __syncthreads();
-        tc_fence_after();
         // The head before: its G, while warps 0 and 1 are at L and its inverse.
         if (p >= C && v > 0) store_g(h - 1);
         // Warps 0 and 1 make L (columns j < i) of rows of K K^T, warps 2 and 3 make P (columns
@@ -385,7 +392,7 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
                 } else {
 #pragma unroll
                     for (int e = 0; e < 8; e += 2) {
-                        const float4 r4 = *reinterpret_cast<const float4*>(&sh.ru[o + 2 * e]);
+                        const float4 r4 = *reinterpret_cast<const float4*>(&sh.ru[v % kHeads][o + 2 * e]);
                         x[e] = __fmul2_rn(x[e], mul2(make_float2(r4.x, r4.y), low_mul));
                         x[e + 1] = __fmul2_rn(x[e + 1], mul2(make_float2(r4.z, r4.w), low_mul));
                     }
@@ -430,7 +437,7 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
                         make_float2(-d[n][2 * e], -d[n][2 * e + 1]);
         }
         // The bulk copies of the T before have read it.
-        if (p == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        if (p == 96) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         __syncthreads();
         {
             // The 32 x 32 block below the diagonal ones, a 16 x 16 tile per warp.
@@ -468,7 +475,8 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
         fence_async_smem();
         tc_fence_before();
         __syncthreads();
-        if (p == 0) {
+        if (p == 96) {
+            // A thread of the warps that wait for this product next.
             tc_fence_after();
             // G = P T in rows 64..: hi hi, hi lo, lo hi. The 8 KB before either part of P are other
             // parts of T or P; the rows 0..63 they make are of no use.
@@ -484,9 +492,10 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
                              : "memory");
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
+        __syncwarp();
     }
     if (p >= C) store_g(hk * group + group - 1);
-    if (p == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (p == 96) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     __syncthreads();
     tc_fence_after();
     if (w == 0) tmem_dealloc(sh.tmem, 128);

@@ -21,13 +21,25 @@ __device__ __forceinline__ float gate(float z) {
     }
 }
 
+// n / d for n below 2^31 by one multiplication (d >= 1), d fixed for a launch.
+struct Divider {
+    uint32_t d, mul, shift;
+    explicit Divider(uint32_t divisor) : d(divisor), mul(0), shift(0) {
+        while (shift < 31 && (1u << shift) < d) ++shift;
+        mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
+        return (__umulhi(n, mul) + n) >> shift;
+    }
+};
+
 template <typename T, int LANES, int VPL, int R>
 __global__ void __launch_bounds__(256)
-norm_kernel(const __grid_constant__ cc1d_norm_args a, int64_t rows) {
+norm_kernel(const __grid_constant__ cc1d_norm_args a, int rows, Divider by_n1) {
     constexpr int V = Vec<T>::V;
     constexpr int GROUPS = 256 / LANES;
     const int lane = threadIdx.x % LANES;
-    const int64_t first = (int64_t)blockIdx.x * (GROUPS * R) + threadIdx.x / LANES;
+    const int first = blockIdx.x * (GROUPS * R) + threadIdx.x / LANES;
     const T* xp = static_cast<const T*>(a.x);
     const T* zp = static_cast<const T*>(a.z);
     T* op = static_cast<T*>(a.out);
@@ -35,8 +47,8 @@ norm_kernel(const __grid_constant__ cc1d_norm_args a, int64_t rows) {
     uint4 x[R][VPL], z[R][VPL];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const int64_t row = first + r * GROUPS;
-        const int64_t i0 = row / a.n1, i1 = row % a.n1;
+        const int row = first + r * GROUPS;
+        const int64_t i0 = by_n1(row), i1 = row - i0 * a.n1;
 #pragma unroll
         for (int m = 0; m < VPL; ++m) {
             const int e = (m * LANES + lane) * V;
@@ -60,7 +72,7 @@ norm_kernel(const __grid_constant__ cc1d_norm_args a, int64_t rows) {
         }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const int64_t row = first + r * GROUPS;
+        const int row = first + r * GROUPS;
         float f[VPL][V], sum = 0.f;
 #pragma unroll
         for (int m = 0; m < VPL; ++m) {
@@ -72,7 +84,7 @@ norm_kernel(const __grid_constant__ cc1d_norm_args a, int64_t rows) {
         for (int o = LANES / 2; o > 0; o /= 2) sum += __shfl_xor_sync(~0u, sum, o);
         const float inv = rsqrtf(sum / (float)a.dim + a.eps);
         if (row >= rows) continue;
-        const int64_t i0 = row / a.n1, i1 = row % a.n1;
+        const int64_t i0 = by_n1(row), i1 = row - i0 * a.n1;
 #pragma unroll
         for (int m = 0; m < VPL; ++m) {
             const int e = (m * LANES + lane) * V;
@@ -117,7 +129,7 @@ norm_generic_kernel(const __grid_constant__ cc1d_norm_args a, int64_t rows) {
 template <typename T, int LANES, int VPL, int R>
 void go(const cc1d_norm_args& a, int64_t rows, cudaStream_t stream) {
     const int64_t grid = ceil_div(rows, (256 / LANES) * R);
-    norm_kernel<T, LANES, VPL, R><<<(unsigned)grid, 256, 0, stream>>>(a, rows);
+    norm_kernel<T, LANES, VPL, R><<<(unsigned)grid, 256, 0, stream>>>(a, (int)rows, Divider((uint32_t)a.n1));
 }
 
 template <typename T>
@@ -128,7 +140,8 @@ cudaError_t launch(const cc1d_norm_args& a, cudaStream_t stream) {
     const bool vec = a.dim % V == 0 && host_aligned16(a.x) && host_aligned16(a.out) &&
                      (a.z == nullptr || (host_aligned16(a.z) && a.z_s0 % V == 0 && a.z_s1 % V == 0)) &&
                      a.x_s0 % V == 0 && a.x_s1 % V == 0 && a.o_s0 % V == 0 && a.o_s1 % V == 0;
-    if (!vec || a.dim > 128 * V) {
+    // 2^30 rows and more (their 32-bit indices and the divider's) take the generic kernel.
+    if (!vec || a.dim > 128 * V || rows >= (1 << 30)) {
         norm_generic_kernel<T><<<(unsigned)ceil_div(rows, 8), 256, 0, stream>>>(a, rows);
     } else if (a.dim <= 8 * V) {
         go<T, 8, 1, 4>(a, rows, stream);

@@ -1,4 +1,4 @@
-// Gated delta rule over packed sequences, chunk by chunk on the tensor cores (bf16, dk = 128).
+// Gated delta rule over packed sequences, chunk by chunk on the tensor cores (bf16 and fp16, dk = 128).
 //
 // Mathematics. In a chunk of C = 64 tokens that starts from state S0, with b the cumulative log
 // decay inside the chunk, r the inverse norms of the keys (1 without l2norm) and s those of the
@@ -8,7 +8,8 @@
 //     R_i  = v_i - r_i e^(b_i) S0^T k_i
 //     u    = T R,      o_i = s_i e^(b_i) S0^T q_i + (G R)_i
 //     S    = e^(b_C) S0 + sum_j k_j (r_j e^(b_C - b_j) u_j)^T.
-// k and q enter every product as the caller's bf16 values, which are exact; norms, gates and
+// k and q enter every product as the caller's bf16 values (fp16 ones as two bf16 parts), which are
+// exact; norms, gates and
 // decays scale rows in fp32 outside the products. All exponents are differences b_i - b_j <= 0.
 //
 // Precision. S, R, T, G and u are fp32 quantities. As operands they are split into two bf16 parts
@@ -37,15 +38,16 @@ namespace {
 
 constexpr int kOrderMax = 256;  // batches up to this many sequences start with the longest
 
-template <int VS>
+template <int VS, bool kLo>
 struct Layout {
     static constexpr int kRow = VS >= 64 ? 128 : 2 * VS;  // bytes of a row of an operand's column atom
     static constexpr int kAtoms = VS >= 64 ? VS / 64 : 1;
     static constexpr int kS = 128 * kRow * kAtoms;        // one part (hi or lo) of S
     static constexpr int kR = C * kRow * kAtoms;          // one part of R or u, or V
-    static constexpr int kStages = VS <= 32 ? 3 : 2;
-    static constexpr int KQ = 0;                          // stages x [2 halves][128 rows][128 B]
-    static constexpr int TG = KQ + kStages * 32768;       // stages x [hi, lo][128 rows][128 B]
+    static constexpr int kKQ = Parts<kLo>::kBytes;
+    static constexpr int kStages = kLo ? 1 : VS <= 32 ? 3 : 2;
+    static constexpr int KQ = 0;                          // stages x K and Q
+    static constexpr int TG = KQ + kStages * kKQ;         // stages x [hi, lo][128 rows][128 B]
     static constexpr int SB = TG + kStages * 32768;       // S hi, S lo; R in S hi, u in S lo
     static constexpr int V = SB + 2 * kS;                 // [atoms][64 rows]
     static constexpr int VEC = V + kR;                    // stages x row factors
@@ -77,7 +79,7 @@ __device__ __forceinline__ uint32_t swz_cols(int rows, int r, int u) {
     if constexpr (VS > 64) {
         return (u >> 3) * rows * 128 + swz<128>(r, u & 7);
     } else {
-        return swz<Layout<VS>::kRow>(r, u);
+        return swz<Layout<VS, false>::kRow>(r, u);
     }
 }
 
@@ -86,8 +88,8 @@ __device__ __forceinline__ uint32_t swz_cols(int rows, int r, int u) {
 template <int VS, int kSteps, int kA, bool kTransposedA>
 __device__ __forceinline__ void two_part_product(uint32_t d, uint64_t a, uint64_t b, uint32_t lo,
                                                  bool accumulate) {
-    constexpr int kB = 8 * Layout<VS>::kRow / 8;
-    if constexpr (Layout<VS>::kWide) {
+    constexpr int kB = Layout<VS, false>::kRow;
+    if constexpr (Layout<VS, false>::kWide) {
         mma_steps<kSteps, kA, kB>(d, a, b, mma_desc(2 * VS, kTransposedA, true), accumulate);
     } else {
         mma_steps<kSteps, kA, kB>(d, a, b, mma_desc(VS, kTransposedA, true), accumulate);
@@ -95,12 +97,13 @@ __device__ __forceinline__ void two_part_product(uint32_t d, uint64_t a, uint64_
     }
 }
 
-template <typename ST, int VS>
-__global__ void __launch_bounds__(Layout<VS>::kThreads, 1)
+template <typename T, typename ST, int VS>
+__global__ void __launch_bounds__(Layout<VS, false>::kThreads, 1)
 gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__ CUtensorMap mapq,
                  const __grid_constant__ CUtensorMap mapk, const __grid_constant__ CUtensorMap mapv,
                  int tiles, bool out32) {
-    using Lay = Layout<VS>;
+    constexpr bool kLo = std::is_same<T, f16>::value;  // fp16 keys and queries come in two bf16 parts
+    using Lay = Layout<VS, kLo>;
     constexpr uint64_t kSwz = VS >= 64 ? kSwizzle128 : kSwizzle64;
     constexpr uint32_t kGroup = 8 * Lay::kRow;  // bytes of eight rows of V columns
     constexpr int kStages = Lay::kStages;
@@ -159,15 +162,10 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
 
     // K, Q, T, G and the row factors of chunk c into stage st, which must be free; one thread.
     auto load = [&](int c, int st) {
-        const uint32_t full = smem_addr(&sh.full[st]), kq = base + Lay::KQ + st * 32768;
-        const int t = (int)tok0 + c * C;
+        const uint32_t full = smem_addr(&sh.full[st]);
         const ChunkImage* from = image + (int64_t)c * a.heads_v;
-        mbar_expect(full, 65536 + kVectorBytes);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            tma_load(kq + half * 16384, &mapk, half * 64, hk, t, full);
-            tma_load(kq + half * 16384 + 8192, &mapq, half * 64, hk, t, full);
-        }
+        mbar_expect(full, Lay::kKQ + 32768 + kVectorBytes);
+        load_kq<kLo>(base + Lay::KQ + st * Lay::kKQ, &mapk, &mapq, hk, (int)tok0 + c * C, full);
         bulk_load(base + Lay::VEC + st * kVectorBytes, from->in, kVectorBytes, full);
         bulk_load(base + Lay::TG + st * 32768, from->tg, 32768, full);
     };
@@ -201,7 +199,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
         sp = static_cast<ST*>(a.states) + slot * a.s_slot + h * a.s_sh + p * a.s_sk + col;
     auto sum = [](float2 x, float2 y) { return Lay::kWide ? __fadd2_rn(x, y) : x; };
     constexpr int SV = Vec<ST>::V;
-    bf16* op = static_cast<bf16*>(a.out) + tok0 * a.o_st + h * a.o_sh + col;
+    T* op = static_cast<T*>(a.out) + tok0 * a.o_st + h * a.o_sh + col;
 
     // The loop below starts with S <- decay S + product; before the first chunk that is S0 + 0.
 #pragma unroll
@@ -259,13 +257,15 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
         }
         if (c == chunks) break;
         tmem_wait_st();
-        const uint32_t kq = base + Lay::KQ + st * 32768, tg = base + Lay::TG + st * 32768;
+        const uint32_t kq = base + Lay::KQ + st * Lay::kKQ, tg = base + Lay::TG + st * 32768;
         const int left = ntok - c * C;
         if (left < C) {
             // The copies of K went on into the next sequence: zeros there, whatever it holds
             // (rows of Q there make outputs that are not stored).
             for (int e = tid; e < (C - left) * 16; e += Lay::kThreads)
-                sts16(kq + (e % 16 >> 3) * 16384 + swz<128>(left + e / 16, e % 8), 0, 0, 0, 0);
+#pragma unroll
+                for (int part = 0; part <= (kLo ? 1 : 0); ++part)
+                    sts16(kq + part * 32768 + (e % 16 >> 3) * 16384 + swz<128>(left + e / 16, e % 8), 0, 0, 0, 0);
         }
         fence_async_smem();
         tc_fence_before();
@@ -276,11 +276,15 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
             const uint64_t k = operand(kq, 16, 1024, kSwizzle128), s = operand(s_hi, 128 * Lay::kRow, kGroup, kSwz);
             two_part_product<VS, 4, 2, false>(D, k, s, Lay::kS / 16, false);
             two_part_product<VS, 4, 2, false>(D, k + 1024, s + kGroup / 2, Lay::kS / 16, true);
+            if constexpr (kLo) {
+                mma_steps<4, 2, kGroup / 8>(D, k + 2048, s, mma_desc(VS, false, true), true);
+                mma_steps<4, 2, kGroup / 8>(D, k + 3072, s + kGroup / 2, mma_desc(VS, false, true), true);
+            }
             mma_commit(mma);
         }
         // While it runs, a thread with little else to do (six copies take 560 cycles to issue) refills
         // the stage of the chunk before.
-        if (tid == 64 && c > 0 && c - 1 + kStages < chunks) load(c - 1 + kStages, st > 0 ? st - 1 : kStages - 1);
+        if (kStages > 1 && tid == 64 && c > 0 && c - 1 + kStages < chunks) load(c - 1 + kStages, st > 0 ? st - 1 : kStages - 1);
         const float in = vec[st].in[p], out = vec[st].out[p % C];
         decay = vec[st].decay;
         float2 q[W / 2];  // rows of Q: their outputs
@@ -312,7 +316,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
                         float2 f[4];
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            f[k] = add_bf16(live ? vv[k] : 0u, mul2(sum(d[g][4 * u + k], e[g][4 * u + k]), -in));
+                            f[k] = add_pair<T>(live ? vv[k] : 0u, mul2(sum(d[g][4 * u + k], e[g][4 * u + k]), -in));
                         const uint32_t at = swz_cols<VS>(C, p, first / 8 + 2 * g + u);
                         store_split8(r_hi + at, r_lo + at, f);
                     }
@@ -376,16 +380,17 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
         if (lead) {
             tc_fence_after();
             // K^T u
-            two_part_product<VS, 4, 128, true>(D, operand(kq, 16384, 1024, kSwizzle128),
-                                               operand(u_hi, C * Lay::kRow, kGroup, kSwz), Lay::kR / 16, false);
+            const uint64_t k = operand(kq, 16384, 1024, kSwizzle128), u = operand(u_hi, C * Lay::kRow, kGroup, kSwz);
+            two_part_product<VS, 4, 128, true>(D, k, u, Lay::kR / 16, false);
+            if constexpr (kLo) mma_steps<4, 128, kGroup / 8>(D, k + 2048, u, mma_desc(VS, true, true), true);
             mma_commit(mma);
         }
         const int t = c * C + p - C;
         if (p >= C && t < ntok) {
-            bf16* to = op + (int64_t)t * a.o_st;
+            T* to = op + (int64_t)t * a.o_st;
 #pragma unroll
             for (int k = 0; k < W; k += 16) {
-                const uint4 lo = pack16<bf16>(&q[k / 2].x), hi = pack16<bf16>(&q[k / 2 + 4].x);
+                const uint4 lo = pack16<T>(&q[k / 2].x), hi = pack16<T>(&q[k / 2 + 4].x);
                 if (out32) {
                     st32_stream(to + k, lo, hi);
                 } else {
@@ -399,10 +404,15 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
             st_phase ^= 1;
         }
         // The next chunk's K, Q, T, G: there by now, and the look costs less here.
-        if (c + 1 < chunks) mbar_wait(smem_addr(&sh.full[st]), st_phase, &sh.abort);
+        if (kStages > 1 && c + 1 < chunks) mbar_wait(smem_addr(&sh.full[st]), st_phase, &sh.abort);
         mbar_wait(mma, phase, &sh.abort);
         phase ^= 1;
         tc_fence_after();
+        if (kStages == 1 && c + 1 < chunks) {
+            // One stage (fp16 keys and queries take twice the room): refilled between chunks.
+            if (lead) load(c + 1, 0);
+            mbar_wait(smem_addr(&sh.full[0]), st_phase, &sh.abort);
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -428,32 +438,50 @@ Encode encoder() {
     return f;
 }
 
-template <typename ST, int VS>
+// The chunk images, in whole 128-byte lines.
+int64_t images_bytes(const cc1d_gdr_args& a) {
+    return ceil_div(chunk_slots(a.tokens, a.rows) * a.heads_v * (int64_t)sizeof(ChunkImage), 128) * 128;
+}
+
+template <typename T, typename ST, int VS>
 cudaError_t go(const cc1d_gdr_args& a, bool out32, cudaStream_t stream) {
-    using Lay = Layout<VS>;
+    constexpr bool kLo = std::is_same<T, f16>::value;  // fp16 keys and queries come in two bf16 parts
+    using Lay = Layout<VS, kLo>;
     constexpr int smem = Lay::END + 1024;
     const int tiles = a.dv / VS;
     const int64_t grid = a.rows * a.heads_v * tiles;
     if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
     CUtensorMap q, k, v;
-    if (!make_map(&q, a.q, a.tokens, a.heads_k, a.dk, a.q_st, a.q_sh, 64) ||
-        !make_map(&k, a.k, a.tokens, a.heads_k, a.dk, a.k_st, a.k_sh, 64) ||
-        !make_map(&v, a.v, a.tokens, a.heads_v, a.dv, a.v_st, a.v_sh, VS < 64 ? VS : 64))
+    cudaError_t err = cudaSuccess;
+    if constexpr (kLo) {
+        void* parts = static_cast<char*>(a.workspace) + images_bytes(a);
+        err = launch_gdr_split(a, parts, stream);
+        if (err != cudaSuccess) return err;
+        if (!make_map(&k, parts, a.tokens, 4 * a.heads_k, a.dk, 4 * a.heads_k * a.dk, a.dk, 64))
+            return cudaErrorInvalidValue;
+        q = k;
+    } else if (!make_map(&q, a.q, a.tokens, a.heads_k, a.dk, a.q_st, a.q_sh, 64) ||
+               !make_map(&k, a.k, a.tokens, a.heads_k, a.dk, a.k_st, a.k_sh, 64)) {
         return cudaErrorInvalidValue;
-    cudaError_t err = launch_gdr_prep(a, q, k, stream);
+    }
+    if (!make_map(&v, a.v, a.tokens, a.heads_v, a.dv, a.v_st, a.v_sh, VS < 64 ? VS : 64))
+        return cudaErrorInvalidValue;
+    err = launch_gdr_prep(a, q, k, stream);
     if (err != cudaSuccess) return err;
-    err = cudaFuncSetAttribute(gdr_chunk_kernel<ST, VS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    err = cudaFuncSetAttribute(gdr_chunk_kernel<T, ST, VS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (err != cudaSuccess) return err;
-    gdr_chunk_kernel<ST, VS><<<(unsigned)grid, Lay::kThreads, smem, stream>>>(a, q, k, v, tiles, out32);
+    gdr_chunk_kernel<T, ST, VS><<<(unsigned)grid, Lay::kThreads, smem, stream>>>(a, q, k, v, tiles, out32);
     return cudaGetLastError();
 }
 
-template <typename ST>
+template <typename T, typename ST>
 cudaError_t pick(const cc1d_gdr_args& a, bool out32, cudaStream_t stream) {
     const int64_t heads = a.rows * a.heads_v;
-    if (a.dv % 128 == 0 && heads * (a.dv / 128) >= 148) return go<ST, 128>(a, out32, stream);
-    if (a.dv % 64 == 0 && heads * (a.dv / 64) >= 148) return go<ST, 64>(a, out32, stream);
-    return go<ST, 32>(a, out32, stream);
+    // The two parts of fp16 keys and queries leave no room for 128 columns.
+    if constexpr (!std::is_same<T, f16>::value)
+        if (a.dv % 128 == 0 && heads * (a.dv / 128) >= 148) return go<T, ST, 128>(a, out32, stream);
+    if (a.dv % 64 == 0 && heads * (a.dv / 64) >= 148) return go<T, ST, 64>(a, out32, stream);
+    return go<T, ST, 32>(a, out32, stream);
 }
 
 }  // namespace
@@ -473,7 +501,7 @@ bool make_map(CUtensorMap* map, const void* p, int64_t tokens, int heads, int di
 }
 
 int64_t gdr_chunk_workspace(const cc1d_gdr_args& a) {
-    return chunk_slots(a.tokens, a.rows) * a.heads_v * (int64_t)sizeof(ChunkImage);
+    return images_bytes(a) + (a.dtype == CC1D_F16 ? a.tokens * a.heads_k * 4 * DK * 2 : 0);
 }
 
 bool gdr_chunk_serves(const cc1d_gdr_args& a) {
@@ -485,7 +513,7 @@ bool gdr_chunk_serves(const cc1d_gdr_args& a) {
         return rows_ok(p, st, sh, 8) && st > 0 && sh > 0 && st < (1ll << 38) && sh < (1ll << 38);
     };
     const int64_t sv = a.sdtype == CC1D_F32 ? 4 : 8;
-    return a.dtype == CC1D_BF16 && a.dk == DK && a.dv % 32 == 0 && a.q_sd == 1 && a.k_sd == 1 &&
+    return (a.dtype == CC1D_BF16 || a.dtype == CC1D_F16) && a.dk == DK && a.dv % 32 == 0 && a.q_sd == 1 && a.k_sd == 1 &&
            a.v_sd == 1 && a.o_sd == 1 && map_ok(a.q, a.q_st, a.q_sh) && map_ok(a.k, a.k_st, a.k_sh) &&
            map_ok(a.v, a.v_st, a.v_sh) && rows_ok(a.out, a.o_st, a.o_sh, 8) &&
            rows_ok(a.states, a.s_slot, a.s_sh, sv) && a.s_sk % sv == 0 &&
@@ -494,7 +522,9 @@ bool gdr_chunk_serves(const cc1d_gdr_args& a) {
 
 cudaError_t launch_gdr_chunk(const cc1d_gdr_args& a, cudaStream_t stream) {
     const bool out32 = host_aligned32(a.out) && a.o_st % 16 == 0 && a.o_sh % 16 == 0;
-    return a.sdtype == CC1D_F32 ? pick<float>(a, out32, stream) : pick<bf16>(a, out32, stream);
+    if (a.dtype == CC1D_F16)
+        return a.sdtype == CC1D_F32 ? pick<f16, float>(a, out32, stream) : pick<f16, f16>(a, out32, stream);
+    return a.sdtype == CC1D_F32 ? pick<bf16, float>(a, out32, stream) : pick<bf16, bf16>(a, out32, stream);
 }
 
 }  // namespace cc1d

@@ -55,7 +55,30 @@ __device__ __forceinline__ float2 bf16_pair(uint32_t v) {
     return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
 
-// One box (cols x 64 tokens of a head) of the tensor map of a (tokens, heads, dim) bf16 view.
+// fp16 keys and queries as two bf16 parts, which hold their 11 bits: the first kernel of the fp16
+// path writes (tokens, heads_k, 4, 128) bf16, parts k hi, q hi, k lo, q lo, behind the chunk images,
+// and the kernels after it add the products with the low parts.
+template <bool kLo>
+struct Parts {
+    static constexpr int kBytes = kLo ? 65536 : 32768;  // K and Q of a chunk in shared memory
+    static __device__ __forceinline__ int k(int hk) { return kLo ? 4 * hk : hk; }
+    static __device__ __forceinline__ int q(int hk) { return kLo ? 4 * hk + 1 : hk; }
+};
+// K and Q of 64 tokens: [hi, lo][2 halves of 64 columns][K 64 rows, Q 64 rows][128 B].
+template <bool kLo>
+__device__ __forceinline__ void load_kq(uint32_t dst, const CUtensorMap* mapk, const CUtensorMap* mapq,
+                                        int hk, int t, uint32_t bar) {
+#pragma unroll
+    for (int part = 0; part <= (kLo ? 1 : 0); ++part)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const uint32_t at = dst + part * 32768 + half * 16384;
+            tma_load(at, mapk, half * 64, Parts<kLo>::k(hk) + 2 * part, t, bar);
+            tma_load(at + 8192, mapq, half * 64, Parts<kLo>::q(hk) + 2 * part, t, bar);
+        }
+}
+
+// One box (cols x 64 tokens of a head) of the tensor map of a (tokens, heads, dim) view of 16-bit values.
 bool make_map(CUtensorMap* map, const void* p, int64_t tokens, int heads, int dim, int64_t st,
               int64_t sh, int cols);
 // Whether the driver offers tensor maps.
@@ -63,5 +86,7 @@ bool have_maps();
 
 cudaError_t launch_gdr_prep(const cc1d_gdr_args& a, const CUtensorMap& q, const CUtensorMap& k,
                             cudaStream_t stream);
+// The split of fp16 keys and queries, into the workspace at `to`.
+cudaError_t launch_gdr_split(const cc1d_gdr_args& a, void* to, cudaStream_t stream);
 
 }  // namespace cc1d

@@ -33,8 +33,9 @@ struct Gates {
     alignas(16) float nbh[C], nbl[C], beta[C], grow[C], out[C], far[32];
 };
 
+template <bool kLo>
 struct Smem {
-    unsigned char kq[32768];  // [2 halves][K 64 rows, Q 64 rows][128 B]; later T hi, T lo, P hi, P lo
+    unsigned char kq[Parts<kLo>::kBytes];  // K and Q; later T hi, T lo, P hi, P lo
     Blocks blk;
     Gates gates[kHeads];
     alignas(16) float rk[C], ru[kHeads][32];  // inverse norms of the keys; with e^(b_31 - b_j)
@@ -144,11 +145,12 @@ __device__ __forceinline__ float bits_value(uint32_t b, int dtype) {
     return __uint_as_float(b);
 }
 
+template <bool kLo>
 __global__ void __launch_bounds__(128, 4)
 gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__ CUtensorMap mapq,
                 const __grid_constant__ CUtensorMap mapk) {
     extern __shared__ __align__(1024) unsigned char raw[];
-    Smem& sh = *reinterpret_cast<Smem*>(raw + ((1024 - (smem_addr(raw) & 1023)) & 1023));
+    Smem<kLo>& sh = *reinterpret_cast<Smem<kLo>*>(raw + ((1024 - (smem_addr(raw) & 1023)) & 1023));
     const uint32_t kq = smem_addr(sh.kq), tb = kq, pb = kq + 16384;
     const int p = threadIdx.x, w = p / 32, lane = p % 32, i = p % C;
     const int hk = blockIdx.x % a.heads_k;
@@ -189,12 +191,8 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
     const uint32_t lanes = (uint32_t)w << 21;   // the warp's first TMEM lane, in bits 16..
     if (p == 0) {
         const uint32_t full = smem_addr(&sh.full);
-        mbar_expect(full, 32768);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            tma_load(kq + half * 16384, &mapk, half * 64, hk, (int)tok0, full);
-            tma_load(kq + half * 16384 + 8192, &mapq, half * 64, hk, (int)tok0, full);
-        }
+        mbar_expect(full, Parts<kLo>::kBytes);
+        load_kq<kLo>(kq, &mapk, &mapq, hk, (int)tok0, full);
     }
 
     // Gates of one value head by one warp, two tokens a lane: the loads, all at once, and the rest.
@@ -265,7 +263,9 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
         // The copies went on into the next sequence: zeros there, whatever it holds.
         for (int e = p; e < (C - left) * 32; e += 128) {
             const int r = left + e / 32, u = e % 16;
-            sts16(kq + (u >> 3) * 16384 + swz<128>(r + (e & 16) * 4, u & 7), 0, 0, 0, 0);
+#pragma unroll
+            for (int part = 0; part <= (kLo ? 1 : 0); ++part)
+                sts16(kq + part * 32768 + (u >> 3) * 16384 + swz<128>(r + (e & 16) * 4, u & 7), 0, 0, 0, 0);
         }
         fence_async_smem();
     }
@@ -276,6 +276,14 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
         const uint64_t d = operand(kq, 16, 1024, kSwizzle128);
         mma_steps<4, 2, 2>(D0, d, d, mma_desc(64, false, false), false);
         mma_steps<4, 2, 2>(D0, d + 1024, d + 1024, mma_desc(64, false, false), true);
+        if constexpr (kLo) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const uint64_t hi = d + half * 1024, lo = hi + 2048;
+                mma_steps<4, 2, 2>(D0, hi, lo, mma_desc(64, false, false), true);
+                mma_steps<4, 2, 2>(D0, lo, hi, mma_desc(64, false, false), true);
+            }
+        }
         mma_commit(smem_addr(&sh.mma));
     }
     // Norm of row p of [K;Q].
@@ -284,11 +292,13 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll 4
         for (int u = 0; u < 16; ++u) {
-            const uint4 v = lds16(kq + (u >> 3) * 16384 + swz<128>(p, u & 7));
-            const uint32_t vv[4] = {v.x, v.y, v.z, v.w};
+            const uint32_t at = kq + (u >> 3) * 16384 + swz<128>(p, u & 7);
+            const uint4 v = lds16(at), l = kLo ? lds16(at + 32768) : make_uint4(0, 0, 0, 0);
+            const uint32_t vv[4] = {v.x, v.y, v.z, v.w}, ll[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float2 f = bf16_pair(vv[e]);
+                float2 f = bf16_pair(vv[e]);
+                if (kLo) f = add_pair<bf16>(ll[e], f);
                 sum[e % 2] = __ffma2_rn(f, f, sum[e % 2]);
             }
         }
@@ -502,17 +512,51 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
     if (p == 0 && sh.abort) flag_status(a.dev_status, CC1D_DEV_TIMEOUT);
 }
 
+// fp16 keys and queries to bf16 parts, four values a lane; bound by HBM. One warp per token and head.
+__global__ void __launch_bounds__(256)
+gdr_split_kernel(const __grid_constant__ cc1d_gdr_args a, uint2* to) {
+    const int64_t item = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+    if (item >= a.tokens * a.heads_k) return;
+    const int64_t t = item / a.heads_k;
+    const int h = (int)(item - t * a.heads_k), lane = threadIdx.x % 32;
+    const f16* src[2] = {static_cast<const f16*>(a.k) + t * a.k_st + h * a.k_sh,
+                         static_cast<const f16*>(a.q) + t * a.q_st + h * a.q_sh};
+    uint2* dst = to + item * (4 * DK / 4) + lane;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        const uint2 v = ldg_raw<8>(src[m] + 4 * lane);
+        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&v.x));
+        const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+        uint2 hi, lo;
+        split2(x, hi.x, lo.x);
+        split2(y, hi.y, lo.y);
+        dst[m * (DK / 4)] = hi;
+        dst[(2 + m) * (DK / 4)] = lo;
+    }
+}
+
 }  // namespace
 
 cudaError_t launch_gdr_prep(const cc1d_gdr_args& a, const CUtensorMap& q, const CUtensorMap& k,
                             cudaStream_t stream) {
-    constexpr int smem = (int)sizeof(Smem) + 1024;
-    const cudaError_t err =
-        cudaFuncSetAttribute(gdr_prep_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (err != cudaSuccess) return err;
     const int64_t grid = chunk_slots(a.tokens, a.rows) * a.heads_k;
     if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
-    gdr_prep_kernel<<<(unsigned)grid, 128, smem, stream>>>(a, q, k);
+    auto go = [&](auto lo) {
+        constexpr bool kLo = decltype(lo)::value;
+        constexpr int smem = (int)sizeof(Smem<kLo>) + 1024;
+        const cudaError_t err = cudaFuncSetAttribute(
+            gdr_prep_kernel<kLo>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (err != cudaSuccess) return err;
+        gdr_prep_kernel<kLo><<<(unsigned)grid, 128, smem, stream>>>(a, q, k);
+        return cudaGetLastError();
+    };
+    return a.dtype == CC1D_F16 ? go(std::true_type()) : go(std::false_type());
+}
+
+cudaError_t launch_gdr_split(const cc1d_gdr_args& a, void* to, cudaStream_t stream) {
+    const int64_t grid = ceil_div(a.tokens * a.heads_k, 8);
+    if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
+    gdr_split_kernel<<<(unsigned)grid, 256, 0, stream>>>(a, static_cast<uint2*>(to));
     return cudaGetLastError();
 }
 

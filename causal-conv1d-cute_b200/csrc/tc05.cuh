@@ -214,9 +214,19 @@ __device__ __forceinline__ void split2(float2 f, uint32_t& hi, uint32_t& lo) {
         : "r"(hi), "f"(f.x), "f"(f.y));
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(r.y), "f"(r.x));
 }
-// A bf16 pair plus two fp32 values.
-__device__ __forceinline__ float2 add_bf16(uint32_t v, float2 f) {
+// A pair of T (bf16 or fp16) plus two fp32 values.
+template <typename T>
+__device__ __forceinline__ float2 add_pair(uint32_t v, float2 f) {
     float2 r;
+    if constexpr (std::is_same<T, f16>::value) {
+        asm("{\n\t.reg .b16 l, h;\n\t"
+            "mov.b32 {l, h}, %2;\n\t"
+            "add.rn.f32.f16 %0, l, %3;\n\t"
+            "add.rn.f32.f16 %1, h, %4;\n\t}"
+            : "=f"(r.x), "=f"(r.y)
+            : "r"(v), "f"(f.x), "f"(f.y));
+        return r;
+    }
     asm("{\n\t.reg .b16 l, h;\n\t"
         "mov.b32 {l, h}, %2;\n\t"
         "add.rn.f32.bf16 %0, l, %3;\n\t"

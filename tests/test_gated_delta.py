@@ -242,12 +242,12 @@ def test_varlen_batches(lengths):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("n", [13, 25, 60, 300])
-@pytest.mark.parametrize("sdtype", [F32, BF])
-def test_varlen_many_sequences(n, sdtype):
+@pytest.mark.parametrize("dtype,sdtype", [(BF, F32), (BF, BF), (F16, F32), (F16, F16)])
+def test_varlen_many_sequences(n, dtype, sdtype):
     """Enough (sequence, head) pairs to fill the GPU with each width of a work tile; uneven lengths."""
     r = torch.Generator().manual_seed(n)
     lengths = torch.randint(0, 150, (n,), generator=r).tolist()
-    varlen_case(lengths, hk=1, hv=6, sdtype=sdtype, seed=n)
+    varlen_case(lengths, hk=1, hv=6, dtype=dtype, sdtype=sdtype, seed=n)
 
 
 @pytest.mark.gpu
@@ -299,11 +299,12 @@ def test_varlen_strong_and_total_decay(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
-def test_varlen_sequences_do_not_see_each_other(bad):
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_varlen_sequences_do_not_see_each_other(bad, dtype):
     """Values that are not finite in one sequence stay in it, tails of its chunks included."""
     lengths = [70, 33, 129, 64]
     T = sum(lengths)
-    q, k, v, g, b, A, dt = (gpu(t) for t in make(T, 2, 4, 128, 128, BF))
+    q, k, v, g, b, A, dt = (gpu(t) for t in make(T, 2, 4, 128, 128, dtype))
     start = torch.tensor([0] + list(itertools.accumulate(lengths)), dtype=torch.int32)
     st = torch.randn(4, 4, 128, 128, device="cuda")
     hinit = torch.ones(4, dtype=torch.bool, device="cuda")

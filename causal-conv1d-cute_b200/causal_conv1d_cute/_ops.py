@@ -218,6 +218,18 @@ def _update_unpack_impl(qkvz, ba, state, weight, bias, out, z, b, a, idx, heads,
     return out, z, b, a
 
 
+def _run(device, f, *args):
+    """Call a C entry point with device current (the default stream does not name its device)."""
+    if torch.cuda.current_device() == device.index:
+        return check(f(*args, _stream(device)))
+    with torch.cuda.device(device):
+        return check(f(*args, _stream(device)))
+
+
+# Most bytes of the packed delta rule's workspace: larger calls go in groups of heads.
+_GDR_WORKSPACE = 4 << 30
+
+
 def _gdr_args(q, k, v, g, beta, a_log, dt_bias, out, states, inter, idx, iidx, qsl, hinit, rows,
               tokens, steps, scale, l2norm, update, pad, workspace=None):
     """The packed cc1d_gdr_args; the token-major tensors are (rows, steps, ...) or (tokens, ...)."""
@@ -251,21 +263,40 @@ def _gdr_update_impl(q, k, v, g, beta, a_log, dt_bias, out, states, idx, inter, 
         q, k, v, g, beta, out = (t.unsqueeze(1) for t in (q, k, v, g, beta, out))
     args = _gdr_args(q, k, v, g, beta, a_log, dt_bias, out, states, inter, idx, iidx, None, None,
                      q.shape[0], 0, q.shape[1], scale, l2norm, update, pad)
-    check(load().cc1d_gdr_update(args, _stream(q.device)))
+    _run(q.device, load().cc1d_gdr_update, args)
 
 
 def _gdr_varlen_impl(q, k, v, g, beta, a_log, dt_bias, out, states, qsl, idx, hinit, scale,
                      l2norm, pad):
     """Gated delta rule over packed sequences (cc1d_gdr_varlen): (tokens, heads, dim)."""
     lib = load()
-    call = (q, k, v, g, beta, a_log, dt_bias, out, states, None, idx, None, qsl, hinit,
-            qsl.numel() - 1, q.shape[0], 0, scale, l2norm, True, pad)
-    args, need = _gdr_args(*call), ctypes.c_int64()
+
+    def heads(x, i, n, axis=1):
+        return None if x is None else x.narrow(axis, i, n)
+
+    def call(hk0, hks, workspace=None):
+        r = v.shape[1] // q.shape[1]
+        h0, hs = hk0 * r, hks * r
+        part = hks < q.shape[1]
+        qk = [x.narrow(1, hk0, hks) if part else x for x in (q, k)]
+        vs = [heads(x, h0, hs) if part else x for x in (v, g, beta)]
+        par = [heads(x, h0, hs, 0) if part else x for x in (a_log, dt_bias)]
+        os = [heads(x, h0, hs) if part else x for x in (out, states)]
+        return _gdr_args(*qk, *vs, *par, *os, None, idx, None, qsl, hinit, qsl.numel() - 1, q.shape[0],
+                         0, scale, l2norm, True, pad, workspace)
+
+    hk = q.shape[1]
+    args, need = call(0, hk), ctypes.c_int64()
     check(lib.cc1d_gdr_workspace(args, ctypes.byref(need)))
-    if need.value:
-        # From the caching allocator, on the current stream: reused by the stream's later work only.
-        args = _gdr_args(*call, torch.empty(need.value, dtype=torch.uint8, device=q.device))
-    check(lib.cc1d_gdr_varlen(args, _stream(q.device)))
+    if not need.value:
+        return _run(q.device, lib.cc1d_gdr_varlen, args)
+    # Heads do not depend on one another. The workspace is the caching allocator's, on the current
+    # stream: reused by the stream's later work only.
+    groups = min(hk, -(-need.value // _GDR_WORKSPACE))
+    step = -(-hk // groups)
+    space = torch.empty(-(-need.value // hk) * step + 128, dtype=torch.uint8, device=q.device)
+    for at in range(0, hk, step):
+        _run(q.device, lib.cc1d_gdr_varlen, call(at, min(step, hk - at), space))
 
 
 def _rms_norm_gated_impl(x, z, weight, eps, out):
@@ -276,23 +307,22 @@ def _rms_norm_gated_impl(x, z, weight, eps, out):
         out.stride(0), out.stride(1), *x.shape,
         dtype_code(x.dtype), dtype_code(weight.dtype), eps,
     )
-    check(load().cc1d_rms_norm_gated(args, _stream(x.device)))
+    _run(x.device, load().cc1d_rms_norm_gated, args)
 
 
 def _slots_copy_impl(caches, sources, table, ncaches, src, dst, src_slots, dst_slots, pad):
     """Slot copies between caches (cc1d_slots_copy); table is the address of a cc1d_slot_cache
     array that describes caches (and sources, where they are not the caches themselves)."""
     dev = caches[0].device
-    check(load().cc1d_slots_copy(table, ncaches, src.data_ptr(), dst.data_ptr(), src.numel(),
-                                 src_slots, dst_slots, pad, _status_ptr(dev), _stream(dev)))
+    _run(dev, load().cc1d_slots_copy, table, ncaches, src.data_ptr(), dst.data_ptr(), src.numel(),
+         src_slots, dst_slots, pad, _status_ptr(dev))
 
 
 def _slots_compact_impl(caches, table, ncaches, live, remap, count, moves):
     """Live slots to the front of the caches (cc1d_slots_compact)."""
     dev = live.device
-    check(load().cc1d_slots_compact(table or None, ncaches, live.data_ptr(), live.numel(),
-                                    remap.data_ptr(), count.data_ptr(), moves.data_ptr(),
-                                    _stream(dev)))
+    _run(dev, load().cc1d_slots_compact, table or None, ncaches, live.data_ptr(), live.numel(),
+         remap.data_ptr(), count.data_ptr(), moves.data_ptr())
 
 
 # ---------------------------------------------------------------------------------------------

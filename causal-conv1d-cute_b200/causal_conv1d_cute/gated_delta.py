@@ -75,6 +75,12 @@ def gated_delta_rule_reason(q, k, v, g, beta, states=None, A_log=None, dt_bias=N
     return None
 
 
+def _index(index, device):
+    """Slot indices as contiguous int32 on device; None stays None."""
+    index = _int32(index, device)
+    return index if index is None or index.is_contiguous() else index.contiguous()
+
+
 def gated_delta_rule_varlen_fn(
     q,
     k,
@@ -110,6 +116,10 @@ def gated_delta_rule_varlen_fn(
             and their slots untouched).
         out: optional output of the shape and dtype of v.
 
+    bf16 and fp16 calls with dk = 128, rows on 16-byte boundaries and 16 tokens a sequence on average
+    run chunk by chunk on the tensor cores, with a temporary of 524 bytes per token and value head (in
+    groups of heads from 4 GiB on); others token by token in fp32.
+
     Returns:
         (total_tokens, heads_v, dv) output.
     """
@@ -131,9 +141,11 @@ def gated_delta_rule_varlen_fn(
         raise ValueError(f"states has {states.shape[0]} slots for {n} sequences and no cache_indices")
     out = _output(out, v)
     dev = q.device
-    qsl = query_start_loc if query_start_loc.device == dev else query_start_loc.to(dev)
-    idx = _int32(cache_indices, dev) if states is not None else None
+    qsl = _index(query_start_loc, dev)
+    idx = _index(cache_indices, dev) if states is not None else None
     hinit = _flags(has_initial_state, dev) if states is not None else None
+    if hinit is not None and not hinit.is_contiguous():
+        hinit = hinit.contiguous()
     _ops.gdr_varlen(q, k, v, g, beta, A_log, dt_bias, out, states, qsl, idx, hinit,
                     q.shape[-1] ** -0.5 if scale is None else scale, qk_l2norm, pad_slot_id)
     return out
@@ -264,8 +276,8 @@ def gated_delta_rule_update(
         raise ValueError(f"states has {states.shape[0]} slots for {B} rows and no state_indices")
     out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
     dev = q.device
-    idx = _int32(state_indices, dev)
-    iidx = _int32(intermediate_state_indices, dev) if inter is not None else None
+    idx = _index(state_indices, dev)
+    iidx = _index(intermediate_state_indices, dev) if inter is not None else None
     _ops.gdr_update(q, k, v, g, beta, A_log, dt_bias, out, states, idx, inter, iidx,
                     q.shape[-1] ** -0.5 if scale is None else scale, qk_l2norm, update_states,
                     pad_slot_id)

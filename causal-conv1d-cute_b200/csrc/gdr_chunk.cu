@@ -9,12 +9,16 @@
 //     u    = T R,      o_i = s_i e^(b_i) S0^T q_i + (G R)_i
 //     S    = e^(b_C) S0 + sum_j k_j (r_j e^(b_C - b_j) u_j)^T.
 // k and q enter every product as the caller's bf16 values (fp16 ones as two bf16 parts), which are
-// exact; norms, gates and
-// decays scale rows in fp32 outside the products. All exponents are differences b_i - b_j <= 0.
+// exact; norms, gates and decays scale rows in fp32 outside the products. All exponents are
+// differences b_i - b_j <= 0. Within a chunk, as in any chunked form, a value that is not finite
+// spoils the rows of its chunk, earlier ones included; it reaches no earlier chunk, and no other
+// sequence (rows behind a sequence's end are zeroed).
 //
 // Precision. S, R, T, G and u are fp32 quantities. As operands they are split into two bf16 parts
-// (2^-17), and the products keep hi*hi + hi*lo + lo*hi, so that fp32 final states are good to about
-// 1e-5 where a single bf16 rounding would leave 2e-3. The state itself stays in fp32 registers.
+// (2^-17), and the products keep hi*hi + hi*lo + lo*hi: fp32 final states come out within 6e-6 of
+// the definition (2-norm, worst of 60 drawn batches, median 3e-6), where single bf16 operands would
+// leave 2e-3 and three parts would cost 1.6 times the products. Outputs of 16 bits are within 1.01 of
+// their own rounding. The state itself is carried in fp32 in tensor memory.
 //
 // Split of the work. Chunks of one sequence form a chain; heads, sequences and the columns of the
 // state are independent. T, G and the row factors do not depend on the state: a first kernel
@@ -22,15 +26,22 @@
 // chunk and head. (One kernel with warps for either part was tried first: a chunk's T and G take
 // longer than its step of the chain, and shared memory has no room for more of them in flight.)
 // The kernel here walks the chain: [K;Q] S0, R, [T;G] R, u, K^T u, S. A CTA takes one head of one
-// sequence and VS state columns; K, Q, T and G come by TMA and bulk copies a chunk or two ahead. The
-// state lies in TMEM. (Two chains of 64 columns in one CTA took 7700 cycles a chunk and one of 128
-// columns takes XXXX: tensor memory serves the products of one and the loads of the other in turn.)
+// sequence and VS state columns; all its warps turn a product into the operand of the next together.
+// K, Q, T and G come by TMA and bulk copies a chunk or two ahead.
+//
+// Bound. The latency of the chain: 2950 cycles a chunk at VS = 32, of which the products take half
+// and the rest is TMEM loads, splitting, barriers. At VS = 128 (6800 cycles) also the integer pipe
+// (four half-rate instructions per split pair) and shared memory, of whose 128 bytes a cycle the
+// products take 2400 cycles' worth, the operands written for them 1000 and the loads 650. Tried and
+// slower at 128 columns: two independent chains of 64 in one CTA (7700 cycles), and two tiles in
+// turn, with warps of their own for products and loads (7400; 3500 at 32 columns): a product that
+// runs beside operand stores takes up to three times as long, and hand-overs by mbarrier cost more
+// than the barrier of one CTA.
+//
 // Stacking K over Q and T over G makes every product M = 128, the full tensor core rate; the two
 // parts of an operand lie side by side as one operand of 2 VS columns (measured: a K step of 16
 // costs 46 cycles up to 64 columns, 66 with 128 and 137 with 256, so one wide step beats two narrow
 // ones up to VS = 64).
-// Loops over columns stay rolled where registers allow it: with all of them unrolled the warps
-// spent a quarter of their time waiting for instructions.
 #include "gdr_chunk.cuh"
 
 namespace cc1d {
@@ -45,7 +56,7 @@ struct Layout {
     static constexpr int kS = 128 * kRow * kAtoms;        // one part (hi or lo) of S
     static constexpr int kR = C * kRow * kAtoms;          // one part of R or u, or V
     static constexpr int kKQ = Parts<kLo>::kBytes;
-    static constexpr int kStages = kLo ? 1 : VS <= 32 ? 3 : 2;
+    static constexpr int kStages = VS <= 32 ? (kLo ? 2 : 3) : kLo ? 1 : 2;
     static constexpr int KQ = 0;                          // stages x K and Q
     static constexpr int TG = KQ + kStages * kKQ;         // stages x [hi, lo][128 rows][128 B]
     static constexpr int SB = TG + kStages * 32768;       // S hi, S lo; R in S hi, u in S lo
@@ -476,11 +487,14 @@ cudaError_t go(const cc1d_gdr_args& a, bool out32, cudaStream_t stream) {
 
 template <typename T, typename ST>
 cudaError_t pick(const cc1d_gdr_args& a, bool out32, cudaStream_t stream) {
-    const int64_t heads = a.rows * a.heads_v;
-    // The two parts of fp16 keys and queries leave no room for 128 columns.
-    if constexpr (!std::is_same<T, f16>::value)
-        if (a.dv % 128 == 0 && heads * (a.dv / 128) >= 148) return go<T, ST, 128>(a, out32, stream);
-    if (a.dv % 64 == 0 && heads * (a.dv / 64) >= 148) return go<T, ST, 64>(a, out32, stream);
+    // Columns per CTA. A chunk's step takes 1.7, 2.6 and 3.7 us with 32, 64 and 128 columns: wide
+    // tiles do more per SM, narrow ones finish a chain sooner. Many heads take the widest (768 heads,
+    // 16384 tokens: 798, 595, 530 us with 32, 64, 128; 384 heads 745, 562, 530; 192 heads 808, 607,
+    // 890), few that leave SMs free the narrowest (12 heads, 4096 tokens: 126, 160, 250; 24 heads
+    // 139, 173, 265; 48 heads in one sequence 262, 196, 289, in four 105, 130, 203 for 4096).
+    const int64_t heads = a.rows * a.heads_v, narrow = heads * (a.dv / 32);
+    if (a.dv % 128 == 0 && heads * (a.dv / 128) >= 370) return go<T, ST, 128>(a, out32, stream);
+    if (a.dv % 64 == 0 && narrow > (a.rows >= 4 ? 296 : 148)) return go<T, ST, 64>(a, out32, stream);
     return go<T, ST, 32>(a, out32, stream);
 }
 

@@ -389,6 +389,44 @@ def test_varlen_strided_cache(shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("limit", [1, 500_000, 1_300_000])
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_varlen_in_groups_of_heads(monkeypatch, limit, dtype):
+    """A workspace above its limit: the heads in groups, uneven ones too, bit for bit the same."""
+    from causal_conv1d_cute import _ops
+
+    lengths = [100, 65, 3]
+    q, k, v, g, b, A, dt = (gpu(t) for t in make(sum(lengths), 5, 10, 128, 128, dtype))
+    start = torch.tensor([0] + list(itertools.accumulate(lengths)), dtype=torch.int32, device="cuda")
+
+    def run():
+        s = torch.ones(3, 10, 128, 128, device="cuda")
+        hinit = torch.ones(3, dtype=torch.bool, device="cuda")
+        return C.gated_delta_rule_varlen_fn(q, k, v, g, b, start, None, hinit, s, A_log=A, dt_bias=dt, qk_l2norm=True), s
+
+    o0, s0 = run()
+    monkeypatch.setattr(_ops, "_GDR_WORKSPACE", limit)
+    o1, s1 = run()
+    assert torch.equal(o0, o1) and torch.equal(s0, s1)
+
+
+@pytest.mark.gpu
+def test_strided_index_tensors():
+    q, k, v, g, b, A, dt = (gpu(t) for t in make(130, 1, 2, 128, 128, BF))
+    kw = dict(A_log=A, dt_bias=dt, qk_l2norm=True)
+    wide = lambda x, t: torch.stack([torch.tensor(x, dtype=t), torch.full((len(x),), 7, dtype=t)], 1).cuda()[:, 0]  # noqa: E731
+    i32 = torch.int32
+    a, s = [], []
+    for view in (lambda t: t, lambda t: t.contiguous()):
+        st = torch.ones(4, 2, 128, 128, device="cuda")
+        a.append(C.gated_delta_rule_varlen_fn(q, k, v, g, b, view(wide([0, 70, 130], i32)), view(wide([3, 0], i32)),
+                                              view(wide([1, 0], torch.uint8)), st, **kw))
+        a.append(C.gated_delta_rule_update(q[:2], k[:2], v[:2], g[:2], b[:2], st, view(wide([2, 3], i32)), **kw))
+        s.append(st)
+    assert torch.equal(a[0], a[2]) and torch.equal(a[1], a[3]) and torch.equal(s[0], s[1])
+
+
+@pytest.mark.gpu
 def test_varlen_bad_indices_are_skipped_and_reported(request):
     request.node._expect_status = True
     lengths = [65, 66, 67]

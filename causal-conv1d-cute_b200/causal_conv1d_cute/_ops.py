@@ -271,32 +271,31 @@ def _gdr_varlen_impl(q, k, v, g, beta, a_log, dt_bias, out, states, qsl, idx, hi
     """Gated delta rule over packed sequences (cc1d_gdr_varlen): (tokens, heads, dim)."""
     lib = load()
 
-    def heads(x, i, n, axis=1):
-        return None if x is None else x.narrow(axis, i, n)
+    def call(*tensors, workspace=None):
+        return _gdr_args(*tensors, None, idx, None, qsl, hinit, qsl.numel() - 1, q.shape[0], 0, scale,
+                         l2norm, True, pad, workspace)
 
-    def call(hk0, hks, workspace=None):
-        r = v.shape[1] // q.shape[1]
-        h0, hs = hk0 * r, hks * r
-        part = hks < q.shape[1]
-        qk = [x.narrow(1, hk0, hks) if part else x for x in (q, k)]
-        vs = [heads(x, h0, hs) if part else x for x in (v, g, beta)]
-        par = [heads(x, h0, hs, 0) if part else x for x in (a_log, dt_bias)]
-        os = [heads(x, h0, hs) if part else x for x in (out, states)]
-        return _gdr_args(*qk, *vs, *par, *os, None, idx, None, qsl, hinit, qsl.numel() - 1, q.shape[0],
-                         0, scale, l2norm, True, pad, workspace)
+    def heads(x, at, n, axis=1):
+        return None if x is None else x.narrow(axis, at, n)
 
-    hk = q.shape[1]
-    args, need = call(0, hk), ctypes.c_int64()
+    whole = (q, k, v, g, beta, a_log, dt_bias, out, states)
+    args, need = call(*whole), ctypes.c_int64()
     check(lib.cc1d_gdr_workspace(args, ctypes.byref(need)))
     if not need.value:
         return _run(q.device, lib.cc1d_gdr_varlen, args)
-    # Heads do not depend on one another. The workspace is the caching allocator's, on the current
-    # stream: reused by the stream's later work only.
-    groups = min(hk, -(-need.value // _GDR_WORKSPACE))
-    step = -(-hk // groups)
-    space = torch.empty(-(-need.value // hk) * step + 128, dtype=torch.uint8, device=q.device)
-    for at in range(0, hk, step):
-        _run(q.device, lib.cc1d_gdr_varlen, call(at, min(step, hk - at), space))
+    # The workspace is the caching allocator's, on the current stream: reused by the stream's later
+    # work only. Heads do not depend on one another, so a call that would need too much goes in groups.
+    hk, r = q.shape[1], v.shape[1] // q.shape[1]
+    n = -(-hk // min(hk, -(-need.value // _GDR_WORKSPACE)))
+    space = torch.empty(-(-need.value // hk) * n + 128, dtype=torch.uint8, device=q.device)
+    if n == hk:
+        return _run(q.device, lib.cc1d_gdr_varlen, call(*whole, workspace=space))
+    for at in range(0, hk, n):
+        m = min(n, hk - at)
+        part = (heads(q, at, m), heads(k, at, m), *(heads(x, at * r, m * r) for x in (v, g, beta)),
+                *(heads(x, at * r, m * r, 0) for x in (a_log, dt_bias)),
+                *(heads(x, at * r, m * r) for x in (out, states)))
+        _run(q.device, lib.cc1d_gdr_varlen, call(*part, workspace=space))
 
 
 def _rms_norm_gated_impl(x, z, weight, eps, out):

@@ -116,7 +116,7 @@ def gated_delta_rule_varlen_fn(
             and their slots untouched).
         out: optional output of the shape and dtype of v.
 
-    bf16 and fp16 calls with dk = 128, rows on 16-byte boundaries and 16 tokens a sequence on average
+    bf16 and fp16 calls with dk = 128, rows on 16-byte boundaries and 10 tokens a sequence on average
     run chunk by chunk on the tensor cores, with a temporary of 524 bytes per token and value head (in
     groups of heads from 4 GiB on); others token by token in fp32.
 

@@ -188,6 +188,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
         for (int at = 0; at < Lay::kAtoms; ++at)
             tma_load(base + Lay::V + at * C * Lay::kRow, &mapv, vt * VS + at * 64, h, (int)tok0 + c * C, full);
     };
+    grid_dependency_wait();  // for the prep kernel's images
     if (tid == 0) {
         for (int c = 0; c < kStages && c < chunks; ++c) load(c, c);
         load_v(0);
@@ -481,8 +482,17 @@ cudaError_t go(const cc1d_gdr_args& a, bool out32, cudaStream_t stream) {
     if (err != cudaSuccess) return err;
     err = cudaFuncSetAttribute(gdr_chunk_kernel<T, ST, VS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (err != cudaSuccess) return err;
-    gdr_chunk_kernel<T, ST, VS><<<(unsigned)grid, Lay::kThreads, smem, stream>>>(a, q, k, v, tiles, out32);
-    return cudaGetLastError();
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(Lay::kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, gdr_chunk_kernel<T, ST, VS>, a, q, k, v, tiles, out32);
 }
 
 template <typename T, typename ST>
@@ -527,11 +537,14 @@ bool gdr_chunk_serves(const cc1d_gdr_args& a) {
         return rows_ok(p, st, sh, 8) && st > 0 && sh > 0 && st < (1ll << 38) && sh < (1ll << 38);
     };
     const int64_t sv = a.sdtype == CC1D_F32 ? 4 : 8;
+    // Token by token is faster up to some 10 tokens a sequence (measured, uneven lengths: 6 heads,
+    // one sequence of 12 tokens 17 us against 19, four of 6 on average 21 against 19; 128 sequences
+    // x 48 heads, 8 on average, 492 against 621, 12 on average 696 against 625).
     return (a.dtype == CC1D_BF16 || a.dtype == CC1D_F16) && a.dk == DK && a.dv % 32 == 0 && a.q_sd == 1 && a.k_sd == 1 &&
            a.v_sd == 1 && a.o_sd == 1 && map_ok(a.q, a.q_st, a.q_sh) && map_ok(a.k, a.k_st, a.k_sh) &&
            map_ok(a.v, a.v_st, a.v_sh) && rows_ok(a.out, a.o_st, a.o_sh, 8) &&
            rows_ok(a.states, a.s_slot, a.s_sh, sv) && a.s_sk % sv == 0 &&
-           a.tokens >= 16 * a.rows && have_maps();
+           a.tokens >= 10 * a.rows && have_maps();
 }
 
 cudaError_t launch_gdr_chunk(const cc1d_gdr_args& a, cudaStream_t stream) {

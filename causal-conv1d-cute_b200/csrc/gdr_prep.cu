@@ -158,6 +158,8 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
     const int hk = blockIdx.x % a.heads_k;
     const int64_t image = blockIdx.x / a.heads_k;
 
+    // The scan kernel may come up (its CTAs wait there for this kernel's end).
+    allow_dependent_launch();
     // The sequence whose chunk this is.
     if (p == 0) sh.seq = -1;
     __syncthreads();

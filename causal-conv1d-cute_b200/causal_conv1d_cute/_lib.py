@@ -53,6 +53,9 @@ SIGNATURES = {
 # host less than setting the fields of a ctypes structure: pointers, then int64, int32 and float.
 GDR_ARGS = struct.Struct("16P34q13if")
 NORM_ARGS = struct.Struct("4P9q2if4x")
+# The workspace's fields in the first: the last pointer and the last int64.
+GDR_WORKSPACE, GDR_WORKSPACE_AT = struct.Struct("P"), 15 * 8
+GDR_WORKSPACE_BYTES, GDR_WORKSPACE_BYTES_AT = struct.Struct("q"), (16 + 33) * 8
 
 EXPORTS = ("cc1d_abi_version", "cc1d_status_string", "cc1d_last_error", *SIGNATURES)
 

@@ -218,12 +218,18 @@ def _update_unpack_impl(qkvz, ba, state, weight, bias, out, z, b, a, idx, heads,
     return out, z, b, a
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def _run(device, f, *args):
     """Call a C entry point with device current (the default stream does not name its device)."""
-    if torch.cuda.current_device() == device.index:
-        return check(f(*args, _stream(device)))
-    with torch.cuda.device(device):
-        return check(f(*args, _stream(device)))
+    if _current_device() == device.index:
+        status = f(*args, _stream(device))
+    else:
+        with torch.cuda.device(device):
+            status = f(*args, _stream(device))
+    if status:
+        check(status)
 
 
 # Most bytes of the packed delta rule's workspace: larger calls go in groups of heads.
@@ -231,7 +237,7 @@ _GDR_WORKSPACE = 4 << 30
 
 
 def _gdr_args(q, k, v, g, beta, a_log, dt_bias, out, states, inter, idx, iidx, qsl, hinit, rows,
-              tokens, steps, scale, l2norm, update, pad, workspace=None):
+              tokens, steps, scale, l2norm, update, pad):
     """The packed cc1d_gdr_args; the token-major tensors are (rows, steps, ...) or (tokens, ...)."""
     zero = (0,) if q.dim() == 3 else ()
     ss, nslots = ((0, 0, 0), 0) if states is None else (states.stride()[:3], states.shape[0])
@@ -243,16 +249,24 @@ def _gdr_args(q, k, v, g, beta, a_log, dt_bias, out, states, inter, idx, iidx, q
         0 if inter is None else inter.data_ptr(),
         0 if idx is None else idx.data_ptr(), 0 if iidx is None else iidx.data_ptr(),
         0 if qsl is None else qsl.data_ptr(), 0 if hinit is None else hinit.data_ptr(),
-        _status_ptr(q.device) or 0, 0 if workspace is None else workspace.data_ptr(),
+        (_status_ptr(q.device) or 0) if _checks else 0, 0,
         *zero, *q.stride(), *zero, *k.stride(), *zero, *v.stride(), *zero, *out.stride(),
         *zero, *g.stride(), *zero, *beta.stride(), *ss, *si,
-        rows, tokens, nslots, ni, 0 if workspace is None else workspace.numel(),
+        rows, tokens, nslots, ni, 0,
         steps, q.shape[-2], v.shape[-2], q.shape[-1], v.shape[-1],
         dtype_code(q.dtype), dtype_code(g.dtype), dtype_code(beta.dtype),
         F32 if a_log is None else dtype_code(a_log.dtype),
         F32 if states is None else dtype_code(states.dtype),
         int(l2norm), int(update), pad, scale,
     )
+
+
+def _with_workspace(args, workspace):
+    """The same argument block with a workspace tensor."""
+    block = bytearray(args)
+    _lib.GDR_WORKSPACE.pack_into(block, _lib.GDR_WORKSPACE_AT, workspace.data_ptr())
+    _lib.GDR_WORKSPACE_BYTES.pack_into(block, _lib.GDR_WORKSPACE_BYTES_AT, workspace.numel())
+    return bytes(block)
 
 
 def _gdr_update_impl(q, k, v, g, beta, a_log, dt_bias, out, states, idx, inter, iidx, scale,
@@ -271,15 +285,8 @@ def _gdr_varlen_impl(q, k, v, g, beta, a_log, dt_bias, out, states, qsl, idx, hi
     """Gated delta rule over packed sequences (cc1d_gdr_varlen): (tokens, heads, dim)."""
     lib = load()
 
-    def call(*tensors, workspace=None):
-        return _gdr_args(*tensors, None, idx, None, qsl, hinit, qsl.numel() - 1, q.shape[0], 0, scale,
-                         l2norm, True, pad, workspace)
-
-    def heads(x, at, n, axis=1):
-        return None if x is None else x.narrow(axis, at, n)
-
-    whole = (q, k, v, g, beta, a_log, dt_bias, out, states)
-    args, need = call(*whole), ctypes.c_int64()
+    rest = (None, idx, None, qsl, hinit, qsl.numel() - 1, q.shape[0], 0, scale, l2norm, True, pad)
+    args, need = _gdr_args(q, k, v, g, beta, a_log, dt_bias, out, states, *rest), ctypes.c_int64()
     check(lib.cc1d_gdr_workspace(args, ctypes.byref(need)))
     if not need.value:
         return _run(q.device, lib.cc1d_gdr_varlen, args)
@@ -289,13 +296,17 @@ def _gdr_varlen_impl(q, k, v, g, beta, a_log, dt_bias, out, states, qsl, idx, hi
     n = -(-hk // min(hk, -(-need.value // _GDR_WORKSPACE)))
     space = torch.empty(-(-need.value // hk) * n + 128, dtype=torch.uint8, device=q.device)
     if n == hk:
-        return _run(q.device, lib.cc1d_gdr_varlen, call(*whole, workspace=space))
+        return _run(q.device, lib.cc1d_gdr_varlen, _with_workspace(args, space))
+
+    def heads(x, at, n, axis=1):
+        return None if x is None else x.narrow(axis, at, n)
+
     for at in range(0, hk, n):
         m = min(n, hk - at)
         part = (heads(q, at, m), heads(k, at, m), *(heads(x, at * r, m * r) for x in (v, g, beta)),
                 *(heads(x, at * r, m * r, 0) for x in (a_log, dt_bias)),
                 *(heads(x, at * r, m * r) for x in (out, states)))
-        _run(q.device, lib.cc1d_gdr_varlen, call(*part, workspace=space))
+        _run(q.device, lib.cc1d_gdr_varlen, _with_workspace(_gdr_args(*part, *rest), space))
 
 
 def _rms_norm_gated_impl(x, z, weight, eps, out):

@@ -23,23 +23,24 @@ from .functional import _DTYPES, MAX_STEPS, PAD_SLOT_ID, _flags, _int32, _unsupp
 
 def _shapes(q, k, v, g, beta, lead, A_log, dt_bias):
     """Reject shapes inconsistent with a gated delta rule over lead leading axes."""
-    if not q.dim() == k.dim() == v.dim() == lead + 2:
+    qs, vs = q.shape, v.shape
+    if not len(qs) == k.dim() == len(vs) == lead + 2:
         raise ValueError(f"q, k, v must have {lead + 2} axes, got {q.dim()}, {k.dim()}, {v.dim()}")
-    if q.shape != k.shape or q.shape[:lead] != v.shape[:lead]:
+    if qs != k.shape or qs[:lead] != vs[:lead]:
         raise ValueError(
             f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not go together"
         )
-    hk, hv = q.shape[-2], v.shape[-2]
+    hk, hv = qs[-2], vs[-2]
     if hk < 1 or hv < 1 or hv % hk:
         raise ValueError(f"{hv} value heads are not a multiple of {hk} query/key heads")
-    if q.shape[-1] < 1 or v.shape[-1] < 1:
+    if qs[-1] < 1 or vs[-1] < 1:
         raise ValueError("head dims must be at least 1")
-    want = (*v.shape[:lead], hv)
-    if tuple(g.shape) != want or tuple(beta.shape) != want:
-        raise ValueError(f"g {tuple(g.shape)} and beta {tuple(beta.shape)} must have shape {want}")
+    want = vs[:-1]
+    if g.shape != want or beta.shape != want:
+        raise ValueError(f"g {tuple(g.shape)} and beta {tuple(beta.shape)} must have shape {tuple(want)}")
     if (A_log is None) != (dt_bias is None):
         raise ValueError("A_log and dt_bias come together")
-    if A_log is not None and (tuple(A_log.shape) != (hv,) or tuple(dt_bias.shape) != (hv,)):
+    if A_log is not None and (A_log.shape != (hv,) or dt_bias.shape != (hv,)):
         raise ValueError(f"A_log and dt_bias must have shape ({hv},)")
 
 
@@ -51,12 +52,16 @@ def _state_shape(states, v, dk, what="states"):
 
 def gated_delta_rule_reason(q, k, v, g, beta, states=None, A_log=None, dt_bias=None):
     """Why the kernels cannot serve these tensors, or None."""
-    tensors = [t for t in (q, k, v, g, beta, states, A_log, dt_bias) if t is not None]
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        return "gradients are required and the kernels have no backward pass"
+    grad, device = torch.is_grad_enabled(), q.device
+    apart = False
+    for t in (q, k, v, g, beta, states, A_log, dt_bias):
+        if t is not None:
+            if grad and t.requires_grad:
+                return "gradients are required and the kernels have no backward pass"
+            apart = apart or t.device != device
     if not q.is_cuda:
         return "input is not a CUDA tensor"
-    if any(t.device != q.device for t in tensors):
+    if apart:
         return "tensors are on different devices"
     if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
         return f"dtypes {q.dtype}, {k.dtype}, {v.dtype} are not one of bf16, fp16 or fp32"

@@ -480,7 +480,8 @@ cudaError_t go(const cc1d_gdr_args& a, bool out32, cudaStream_t stream) {
         return cudaErrorInvalidValue;
     err = launch_gdr_prep(a, q, k, stream);
     if (err != cudaSuccess) return err;
-    err = cudaFuncSetAttribute(gdr_chunk_kernel<T, ST, VS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static SmemLimit limit;
+    err = limit.raise(gdr_chunk_kernel<T, ST, VS>, smem);
     if (err != cudaSuccess) return err;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -2,6 +2,8 @@
 // operand images in shared memory, tensor maps.
 #pragma once
 
+#include <atomic>
+
 #include "gdr.cuh"
 #include "kernels.h"
 #include "tc05.cuh"
@@ -77,6 +79,22 @@ __device__ __forceinline__ void load_kq(uint32_t dst, const CUtensorMap* mapk, c
             tma_load(at + 8192, mapq, half * 64, Parts<kLo>::q(hk) + 2 * part, t, bar);
         }
 }
+
+// Dynamic shared memory above 48 KB, asked for once per kernel and device.
+struct SmemLimit {
+    std::atomic<uint64_t> done{0};  // a bit per device
+    template <typename K>
+    cudaError_t raise(K kernel, int bytes) {
+        int dev = 0;
+        cudaError_t err = cudaGetDevice(&dev);
+        if (err != cudaSuccess) return err;
+        const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+        if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+        err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (err == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+        return err;
+    }
+};
 
 // One box (cols x 64 tokens of a head) of the tensor map of a (tokens, heads, dim) view of 16-bit values.
 bool make_map(CUtensorMap* map, const void* p, int64_t tokens, int heads, int dim, int64_t st,

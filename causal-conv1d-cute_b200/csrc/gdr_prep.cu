@@ -548,8 +548,8 @@ cudaError_t launch_gdr_prep(const cc1d_gdr_args& a, const CUtensorMap& q, const 
     auto go = [&](auto lo) {
         constexpr bool kLo = decltype(lo)::value;
         constexpr int smem = (int)sizeof(Smem<kLo>) + 1024;
-        const cudaError_t err = cudaFuncSetAttribute(
-            gdr_prep_kernel<kLo>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        static SmemLimit limit;
+        const cudaError_t err = limit.raise(gdr_prep_kernel<kLo>, smem);
         if (err != cudaSuccess) return err;
         gdr_prep_kernel<kLo><<<(unsigned)grid, 128, smem, stream>>>(a, q, k);
         return cudaGetLastError();

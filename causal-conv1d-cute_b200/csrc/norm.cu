@@ -2,23 +2,38 @@
 //
 // Bound: HBM (x and z read, out written once; about 10 flops and two special-function results per
 // element). A group of LANES lanes owns a row: VPL 16-byte vectors of x and of z per lane, all
-// loaded before the row's sum of squares is reduced by shuffles, so the row is read once. R rows
-// per group keep enough bytes in flight.
+// loaded before the row's sum of squares is reduced by shuffles, so the row is read once. Two rows
+// per group and six CTAs per SM keep enough bytes in flight: 40807 x 48 rows of 128 in bf16 227 us, 6.6
+// TB/s, which is the copy rate (four rows and two CTAs 255 us, one row and eight 245 us).
 #include "common.cuh"
 #include "kernels.h"
 
 namespace cc1d {
 namespace {
 
-// z sigmoid(z) in fp32. The fast exponential and division err by a few ulp of fp32, far below the
-// rounding of a 16-bit output; fp32 outputs take the library's expf and a true division.
+// Two lanes of x inv w z sigmoid(z), the factors that do not depend on the row in w. For 16-bit types
+// the exponential, the reciprocal (a few ulp of fp32 each) and packed arithmetic: with scalar
+// arithmetic and a division the kernel was bound by issue (0.84 a cycle). fp32 takes the library's
+// expf and a true division.
 template <typename T>
-__device__ __forceinline__ float gate(float z) {
+__device__ __forceinline__ float2 gated(float2 x, float2 z, float2 w, float inv, bool gate) {
+    const float2 y = __fmul2_rn(__fmul2_rn(x, make_float2(inv, inv)), w);
+    if (!gate) return y;
+    float2 s;
     if constexpr (sizeof(T) == 4) {
-        return z / (1.f + expf(-z));
+        s = make_float2(z.x / (1.f + expf(-z.x)), z.y / (1.f + expf(-z.y)));
     } else {
-        return __fdividef(z, 1.f + __expf(-z));
+        constexpr float kNegLog2e = -1.4426950408889634f;
+        const float2 e = __fmul2_rn(z, make_float2(kNegLog2e, kNegLog2e));
+        float2 t;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t.x) : "f"(e.x));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t.y) : "f"(e.y));
+        t = __fadd2_rn(t, make_float2(1.f, 1.f));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.x) : "f"(t.x));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.y) : "f"(t.y));
+        s = __fmul2_rn(s, z);
     }
+    return __fmul2_rn(y, s);
 }
 
 // n / d for n below 2^31 by one multiplication (d >= 1), d fixed for a launch.
@@ -34,7 +49,7 @@ struct Divider {
 };
 
 template <typename T, int LANES, int VPL, int R>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, VPL == 1 ? 6 : 1)
 norm_kernel(const __grid_constant__ cc1d_norm_args a, int rows, Divider by_n1) {
     constexpr int V = Vec<T>::V;
     constexpr int GROUPS = 256 / LANES;
@@ -59,27 +74,29 @@ norm_kernel(const __grid_constant__ cc1d_norm_args a, int rows, Divider by_n1) {
             }
         }
     }
-    float w[VPL][V];
+    float2 w[VPL][V / 2];
 #pragma unroll
     for (int m = 0; m < VPL; ++m)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const int e = (m * LANES + lane) * V + i;
-            w[m][i] = 0.f;
+            float& to = i % 2 ? w[m][i / 2].y : w[m][i / 2].x;
+            to = 0.f;
             if (e < a.dim)
-                w[m][i] = a.wdtype == CC1D_F32 ? static_cast<const float*>(a.weight)[e]
+                to = a.wdtype == CC1D_F32 ? static_cast<const float*>(a.weight)[e]
                                                : to_f32(static_cast<const T*>(a.weight)[e]);
         }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const int row = first + r * GROUPS;
-        float f[VPL][V], sum = 0.f;
+        float2 f[VPL][V / 2], sums = make_float2(0.f, 0.f);
 #pragma unroll
         for (int m = 0; m < VPL; ++m) {
-            unpack16<T>(x[r][m], f[m]);
+            unpack16<T>(x[r][m], &f[m][0].x);
 #pragma unroll
-            for (int i = 0; i < V; ++i) sum = fmaf(f[m][i], f[m][i], sum);
+            for (int i = 0; i < V / 2; ++i) sums = __ffma2_rn(f[m][i], f[m][i], sums);
         }
+        float sum = sums.x + sums.y;
 #pragma unroll
         for (int o = LANES / 2; o > 0; o /= 2) sum += __shfl_xor_sync(~0u, sum, o);
         const float inv = rsqrtf(sum / (float)a.dim + a.eps);
@@ -89,12 +106,11 @@ norm_kernel(const __grid_constant__ cc1d_norm_args a, int rows, Divider by_n1) {
         for (int m = 0; m < VPL; ++m) {
             const int e = (m * LANES + lane) * V;
             if (e >= a.dim) continue;
-            float g[V];
-            unpack16<T>(z[r][m], g);
+            float2 g[V / 2];
+            unpack16<T>(z[r][m], &g[0].x);
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                f[m][i] = f[m][i] * inv * w[m][i] * (zp != nullptr ? gate<T>(g[i]) : 1.f);
-            st16_stream(op + i0 * a.o_s0 + i1 * a.o_s1 + e, pack16<T>(f[m]));
+            for (int i = 0; i < V / 2; ++i) f[m][i] = gated<T>(f[m][i], g[i], w[m][i], inv, zp != nullptr);
+            st16_stream(op + i0 * a.o_s0 + i1 * a.o_s1 + e, pack16<T>(&f[m][0].x));
         }
     }
 }
@@ -121,8 +137,8 @@ norm_generic_kernel(const __grid_constant__ cc1d_norm_args a, int64_t rows) {
     for (int64_t e = lane; e < a.dim; e += 32) {
         const float w = a.wdtype == CC1D_F32 ? static_cast<const float*>(a.weight)[e]
                                              : to_f32(static_cast<const T*>(a.weight)[e]);
-        const float g = zp != nullptr ? gate<T>(to_f32(zp[e])) : 1.f;
-        op[e] = from_f32<T>(to_f32(xp[e]) * inv * w * g);
+        const float2 x = make_float2(to_f32(xp[e]), 0.f), z = make_float2(zp != nullptr ? to_f32(zp[e]) : 0.f, 0.f);
+        op[e] = from_f32<T>(gated<T>(x, z, make_float2(w, 0.f), inv, zp != nullptr).x);
     }
 }
 
@@ -144,13 +160,13 @@ cudaError_t launch(const cc1d_norm_args& a, cudaStream_t stream) {
     if (!vec || a.dim > 128 * V || rows >= (1 << 30)) {
         norm_generic_kernel<T><<<(unsigned)ceil_div(rows, 8), 256, 0, stream>>>(a, rows);
     } else if (a.dim <= 8 * V) {
-        go<T, 8, 1, 4>(a, rows, stream);
+        go<T, 8, 1, 2>(a, rows, stream);
     } else if (a.dim <= 16 * V) {
-        go<T, 16, 1, 4>(a, rows, stream);
+        go<T, 16, 1, 2>(a, rows, stream);
     } else if (a.dim <= 32 * V) {
-        go<T, 32, 1, 4>(a, rows, stream);
+        go<T, 32, 1, 2>(a, rows, stream);
     } else if (a.dim <= 64 * V) {
-        go<T, 32, 2, 2>(a, rows, stream);
+        go<T, 32, 2, 1>(a, rows, stream);
     } else {
         go<T, 32, 4, 1>(a, rows, stream);
     }

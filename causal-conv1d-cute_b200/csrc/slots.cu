@@ -130,7 +130,7 @@ slots_move_kernel(const __grid_constant__ SlotTable t, const int32_t* src, const
 __global__ void __launch_bounds__(1024)
 slots_plan_kernel(const uint8_t* __restrict__ live, int nslots, int32_t* __restrict__ remap,
                   int32_t* __restrict__ count, int32_t* __restrict__ plan) {
-    __shared__ int warp_sum[32], total;
+    __shared__ int warp_sum[32];
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
     int m = 0;
     for (int i = tid; i < nslots; i += 1024) m += live[i] != 0;
@@ -138,40 +138,37 @@ slots_plan_kernel(const uint8_t* __restrict__ live, int nslots, int32_t* __restr
     for (int o = 16; o > 0; o /= 2) m += __shfl_xor_sync(~0u, m, o);
     if (lane == 0) warp_sum[warp] = m;
     __syncthreads();
-    if (tid == 0) {
-        int s = 0;
-        for (int w = 0; w < 32; ++w) s += warp_sum[w];
-        total = s;
-        *count = s;
-    }
-    __syncthreads();
-    m = total;
+    m = warp_sum[lane];
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) m += __shfl_xor_sync(~0u, m, o);
+    if (tid == 0) *count = m;
     int32_t* src = plan + 1;
     int32_t* dst = plan + 1 + nslots;
-    // Pairs are numbered by rank: holes below m and movers from m on, each in ascending order.
+    // Pairs are numbered by rank: holes below m and movers from m on, each in ascending order. Both
+    // counts travel in one word (at most 1024 of either in a step of 1024 slots).
     int base[2] = {0, 0};
     for (int at = 0; at < nslots; at += 1024) {
         const int i = at + tid;
         const bool on = i < nslots && live[i] != 0;
-        const bool is[2] = {i < nslots && !on && i < m, on && i >= m};
-        int rank[2];
+        const bool hole = i < nslots && !on && i < m, mover = on && i >= m;
+        const unsigned holes = __ballot_sync(~0u, hole), movers = __ballot_sync(~0u, mover);
+        __syncthreads();
+        if (lane == 0) warp_sum[warp] = __popc(holes) | __popc(movers) << 16;
+        __syncthreads();
+        int sum = warp_sum[lane];  // to the running sum over the warps
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const unsigned votes = __ballot_sync(~0u, is[k]);
-            __syncthreads();
-            if (lane == 0) warp_sum[warp] = __popc(votes);
-            __syncthreads();
-            int before = 0, all = 0;
-            for (int w = 0; w < 32; ++w) {
-                if (w < warp) before += warp_sum[w];
-                all += warp_sum[w];
-            }
-            rank[k] = base[k] + before + __popc(votes & ((1u << lane) - 1u));
-            base[k] += all;
+        for (int o = 1; o < 32; o *= 2) {
+            const int below = __shfl_up_sync(~0u, sum, o);
+            if (lane >= o) sum += below;
         }
-        if (is[0]) dst[rank[0]] = i;
-        if (is[1]) src[rank[1]] = i;
-        if (i < nslots && !is[1]) remap[i] = on ? i : -1;
+        const int all = __shfl_sync(~0u, sum, 31);
+        const int before = __shfl_sync(~0u, sum, warp > 0 ? warp - 1 : 0) & (warp > 0 ? ~0 : 0);
+        const unsigned under = (1u << lane) - 1u;
+        if (hole) dst[base[0] + (before & 0xffff) + __popc(holes & under)] = i;
+        if (mover) src[base[1] + (before >> 16) + __popc(movers & under)] = i;
+        if (i < nslots && !mover) remap[i] = on ? i : -1;
+        base[0] += all & 0xffff;
+        base[1] += all >> 16;
     }
     if (tid == 0) plan[0] = base[1];
     __syncthreads();

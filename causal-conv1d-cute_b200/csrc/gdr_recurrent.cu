@@ -248,8 +248,9 @@ gdr_recurrent_kernel(const __grid_constant__ cc1d_gdr_args a, bool varlen, bool 
 // Decode of whole heads, dk = 128 and tiles of 128 columns: a CTA of 8 warps has a (128, 128) state
 // tile in registers, 16 rows and 4 columns per lane, so that a warp's access is one whole row and
 // the norms, gates and the reduction are done once for the tile. Two CTAs of 64 KB per SM are in
-// flight. Measured at 256 rows x 48 heads, fp32: 295 us, 5.5 TB/s of 6.4 (16 warps of 8 rows 300 us,
-// the same with three CTAs an SM, which spills, 538 us).
+// flight, and the stores are evict-first: a step's states are next read a whole model later.
+// Measured at 256 rows x 48 heads, fp32: 274 us, 5.9 TB/s of 6.4 (plain stores 293 us; 16 warps of 8
+// rows 300 us, the same with three CTAs an SM, which spills, 538 us).
 template <typename T, typename ST>
 __global__ void __launch_bounds__(256, 2)
 gdr_decode_kernel(const __grid_constant__ cc1d_gdr_args a, int tiles) {
@@ -382,12 +383,12 @@ gdr_decode_kernel(const __grid_constant__ cc1d_gdr_args a, int tiles) {
         if (islot >= 0) {
             ST* ip = static_cast<ST*>(a.inter) + islot * a.i_slot + t * a.i_st + h * a.i_sh + first * a.i_sk + col;
 #pragma unroll
-            for (int r = 0; r < ROWS; ++r) st_raw<NB>(ip + r * a.i_sk, pack_raw<ST, NB>(&S[r][0].x));
+            for (int r = 0; r < ROWS; ++r) st_stream_raw<NB>(ip + r * a.i_sk, pack_raw<ST, NB>(&S[r][0].x));
         }
     }
     if (a.update_states) {
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) st_raw<NB>(st + r * a.s_sk, pack_raw<ST, NB>(&S[r][0].x));
+        for (int r = 0; r < ROWS; ++r) st_stream_raw<NB>(st + r * a.s_sk, pack_raw<ST, NB>(&S[r][0].x));
     }
 }
 
@@ -410,7 +411,7 @@ cudaError_t launch(const cc1d_gdr_args& a, bool varlen, cudaStream_t stream) {
     const bool iovec = a.v_sd == 1 && a.o_sd == 1 &&
                        vec_ok(a.v, ib, CPL, {varlen ? 0 : a.v_sb, a.v_st, a.v_sh}) &&
                        vec_ok(a.out, ib, CPL, {varlen ? 0 : a.o_sb, a.o_st, a.o_sh});
-    // Whole heads where the shape allows it (one step, fp32: 12288 heads 295 us against 371 us in
+    // Whole heads where the shape allows it (one step, fp32: 12288 heads 274 us against 371 us in
     // tiles of 32 columns, 6 heads 5.3 against 5.0). Recorded fp32 states are the exception with few
     // heads: their stores are bound by the SM, and four CTAs a head spread them over more SMs (4
     // steps, 6 heads 8.7 against 11.8 us, 384 heads 36 against 41 us, 768 heads 67 against 66 us).

@@ -30,52 +30,36 @@
 // K, Q, T and G come by TMA and bulk copies a chunk or two ahead.
 //
 // Bound. The latency of the chain: 2950 cycles a chunk at VS = 32, of which the products take half
-// and the rest is TMEM loads, splitting, barriers. At VS = 128 (6800 cycles) also the integer pipe
-// (four half-rate instructions per split pair) and shared memory, of whose 128 bytes a cycle the
-// products take 2400 cycles' worth, the operands written for them 1000 and the loads 650. Tried and
-// slower at 128 columns: two independent chains of 64 in one CTA (7700 cycles), and two tiles in
-// turn, with warps of their own for products and loads (7400; 3500 at 32 columns): a product that
-// runs beside operand stores takes up to three times as long, and hand-overs by mbarrier cost more
-// than the barrier of one CTA.
+// and the rest is TMEM loads, splitting, barriers. Tiles of 128 columns, for many heads, have a
+// kernel of their own (gdr_wide.cu); in the form used here they took 6800 cycles a chunk, two
+// independent chains of 64 in one CTA 7700, and two tiles in turn, with warps of their own for
+// products and loads, 7400 (3500 at 32 columns).
 //
 // Stacking K over Q and T over G makes every product M = 128, the full tensor core rate; the two
 // parts of an operand lie side by side as one operand of 2 VS columns (measured: a K step of 16
 // costs 46 cycles up to 64 columns, 66 with 128 and 137 with 256, so one wide step beats two narrow
-// ones up to VS = 64).
+// ones).
 #include "gdr_chunk.cuh"
 
 namespace cc1d {
 namespace {
 
-constexpr int kOrderMax = 256;  // batches up to this many sequences start with the longest
-
 template <int VS, bool kLo>
 struct Layout {
-    static constexpr int kRow = VS >= 64 ? 128 : 2 * VS;  // bytes of a row of an operand's column atom
-    static constexpr int kAtoms = VS >= 64 ? VS / 64 : 1;
-    static constexpr int kS = 128 * kRow * kAtoms;        // one part (hi or lo) of S
-    static constexpr int kR = C * kRow * kAtoms;          // one part of R or u, or V
+    static constexpr int kRow = 2 * VS;        // bytes of a row of columns
+    static constexpr int kS = 128 * kRow;      // one part (hi or lo) of S
+    static constexpr int kR = C * kRow;        // one part of R or u, or V
     static constexpr int kKQ = Parts<kLo>::kBytes;
-    static constexpr int kStages = VS <= 32 ? (kLo ? 2 : 3) : kLo ? 1 : 2;
-    static constexpr int KQ = 0;                          // stages x K and Q
-    static constexpr int TG = KQ + kStages * kKQ;         // stages x [hi, lo][128 rows][128 B]
-    static constexpr int SB = TG + kStages * 32768;       // S hi, S lo; R in S hi, u in S lo
-    static constexpr int V = SB + 2 * kS;                 // [atoms][64 rows]
-    static constexpr int VEC = V + kR;                    // stages x row factors
+    static constexpr int kStages = VS == 32 && !kLo ? 3 : 2;
+    static constexpr int KQ = 0;                       // stages x K and Q
+    static constexpr int TG = KQ + kStages * kKQ;      // stages x [hi, lo][128 rows][128 B]
+    static constexpr int SB = TG + kStages * 32768;    // S hi, S lo; R in S hi, u in S lo
+    static constexpr int V = SB + 2 * kS;              // [64 rows]
+    static constexpr int VEC = V + kR;                 // stages x row factors
     static constexpr int END = VEC + kStages * kVectorBytes;
-    // The products with the two parts of an operand: side by side, and added on the way out of
-    // TMEM, while that is the faster way (see above); on top of each other with 128 columns, where
-    // a step costs the same per column either way.
-    static constexpr bool kWide = VS < 128;
-    static constexpr int kTmem = VS == 32 ? 128 : 256;  // of 3 VS columns, or 2
-    static constexpr int kThreads = VS == 128 ? 512 : 256;
+    static constexpr int kTmem = VS == 32 ? 128 : 256;  // of 3 VS columns
 };
-
-// The row factors of a ChunkImage, as they follow its T and G.
-struct Vectors {
-    float in[2 * C], out[C], decay, pad[3];
-};
-static_assert(sizeof(Vectors) == kVectorBytes, "");
+constexpr int kThreads = 256;
 
 struct Shared {
     uint64_t full[3], v_full, mma;
@@ -84,38 +68,21 @@ struct Shared {
     int row;  // sequence of this CTA
 };
 
-// Row r, unit u of a row of columns whose 64-column atoms lie `rows` rows apart.
-template <int VS>
-__device__ __forceinline__ uint32_t swz_cols(int rows, int r, int u) {
-    if constexpr (VS > 64) {
-        return (u >> 3) * rows * 128 + swz<128>(r, u & 7);
-    } else {
-        return swz<Layout<VS, false>::kRow>(r, u);
-    }
-}
-
-// One thread: D (+)= A B over kSteps K steps, B in two parts: side by side as one operand of 2 VS
-// columns, or, with 128 columns, one after the other (`lo` units apart) onto the same columns.
+// One thread: D (+)= A B over kSteps K steps, the two parts of B side by side as one operand of 2 VS
+// columns, whose products are added on the way out of TMEM.
 template <int VS, int kSteps, int kA, bool kTransposedA>
-__device__ __forceinline__ void two_part_product(uint32_t d, uint64_t a, uint64_t b, uint32_t lo,
-                                                 bool accumulate) {
-    constexpr int kB = Layout<VS, false>::kRow;
-    if constexpr (Layout<VS, false>::kWide) {
-        mma_steps<kSteps, kA, kB>(d, a, b, mma_desc(2 * VS, kTransposedA, true), accumulate);
-    } else {
-        mma_steps<kSteps, kA, kB>(d, a, b, mma_desc(VS, kTransposedA, true), accumulate);
-        mma_steps<kSteps, kA, kB>(d, a, b + lo, mma_desc(VS, kTransposedA, true), true);
-    }
+__device__ __forceinline__ void two_part_product(uint32_t d, uint64_t a, uint64_t b, bool accumulate) {
+    mma_steps<kSteps, kA, 2 * VS>(d, a, b, mma_desc(2 * VS, kTransposedA, true), accumulate);
 }
 
 template <typename T, typename ST, int VS>
-__global__ void __launch_bounds__(Layout<VS, false>::kThreads, 1)
+__global__ void __launch_bounds__(kThreads, 1)
 gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__ CUtensorMap mapq,
                  const __grid_constant__ CUtensorMap mapk, const __grid_constant__ CUtensorMap mapv,
                  int tiles, bool out32) {
     constexpr bool kLo = std::is_same<T, f16>::value;  // fp16 keys and queries come in two bf16 parts
     using Lay = Layout<VS, kLo>;
-    constexpr uint64_t kSwz = VS >= 64 ? kSwizzle128 : kSwizzle64;
+    constexpr uint64_t kSwz = VS == 64 ? kSwizzle128 : kSwizzle64;
     constexpr uint32_t kGroup = 8 * Lay::kRow;  // bytes of eight rows of V columns
     constexpr int kStages = Lay::kStages;
     extern __shared__ __align__(1024) unsigned char raw[];
@@ -130,21 +97,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
     int64_t row = blockIdx.x / tiles / a.heads_v;
     const int hk = h / (a.heads_v / a.heads_k);
 
-    // Longest sequences first, so that the last CTAs to start are short. Ties go by index.
-    if (a.rows > 1 && a.rows <= kOrderMax) {
-        const int n = (int)a.rows;
-        int* len = reinterpret_cast<int*>(gen);
-        for (int j = tid; j < n; j += Lay::kThreads)
-            len[j] = a.query_start_loc[j + 1] - a.query_start_loc[j];
-        __syncthreads();
-        for (int j = tid; j < n; j += Lay::kThreads) {
-            int rank = 0;
-            for (int i = 0; i < n; ++i) rank += len[i] > len[j] || (len[i] == len[j] && i < j);
-            if (rank == row) sh.row = j;
-        }
-        __syncthreads();
-        row = sh.row;
-    }
+    row = longest_first(a, row, reinterpret_cast<int*>(gen), &sh.row);
     int64_t tok0, slot;
     int ntok;
     if (!gdr_row(a, true, row, tok0, ntok, slot, h == 0 && vt == 0 && tid == 0)) return;
@@ -184,9 +137,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
     auto load_v = [&](int c) {
         const uint32_t full = smem_addr(&sh.v_full);
         mbar_expect(full, C * VS * 2);
-#pragma unroll
-        for (int at = 0; at < Lay::kAtoms; ++at)
-            tma_load(base + Lay::V + at * C * Lay::kRow, &mapv, vt * VS + at * 64, h, (int)tok0 + c * C, full);
+        tma_load(base + Lay::V, &mapv, vt * VS, h, (int)tok0 + c * C, full);
     };
     grid_dependency_wait();  // for the prep kernel's images
     if (tid == 0) {
@@ -195,11 +146,11 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
     }
 
     // A thread has row p and columns first .. first + W of the tile.
-    constexpr int W = VS * 128 / Lay::kThreads;
+    constexpr int W = VS * 128 / kThreads;
     const int first = warp / 4 * W;
     const bool lead = tid == 0;
-    const uint32_t D = tmem;  // the product, or [product with hi parts | with lo parts]
-    const uint32_t Dh = D + lanes + first, Dl = Dh + VS, TS = Lay::kWide ? Dl + VS : Dl;  // TS: the state
+    const uint32_t D = tmem;  // [product with hi parts | with lo parts]
+    const uint32_t Dh = D + lanes + first, Dl = Dh + VS, TS = Dl + VS;  // TS: the state
     const uint32_t mma = smem_addr(&sh.mma);
     const uint32_t s_hi = base + Lay::SB, s_lo = s_hi + Lay::kS;
     const uint32_t r_hi = s_hi, r_lo = r_hi + Lay::kR, u_hi = s_lo, u_lo = u_hi + Lay::kR;
@@ -209,7 +160,6 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
     ST* sp = nullptr;
     if (a.states != nullptr)
         sp = static_cast<ST*>(a.states) + slot * a.s_slot + h * a.s_sh + p * a.s_sk + col;
-    auto sum = [](float2 x, float2 y) { return Lay::kWide ? __fadd2_rn(x, y) : x; };
     constexpr int SV = Vec<ST>::V;
     T* op = static_cast<T*>(a.out) + tok0 * a.o_st + h * a.o_sh + col;
 
@@ -220,7 +170,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
 #pragma unroll
         for (int k = 0; k < 8; ++k) s[k] = make_float2(0.f, 0.f);
         tmem_st16(Dh + 16 * g, s);
-        if (Lay::kWide) tmem_st16(Dl + 16 * g, s);
+        tmem_st16(Dl + 16 * g, s);
         if (initial) {
 #pragma unroll
             for (int k = 0; k < 16; k += SV) unpack16<ST>(ld16(sp + 16 * g + k), &s[0].x + k);
@@ -240,18 +190,18 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
 #pragma unroll
             for (int g = 0; g < W / 16; ++g) {
                 tmem_ld16_async(Dh + 16 * g, d[g]);
-                if (Lay::kWide) tmem_ld16_async(Dl + 16 * g, e[g]);
+                tmem_ld16_async(Dl + 16 * g, e[g]);
                 tmem_ld16_async(TS + 16 * g, s[g]);
             }
             tmem_wait_ld();
 #pragma unroll
             for (int g = 0; g < W / 16; ++g) {
                 tmem_ready(d[g]);
-                if (Lay::kWide) tmem_ready(e[g]);
+                tmem_ready(e[g]);
                 tmem_ready(s[g]);
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
-                    s[g][k] = __ffma2_rn(make_float2(decay, decay), s[g][k], sum(d[g][k], e[g][k]));
+                    s[g][k] = __ffma2_rn(make_float2(decay, decay), s[g][k], __fadd2_rn(d[g][k], e[g][k]));
                 if (c == chunks) {
                     if (sp != nullptr) {
 #pragma unroll
@@ -261,7 +211,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
                     tmem_st16(TS + 16 * g, s[g]);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const uint32_t at = swz_cols<VS>(128, p, first / 8 + 2 * g + u);
+                        const uint32_t at = swz<Lay::kRow>(p, first / 8 + 2 * g + u);
                         store_split8(s_hi + at, s_lo + at, s[g] + 4 * u);
                     }
                 }
@@ -274,7 +224,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
         if (left < C) {
             // The copies of K went on into the next sequence: zeros there, whatever it holds
             // (rows of Q there make outputs that are not stored).
-            for (int e = tid; e < (C - left) * 16; e += Lay::kThreads)
+            for (int e = tid; e < (C - left) * 16; e += kThreads)
 #pragma unroll
                 for (int part = 0; part <= (kLo ? 1 : 0); ++part)
                     sts16(kq + part * 32768 + (e % 16 >> 3) * 16384 + swz<128>(left + e / 16, e % 8), 0, 0, 0, 0);
@@ -286,8 +236,8 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
             tc_fence_after();
             // [K;Q] S
             const uint64_t k = operand(kq, 16, 1024, kSwizzle128), s = operand(s_hi, 128 * Lay::kRow, kGroup, kSwz);
-            two_part_product<VS, 4, 2, false>(D, k, s, Lay::kS / 16, false);
-            two_part_product<VS, 4, 2, false>(D, k + 1024, s + kGroup / 2, Lay::kS / 16, true);
+            two_part_product<VS, 4, 2, false>(D, k, s, false);
+            two_part_product<VS, 4, 2, false>(D, k + 1024, s + kGroup / 2, true);
             if constexpr (kLo) {
                 mma_steps<4, 2, kGroup / 8>(D, k + 2048, s, mma_desc(VS, false, true), true);
                 mma_steps<4, 2, kGroup / 8>(D, k + 3072, s + kGroup / 2, mma_desc(VS, false, true), true);
@@ -296,7 +246,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
         }
         // While it runs, a thread with little else to do (six copies take 560 cycles to issue) refills
         // the stage of the chunk before.
-        if (kStages > 1 && tid == 64 && c > 0 && c - 1 + kStages < chunks) load(c - 1 + kStages, st > 0 ? st - 1 : kStages - 1);
+        if (tid == 64 && c > 0 && c - 1 + kStages < chunks) load(c - 1 + kStages, st > 0 ? st - 1 : kStages - 1);
         const float in = vec[st].in[p], out = vec[st].out[p % C];
         decay = vec[st].decay;
         float2 q[W / 2];  // rows of Q: their outputs
@@ -309,27 +259,27 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
 #pragma unroll
             for (int g = 0; g < W / 16; ++g) {
                 tmem_ld16_async(Dh + 16 * g, d[g]);
-                if (Lay::kWide) tmem_ld16_async(Dl + 16 * g, e[g]);
+                tmem_ld16_async(Dl + 16 * g, e[g]);
             }
             if (p < C) {
                 // R = V - r e^b (K S), zero behind the sequence's end, whatever V holds there
                 const bool live = p < left;
                 uint4 v[W / 8];
 #pragma unroll
-                for (int u = 0; u < W / 8; ++u) v[u] = lds16(vb + swz_cols<VS>(C, p, first / 8 + u));
+                for (int u = 0; u < W / 8; ++u) v[u] = lds16(vb + swz<Lay::kRow>(p, first / 8 + u));
                 tmem_wait_ld();
 #pragma unroll
                 for (int g = 0; g < W / 16; ++g) {
                     tmem_ready(d[g]);
-                    if (Lay::kWide) tmem_ready(e[g]);
+                    tmem_ready(e[g]);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         const uint32_t vv[4] = {v[2 * g + u].x, v[2 * g + u].y, v[2 * g + u].z, v[2 * g + u].w};
                         float2 f[4];
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            f[k] = add_pair<T>(live ? vv[k] : 0u, mul2(sum(d[g][4 * u + k], e[g][4 * u + k]), -in));
-                        const uint32_t at = swz_cols<VS>(C, p, first / 8 + 2 * g + u);
+                            f[k] = add_pair<T>(live ? vv[k] : 0u, mul2(__fadd2_rn(d[g][4 * u + k], e[g][4 * u + k]), -in));
+                        const uint32_t at = swz<Lay::kRow>(p, first / 8 + 2 * g + u);
                         store_split8(r_hi + at, r_lo + at, f);
                     }
                 }
@@ -339,9 +289,9 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
 #pragma unroll
                 for (int g = 0; g < W / 16; ++g) {
                     tmem_ready(d[g]);
-                    if (Lay::kWide) tmem_ready(e[g]);
+                    tmem_ready(e[g]);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) q[8 * g + k] = mul2(sum(d[g][k], e[g][k]), in);
+                    for (int k = 0; k < 8; ++k) q[8 * g + k] = mul2(__fadd2_rn(d[g][k], e[g][k]), in);
                 }
             }
         }
@@ -351,7 +301,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
             tc_fence_after();
             // [T;G] R: hi [hi | lo], then lo hi
             const uint64_t r = operand(r_hi, C * Lay::kRow, kGroup, kSwz);
-            two_part_product<VS, 4, 2, false>(D, operand(tg, 16, 1024, kSwizzle128), r, Lay::kR / 16, false);
+            two_part_product<VS, 4, 2, false>(D, operand(tg, 16, 1024, kSwizzle128), r, false);
             mma_steps<4, 2, kGroup / 8>(D, operand(tg + 16384, 16, 1024, kSwizzle128), r, mma_desc(VS, false, true), true);
             mma_commit(mma);
             if (c + 1 < chunks) load_v(c + 1);
@@ -364,25 +314,25 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
 #pragma unroll
             for (int g = 0; g < W / 16; ++g) {
                 tmem_ld16_async(Dh + 16 * g, d[g]);
-                if (Lay::kWide) tmem_ld16_async(Dl + 16 * g, e[g]);
+                tmem_ld16_async(Dl + 16 * g, e[g]);
             }
             tmem_wait_ld();
 #pragma unroll
             for (int g = 0; g < W / 16; ++g) {
                 tmem_ready(d[g]);
-                if (Lay::kWide) tmem_ready(e[g]);
+                tmem_ready(e[g]);
                 if (p < C) {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) d[g][k] = mul2(sum(d[g][k], e[g][k]), out);
+                    for (int k = 0; k < 8; ++k) d[g][k] = mul2(__fadd2_rn(d[g][k], e[g][k]), out);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const uint32_t at = swz_cols<VS>(C, p, first / 8 + 2 * g + u);
+                        const uint32_t at = swz<Lay::kRow>(p, first / 8 + 2 * g + u);
                         store_split8(u_hi + at, u_lo + at, d[g] + 4 * u);
                     }
                 } else {
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
-                        q[8 * g + k] = __fadd2_rn(q[8 * g + k], sum(d[g][k], e[g][k]));
+                        q[8 * g + k] = __fadd2_rn(q[8 * g + k], __fadd2_rn(d[g][k], e[g][k]));
                 }
             }
             if (p < C) fence_async_smem();
@@ -393,7 +343,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
             tc_fence_after();
             // K^T u
             const uint64_t k = operand(kq, 16384, 1024, kSwizzle128), u = operand(u_hi, C * Lay::kRow, kGroup, kSwz);
-            two_part_product<VS, 4, 128, true>(D, k, u, Lay::kR / 16, false);
+            two_part_product<VS, 4, 128, true>(D, k, u, false);
             if constexpr (kLo) mma_steps<4, 128, kGroup / 8>(D, k + 2048, u, mma_desc(VS, true, true), true);
             mma_commit(mma);
         }
@@ -416,15 +366,10 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
             st_phase ^= 1;
         }
         // The next chunk's K, Q, T, G: there by now, and the look costs less here.
-        if (kStages > 1 && c + 1 < chunks) mbar_wait(smem_addr(&sh.full[st]), st_phase, &sh.abort);
+        if (c + 1 < chunks) mbar_wait(smem_addr(&sh.full[st]), st_phase, &sh.abort);
         mbar_wait(mma, phase, &sh.abort);
         phase ^= 1;
         tc_fence_after();
-        if (kStages == 1 && c + 1 < chunks) {
-            // One stage (fp16 keys and queries take twice the room): refilled between chunks.
-            if (lead) load(c + 1, 0);
-            mbar_wait(smem_addr(&sh.full[0]), st_phase, &sh.abort);
-        }
     }
     tc_fence_before();
     __syncthreads();
@@ -456,57 +401,40 @@ int64_t images_bytes(const cc1d_gdr_args& a) {
 }
 
 template <typename T, typename ST, int VS>
-cudaError_t go(const cc1d_gdr_args& a, bool out32, cudaStream_t stream) {
-    constexpr bool kLo = std::is_same<T, f16>::value;  // fp16 keys and queries come in two bf16 parts
-    using Lay = Layout<VS, kLo>;
-    constexpr int smem = Lay::END + 1024;
+cudaError_t go(const cc1d_gdr_args& a, const CUtensorMap& q, const CUtensorMap& k, bool out32,
+               cudaStream_t stream) {
+    constexpr int smem = Layout<VS, std::is_same<T, f16>::value>::END + 1024;
     const int tiles = a.dv / VS;
     const int64_t grid = a.rows * a.heads_v * tiles;
     if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
-    CUtensorMap q, k, v;
-    cudaError_t err = cudaSuccess;
-    if constexpr (kLo) {
-        void* parts = static_cast<char*>(a.workspace) + images_bytes(a);
-        err = launch_gdr_split(a, parts, stream);
-        if (err != cudaSuccess) return err;
-        if (!make_map(&k, parts, a.tokens, 4 * a.heads_k, a.dk, 4 * a.heads_k * a.dk, a.dk, 64))
-            return cudaErrorInvalidValue;
-        q = k;
-    } else if (!make_map(&q, a.q, a.tokens, a.heads_k, a.dk, a.q_st, a.q_sh, 64) ||
-               !make_map(&k, a.k, a.tokens, a.heads_k, a.dk, a.k_st, a.k_sh, 64)) {
-        return cudaErrorInvalidValue;
-    }
-    if (!make_map(&v, a.v, a.tokens, a.heads_v, a.dv, a.v_st, a.v_sh, VS < 64 ? VS : 64))
-        return cudaErrorInvalidValue;
-    err = launch_gdr_prep(a, q, k, stream);
-    if (err != cudaSuccess) return err;
+    CUtensorMap v;
+    if (!make_map(&v, a.v, a.tokens, a.heads_v, a.dv, a.v_st, a.v_sh, VS)) return cudaErrorInvalidValue;
     static SmemLimit limit;
-    err = limit.raise(gdr_chunk_kernel<T, ST, VS>, smem);
+    const cudaError_t err = limit.raise(gdr_chunk_kernel<T, ST, VS>, smem);
     if (err != cudaSuccess) return err;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(Lay::kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, gdr_chunk_kernel<T, ST, VS>, a, q, k, v, tiles, out32);
+    return launch_dependent(gdr_chunk_kernel<T, ST, VS>, (unsigned)grid, kThreads, smem, stream, a, q, k, v,
+                            tiles, out32);
 }
 
 template <typename T, typename ST>
-cudaError_t pick(const cc1d_gdr_args& a, bool out32, cudaStream_t stream) {
-    // Columns per CTA. A chunk's step takes 1.7, 2.6 and 3.7 us with 32, 64 and 128 columns: wide
-    // tiles do more per SM, narrow ones finish a chain sooner. Many heads take the widest (768 heads,
-    // 16384 tokens: 798, 595, 530 us with 32, 64, 128; 384 heads 745, 562, 530; 192 heads 808, 607,
-    // 890), few that leave SMs free the narrowest (12 heads, 4096 tokens: 126, 160, 250; 24 heads
-    // 139, 173, 265; 48 heads in one sequence 262, 196, 289, in four 105, 130, 203 for 4096).
-    const int64_t heads = a.rows * a.heads_v, narrow = heads * (a.dv / 32);
-    if (a.dv % 128 == 0 && heads * (a.dv / 128) >= 370) return go<T, ST, 128>(a, out32, stream);
-    if (a.dv % 64 == 0 && narrow > (a.rows >= 4 ? 296 : 148)) return go<T, ST, 64>(a, out32, stream);
-    return go<T, ST, 32>(a, out32, stream);
+cudaError_t pick(const cc1d_gdr_args& a, const CUtensorMap& q, const CUtensorMap& k, cudaStream_t stream) {
+    const bool out32 = host_aligned32(a.out) && a.o_st % 16 == 0 && a.o_sh % 16 == 0;
+    // Columns per CTA. A chunk's step takes 1.6, 2.2 and 2.8 us with 32, 64 and 128 columns: wide
+    // tiles do more per SM, narrow ones finish a chain sooner. Many heads take the widest (bf16,
+    // uneven lengths, us with 32, 64, 128: 768 heads, 16384 tokens 800, 599, 458; 336 heads 235,
+    // 178, 160; 288 heads 226, 174, 172; 240 heads 221, 169, 196), few that leave SMs free the
+    // narrowest (12 heads, 4096 tokens 126, 162, 200; 48 heads in four sequences 104, 131, 162, in
+    // one 263, 198, 237). fp16 has no tile of 64, which would load twice the keys for no more than
+    // the narrow one's speed (768 heads 1014, 974, 639; 144 heads 552, 550, 508; 72 heads 184, 302,
+    // 282).
+    constexpr bool kF16 = std::is_same<T, f16>::value;
+    const int64_t heads = a.rows * a.heads_v;
+    if (a.dv % 128 == 0 && heads * (a.dv / 128) >= (kF16 ? 148 : 296)) return launch_gdr_wide(a, q, k, stream);
+    if constexpr (!kF16) {
+        if (a.dv % 64 == 0 && heads * (a.dv / 32) > (a.rows >= 4 ? 296 : 148))
+            return go<T, ST, 64>(a, q, k, out32, stream);
+    }
+    return go<T, ST, 32>(a, q, k, out32, stream);
 }
 
 }  // namespace
@@ -549,10 +477,23 @@ bool gdr_chunk_serves(const cc1d_gdr_args& a) {
 }
 
 cudaError_t launch_gdr_chunk(const cc1d_gdr_args& a, cudaStream_t stream) {
-    const bool out32 = host_aligned32(a.out) && a.o_st % 16 == 0 && a.o_sh % 16 == 0;
+    CUtensorMap q, k;
+    if (a.dtype == CC1D_F16) {
+        void* parts = static_cast<char*>(a.workspace) + images_bytes(a);
+        const cudaError_t err = launch_gdr_split(a, parts, stream);
+        if (err != cudaSuccess) return err;
+        if (!make_map(&k, parts, a.tokens, 4 * a.heads_k, a.dk, 4 * a.heads_k * a.dk, a.dk, 64))
+            return cudaErrorInvalidValue;
+        q = k;
+    } else if (!make_map(&q, a.q, a.tokens, a.heads_k, a.dk, a.q_st, a.q_sh, 64) ||
+               !make_map(&k, a.k, a.tokens, a.heads_k, a.dk, a.k_st, a.k_sh, 64)) {
+        return cudaErrorInvalidValue;
+    }
+    const cudaError_t err = launch_gdr_prep(a, q, k, stream);
+    if (err != cudaSuccess) return err;
     if (a.dtype == CC1D_F16)
-        return a.sdtype == CC1D_F32 ? pick<f16, float>(a, out32, stream) : pick<f16, f16>(a, out32, stream);
-    return a.sdtype == CC1D_F32 ? pick<bf16, float>(a, out32, stream) : pick<bf16, bf16>(a, out32, stream);
+        return a.sdtype == CC1D_F32 ? pick<f16, float>(a, q, k, stream) : pick<f16, f16>(a, q, k, stream);
+    return a.sdtype == CC1D_F32 ? pick<bf16, float>(a, q, k, stream) : pick<bf16, bf16>(a, q, k, stream);
 }
 
 }  // namespace cc1d

@@ -23,6 +23,12 @@ struct ChunkImage {
 };
 constexpr int kVectorBytes = (int)sizeof(ChunkImage) - 32768;  // what follows tg
 
+// The row factors of a ChunkImage, as they follow its T and G.
+struct Vectors {
+    float in[2 * C], out[C], decay, pad[3];
+};
+static_assert(sizeof(Vectors) == kVectorBytes, "");
+
 // Image slots: the chunks of sequence n start at slot floor(first token / 64) + n, which leaves
 // every sequence room for its chunks without a prefix sum over the lengths.
 __device__ __forceinline__ int64_t chunk_base(int64_t first_token, int64_t n) {
@@ -80,6 +86,24 @@ __device__ __forceinline__ void load_kq(uint32_t dst, const CUtensorMap* mapk, c
         }
 }
 
+// The sequence of a CTA that was given index `row`: the row-th longest, so that the last CTAs to
+// start are short. Ties go by index. All threads of the CTA call it; len and *mine are shared.
+constexpr int kOrderMax = 256;  // batches up to this many sequences are ordered
+__device__ __forceinline__ int64_t longest_first(const cc1d_gdr_args& a, int64_t row, int* len, int* mine) {
+    if (a.rows < 2 || a.rows > kOrderMax) return row;
+    const int n = (int)a.rows;
+    for (int j = threadIdx.x; j < n; j += blockDim.x)
+        len[j] = a.query_start_loc[j + 1] - a.query_start_loc[j];
+    __syncthreads();
+    for (int j = threadIdx.x; j < n; j += blockDim.x) {
+        int rank = 0;
+        for (int i = 0; i < n; ++i) rank += len[i] > len[j] || (len[i] == len[j] && i < j);
+        if (rank == row) *mine = j;
+    }
+    __syncthreads();
+    return *mine;
+}
+
 // Dynamic shared memory above 48 KB, asked for once per kernel and device.
 struct SmemLimit {
     std::atomic<uint64_t> done{0};  // a bit per device
@@ -96,9 +120,29 @@ struct SmemLimit {
     }
 };
 
+// A launch whose CTAs may come up while the kernel before drains; they wait for its end themselves.
+template <typename... Params, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Params...), unsigned grid, int threads, int smem,
+                             cudaStream_t stream, const Args&... args) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // One box (cols x 64 tokens of a head) of the tensor map of a (tokens, heads, dim) view of 16-bit values.
 bool make_map(CUtensorMap* map, const void* p, int64_t tokens, int heads, int dim, int64_t st,
               int64_t sh, int cols);
+// gdr_wide.cu: the scan with 128 state columns to a CTA.
+cudaError_t launch_gdr_wide(const cc1d_gdr_args& a, const CUtensorMap& q, const CUtensorMap& k,
+                            cudaStream_t stream);
 // Whether the driver offers tensor maps.
 bool have_maps();
 

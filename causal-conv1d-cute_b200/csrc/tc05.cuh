@@ -189,6 +189,22 @@ __device__ __forceinline__ void mma_steps(uint32_t d, uint64_t a, uint64_t b, ui
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) mma_bf16(d, a + i * kA, b + i * kB, desc, accumulate || i > 0);
 }
+// The same with A in tensor memory: 128 lanes, a row of M each, two K elements to a column.
+__device__ __forceinline__ void mma_bf16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc,
+                                            bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(desc), "r"(accumulate ? 1u : 0u)
+        : "memory");
+}
+template <int kSteps, int kB>
+__device__ __forceinline__ void mma_steps_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc,
+                                             bool accumulate) {
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) mma_bf16_ts(d, a + i * 8, b + i * kB, desc, accumulate || i > 0);
+}
 // Arrive on the mbarrier when all MMAs this thread has issued so far are complete.
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile(

@@ -329,6 +329,43 @@ def test_varlen_sequences_do_not_see_each_other(bad, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,sdtype", [(BF, F32), (F16, F16)])
+@pytest.mark.parametrize("dv,states,raw,pad", [(128, True, False, 3), (256, True, True, None), (128, False, True, None)])
+def test_varlen_wide_tiles(dtype, sdtype, dv, states, raw, pad):
+    """Batches with work for the widest tile: several tiles of a head, made gates, no cache, a pad."""
+    varlen_case([65, 1, 0, 130, 64, 3, 20, 97], hk=20, hv=40, dv=dv, dtype=dtype, sdtype=sdtype, states=states, raw=raw,
+                pad=pad, seed=dv)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_varlen_wide_tiles_do_not_see_each_other(bad, dtype):
+    """The same as above for one sequence among many heads; the outputs of the others bit for bit."""
+    lengths = [70, 33, 129, 64, 1, 90, 15, 66]
+    T, n, hv = sum(lengths), len(lengths), 40
+    q, k, v, g, b, A, dt = (gpu(t) for t in make(T, 20, hv, 128, 128, dtype))
+    start = torch.tensor([0] + list(itertools.accumulate(lengths)), dtype=torch.int32).cuda()
+    st = torch.randn(n, hv, 128, 128, device="cuda")
+    hinit = torch.ones(n, dtype=torch.bool, device="cuda")
+
+    def run():
+        s = st.clone()
+        o = C.gated_delta_rule_varlen_fn(q, k, v, g, b, start, None, hinit, s, A_log=A, dt_bias=dt, qk_l2norm=True)
+        return o, s
+
+    o0, s0 = run()
+    for x in (q, k, v):
+        x[70:103] = bad
+    st[1] = bad
+    o1, s1 = run()
+    assert torch.equal(o0[:70], o1[:70]) and torch.equal(o0[103:], o1[103:])
+    for i in (0, *range(2, n)):
+        assert torch.equal(s0[i], s1[i])
+    assert not torch.isfinite(o1[70:103].float()).any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_varlen_later_tokens_do_not_reach_back(bad):
     """A value that is not finite shows from its own token on, and in no chunk of 64 before."""

@@ -15,10 +15,11 @@
 // sequence (rows behind a sequence's end are zeroed).
 //
 // Precision. S, R, T, G and u are fp32 quantities. As operands they are split into two bf16 parts
-// (2^-17), and the products keep hi*hi + hi*lo + lo*hi: fp32 final states come out within 6e-6 of
-// the definition (2-norm, worst of 60 drawn batches, median 3e-6), where single bf16 operands would
-// leave 2e-3 and three parts would cost 1.6 times the products. Outputs of 16 bits are within 1.01 of
-// their own rounding. The state itself is carried in fp32 in tensor memory.
+// (2^-17), and the products keep hi*hi + hi*lo + lo*hi: fp32 final states come out within 9e-6 of
+// the definition (2-norm, random keys; median 3e-6), and within 7e-5 where all keys of a sequence
+// are the same and u cancels over its tokens. Single bf16 operands would leave 2e-3; three parts
+// would take 1.6 times the products. Outputs of 16 bits are within 1.01 of their own rounding. The
+// state itself is carried in fp32 from chunk to chunk.
 //
 // Split of the work. Chunks of one sequence form a chain; heads, sequences and the columns of the
 // state are independent. T, G and the row factors do not depend on the state: a first kernel

@@ -6,17 +6,18 @@
 // The operands that the CTA makes (S, R, u, in two bf16 parts) are then the A of their products,
 // which the tensor core reads from tensor memory: shared memory holds copies only, and every warp
 // has a share of every row (with the rows of K and Q along M, the warps of two of the SM's four
-// partitions made all of R and u). The state stays in registers, fp32. Loads and stores of tensor
-// memory use the matrix fragment shapes, so that V comes in and outputs go out by matrix
-// transposes of eight columns instead of 2-byte accesses.
+// partitions made all of R and u). The state stays in registers, fp32. R, u and the outputs use
+// the matrix fragment shapes of tensor memory, so that V comes in and outputs go out by transposes of
+// 8 x 8 matrices instead of 2-byte accesses.
 //
 // Bound. A chunk takes 5400 cycles (6800 in the form of gdr_chunk.cu): products 3100 of them
-// (36 steps of 76 cycles), splitting S, R and u 1000, 450 and 450, outputs 250, the rest waits.
-// 40807 tokens x 48 heads: 691 us against 845. Measured on the way: products issued by a worker
-// (58 cycles a step, which it waits for) 812 us; a warp of their own, 739; outputs read before the
-// last product is issued, since a TMEM load that starts beside a product waits for its end, 708;
-// fragments instead of a row to a thread, 691. Slower: those reads in flight across the arrival
-// (772), the state's update and split interleaved in two halves (726).
+// (36 steps of 76 cycles, and their latency), splitting S, R and u 1000, 450 and 450, outputs 250,
+// the rest waits. 40807 tokens x 48 heads: 687 us against 845, a seventh of it the starts and ends of
+// chains. Measured on the way: products issued by a worker (58 cycles a step, which it waits for)
+// 812 us; by a warp of their own, 739; outputs read before the last product is issued, since a
+// TMEM load that starts beside a product waits for its end, 708; fragments instead of a row to a
+// thread for V and the outputs, 691. Slower: those reads in flight across the arrival (772), the
+// state's update and split interleaved in two halves (726).
 #include "gdr_chunk.cuh"
 
 namespace cc1d {
@@ -75,6 +76,13 @@ __device__ __forceinline__ void tmem_ld_frag(uint32_t t0, float2* f) {
               "=f"(f[4 * h + 2].x), "=f"(f[4 * h + 2].y), "=f"(f[4 * h + 3].x), "=f"(f[4 * h + 3].y)
             : "r"(t0 + h * kHalf)
             : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t t0, const uint32_t* x) {
+    __syncwarp();
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(x[0]), "r"(x[1]),
+        "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]), "r"(t0)
+        : "memory");
 }
 // Pairs as words: 8 columns.
 __device__ __forceinline__ void tmem_st_frag(uint32_t t0, const uint32_t* x) {
@@ -242,18 +250,17 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
             if (++st == kStages) st = 0;
         }
     } else {
-        // This thread's state: in fragments of 16 of the part's 32 rows of the state (columns of the
-        // fragment), columns 32 w .. of the tile.
-        const int r = lane / 4, pair = lane % 4 * 2;
+        // This thread's state: column 32 w + lane of the tile, rows 32 part ..
+        const int pair = lane % 4 * 2;
         const bool initial = a.states != nullptr && a.has_initial_state != nullptr && a.has_initial_state[row];
         ST* sp = nullptr;
         if (a.states != nullptr)
-            sp = static_cast<ST*>(a.states) + slot * a.s_slot + h * a.s_sh + (32 * part + pair) * a.s_sk + vt * VS + 32 * w + r;
+            sp = static_cast<ST*>(a.states) + slot * a.s_slot + h * a.s_sh + 32 * part * a.s_sk + vt * VS + 32 * w + lane;
         float2 s[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
             s[k] = make_float2(0.f, 0.f);
-            const ST* at = sp + (8 * (k >> 3 << 1 | (k >> 1 & 1))) * a.s_sk + 16 * (k >> 2 & 1) + 8 * (k & 1);
+            const ST* at = sp + 2 * k * a.s_sk;
             if (initial) s[k] = make_float2(to_f32(at[0]), to_f32(at[a.s_sk]));
         }
         // Outputs leave in rows of 32 columns, 16 bytes a lane.
@@ -278,8 +285,8 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
                 uint32_t hi[8], lo[8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) split2(s[8 * g + k], hi[k], lo[k]);
-                tmem_st_frag(mine + kSP + 16 * part + 8 * g, hi);
-                tmem_st_frag(mine + kSP + 64 + 16 * part + 8 * g, lo);
+                tmem_st8(mine + kSP + 16 * part + 8 * g, hi);
+                tmem_st8(mine + kSP + 64 + 16 * part + 8 * g, lo);
             }
             if (left < C) {
                 // The copies of K went on into the next sequence: zeros there, whatever it holds
@@ -377,9 +384,7 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 float2 d[8];
-                tmem_ld_frag(mine + kDS + 32 * part + 16 * g, d);
-                tmem_wait_ld();
-                tmem_ready(d);
+                tmem_ld16(mine + kDS + 32 * part + 16 * g, d);
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
                     s[8 * g + k] = __ffma2_rn(make_float2(decay, decay), s[8 * g + k], d[k]);
@@ -388,7 +393,7 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
         if (sp != nullptr) {
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
-                ST* at = sp + (8 * (k >> 3 << 1 | (k >> 1 & 1))) * a.s_sk + 16 * (k >> 2 & 1) + 8 * (k & 1);
+                ST* at = sp + 2 * k * a.s_sk;
                 at[0] = from_f32<ST>(s[k].x);
                 at[a.s_sk] = from_f32<ST>(s[k].y);
             }

@@ -58,7 +58,7 @@ struct Layout {
     static constexpr int V = SB + 2 * kS;              // [64 rows]
     static constexpr int VEC = V + kR;                 // stages x row factors
     static constexpr int END = VEC + kStages * kVectorBytes;
-    static constexpr int kTmem = VS == 32 ? 128 : 256;  // of 3 VS columns
+    static constexpr int kTmem = 2 * VS;
 };
 constexpr int kThreads = 256;
 
@@ -151,7 +151,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
     const int first = warp / 4 * W;
     const bool lead = tid == 0;
     const uint32_t D = tmem;  // [product with hi parts | with lo parts]
-    const uint32_t Dh = D + lanes + first, Dl = Dh + VS, TS = Dl + VS;  // TS: the state
+    const uint32_t Dh = D + lanes + first, Dl = Dh + VS;
     const uint32_t mma = smem_addr(&sh.mma);
     const uint32_t s_hi = base + Lay::SB, s_lo = s_hi + Lay::kS;
     const uint32_t r_hi = s_hi, r_lo = r_hi + Lay::kR, u_hi = s_lo, u_lo = u_hi + Lay::kR;
@@ -164,62 +164,48 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
     constexpr int SV = Vec<ST>::V;
     T* op = static_cast<T*>(a.out) + tok0 * a.o_st + h * a.o_sh + col;
 
-    // The loop below starts with S <- decay S + product; before the first chunk that is S0 + 0.
+    float2 s[W / 16][8];  // the state
 #pragma unroll
     for (int g = 0; g < W / 16; ++g) {
-        float2 s[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) s[k] = make_float2(0.f, 0.f);
-        tmem_st16(Dh + 16 * g, s);
-        tmem_st16(Dl + 16 * g, s);
+        for (int k = 0; k < 8; ++k) s[g][k] = make_float2(0.f, 0.f);
         if (initial) {
 #pragma unroll
-            for (int k = 0; k < 16; k += SV) unpack16<ST>(ld16(sp + 16 * g + k), &s[0].x + k);
+            for (int k = 0; k < 16; k += SV) unpack16<ST>(ld16(sp + 16 * g + k), &s[g][0].x + k);
         }
-        tmem_st16(TS + 16 * g, s);
     }
-    tmem_wait_st();
     int st = 0;
     uint32_t phase = 0, st_phase = 0;
     float decay = 1.f;
     mbar_wait(smem_addr(&sh.full[0]), 0, &sh.abort);
 #pragma unroll 1
     for (int c = 0;; ++c) {
-        // The state after the chunk before, into TMEM, and as an operand if there is another.
-        {
-            float2 d[W / 16][8], e[W / 16][8], s[W / 16][8];
+        // The state after the chunk before, and as an operand if there is another.
+        if (c > 0) {
+            float2 d[W / 16][8], e[W / 16][8];
 #pragma unroll
             for (int g = 0; g < W / 16; ++g) {
                 tmem_ld16_async(Dh + 16 * g, d[g]);
                 tmem_ld16_async(Dl + 16 * g, e[g]);
-                tmem_ld16_async(TS + 16 * g, s[g]);
             }
             tmem_wait_ld();
 #pragma unroll
             for (int g = 0; g < W / 16; ++g) {
                 tmem_ready(d[g]);
                 tmem_ready(e[g]);
-                tmem_ready(s[g]);
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
                     s[g][k] = __ffma2_rn(make_float2(decay, decay), s[g][k], __fadd2_rn(d[g][k], e[g][k]));
-                if (c == chunks) {
-                    if (sp != nullptr) {
-#pragma unroll
-                        for (int k = 0; k < 16; k += SV) st16(sp + 16 * g + k, pack16<ST>(&s[g][0].x + k));
-                    }
-                } else {
-                    tmem_st16(TS + 16 * g, s[g]);
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const uint32_t at = swz<Lay::kRow>(p, first / 8 + 2 * g + u);
-                        store_split8(s_hi + at, s_lo + at, s[g] + 4 * u);
-                    }
-                }
             }
         }
         if (c == chunks) break;
-        tmem_wait_st();
+#pragma unroll
+        for (int g = 0; g < W / 16; ++g)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t at = swz<Lay::kRow>(p, first / 8 + 2 * g + u);
+                store_split8(s_hi + at, s_lo + at, s[g] + 4 * u);
+            }
         const uint32_t kq = base + Lay::KQ + st * Lay::kKQ, tg = base + Lay::TG + st * 32768;
         const int left = ntok - c * C;
         if (left < C) {
@@ -371,6 +357,12 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
         mbar_wait(mma, phase, &sh.abort);
         phase ^= 1;
         tc_fence_after();
+    }
+    if (sp != nullptr) {
+#pragma unroll
+        for (int g = 0; g < W / 16; ++g)
+#pragma unroll
+            for (int k = 0; k < 16; k += SV) st16(sp + 16 * g + k, pack16<ST>(&s[g][0].x + k));
     }
     tc_fence_before();
     __syncthreads();

@@ -34,7 +34,7 @@
 // and the rest is TMEM loads, splitting, barriers. Tiles of 128 columns, for many heads, have a
 // kernel of their own (gdr_wide.cu); in the form used here they took 6800 cycles a chunk, two
 // independent chains of 64 in one CTA 7700, and two tiles in turn, with warps of their own for
-// products and loads, 7400 (3500 at 32 columns).
+// products and loads, 7400 (3500 at 32 columns). Twice the threads at 32 columns: 3050.
 //
 // Stacking K over Q and T over G makes every product M = 128, the full tensor core rate; the two
 // parts of an operand lie side by side as one operand of 2 VS columns (measured: a K step of 16

@@ -47,6 +47,7 @@ enum : uint32_t {
     kDS = 384,         // u^T K
     kColumns = 512
 };
+
 // Named barriers: the operand of a product is written.
 enum { kHaveS = 1, kHaveR, kHaveU };
 
@@ -63,6 +64,7 @@ __device__ __forceinline__ void arrive(int id) {
     tc_fence_before();
     asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(kThreads) : "memory");
 }
+
 // Fragments: a warp's 32 rows (of M) by 16 columns, eight pairs of neighbouring columns to a lane.
 // Pair 4 half + 2 block + below is row 16 half + 8 below + lane / 4, columns 8 block + lane % 4 * 2.
 constexpr uint32_t kHalf = 16u << 16;  // 16 TMEM lanes
@@ -93,6 +95,7 @@ __device__ __forceinline__ void tmem_st_frag(uint32_t t0, const uint32_t* x) {
                      "r"(x[4 * h + 1]), "r"(x[4 * h + 2]), "r"(x[4 * h + 3]), "r"(t0 + h * kHalf)
                      : "memory");
 }
+
 // Four 8 x 8 matrices of 16-bit values, transposed between shared memory and registers. A lane gives
 // the address of row lane % 8 of matrix lane / 8 and has pair lane % 4 of column lane / 4 of each.
 __device__ __forceinline__ void ldsm_t(uint32_t addr, uint32_t* x) {
@@ -113,6 +116,7 @@ __device__ __forceinline__ float2 lds_pair(uint32_t addr) {
     asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
     return v;
 }
+
 // Two values as T, the first in the low half.
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float2 f) {
@@ -124,6 +128,7 @@ __device__ __forceinline__ uint32_t pack2(float2 f) {
     }
     return v;
 }
+
 template <typename T, typename ST>
 __global__ void __launch_bounds__(kThreads, 1)
 gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__ CUtensorMap mapq,
@@ -142,7 +147,8 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
     const int vt = blockIdx.x % tiles;
     const int h = (int)((blockIdx.x / tiles) % a.heads_v);
     const int hk = h / (a.heads_v / a.heads_k);
-    const int64_t row = longest_first(a, blockIdx.x / tiles / a.heads_v, reinterpret_cast<int*>(gen), &sh.row);
+    const int64_t row =
+        longest_first(a, blockIdx.x / tiles / a.heads_v, reinterpret_cast<int*>(gen), &sh.row);
     int64_t tok0, slot;
     int ntok;
     if (!gdr_row(a, true, row, tok0, ntok, slot, h == 0 && vt == 0 && tid == 0)) return;
@@ -186,7 +192,8 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
                     const uint32_t s = tmem + kSP + half * 32;
                     mma_steps_ts<4, 2>(tmem + kDK, s, k, mma_desc(128, false, false), half > 0);
                     mma_steps_ts<4, 2>(tmem + kDK, s + 64, k, mma_desc(128, false, false), true);
-                    if constexpr (kLo) mma_steps_ts<4, 2>(tmem + kDK, s, k + 2048, mma_desc(128, false, false), true);
+                    if constexpr (kLo)
+                        mma_steps_ts<4, 2>(tmem + kDK, s, k + 2048, mma_desc(128, false, false), true);
                 }
                 mma_commit(mma);
             }
@@ -255,7 +262,8 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
         const bool initial = a.states != nullptr && a.has_initial_state != nullptr && a.has_initial_state[row];
         ST* sp = nullptr;
         if (a.states != nullptr)
-            sp = static_cast<ST*>(a.states) + slot * a.s_slot + h * a.s_sh + 32 * part * a.s_sk + vt * VS + 32 * w + lane;
+            sp = static_cast<ST*>(a.states) + slot * a.s_slot + h * a.s_sh + 32 * part * a.s_sk + vt * VS +
+                 32 * w + lane;
         float2 s[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
@@ -264,13 +272,15 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
             if (initial) s[k] = make_float2(to_f32(at[0]), to_f32(at[a.s_sk]));
         }
         // Outputs leave in rows of 32 columns, 16 bytes a lane.
-        T* op = static_cast<T*>(a.out) + (tok0 + 16 * part + lane / 4) * a.o_st + h * a.o_sh + vt * VS + 32 * w + lane % 4 * 8;
+        T* op = static_cast<T*>(a.out) + (tok0 + 16 * part + lane / 4) * a.o_st + h * a.o_sh + vt * VS + 32 * w +
+                lane % 4 * 8;
         // Matrices of V: [block of tokens][below] of a half.
         const uint32_t vb = base + Lay::V + (w >> 1) * 8192;
         const int v_row = 16 * part + (lane >> 4) * 8 + lane % 8, v_unit = (w & 1) * 4 + (lane >> 3 & 1);
         const uint32_t mma = smem_addr(&sh.mma);
         const uint32_t patch = base + Lay::O + warp * 512;
-        const uint32_t patch_st = patch + swz<64>(lane % 8, lane / 8), patch_ld = patch + swz<64>(lane / 4, lane % 4);
+        const uint32_t patch_st = patch + swz<64>(lane % 8, lane / 8);
+        const uint32_t patch_ld = patch + swz<64>(lane / 4, lane % 4);
 
         int st = 0;
         uint32_t phase = 0, st_phase = 0;

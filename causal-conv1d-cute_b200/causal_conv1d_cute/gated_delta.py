@@ -122,8 +122,10 @@ def gated_delta_rule_varlen_fn(
         out: optional output of the shape and dtype of v.
 
     bf16 and fp16 calls with dk = 128, rows on 16-byte boundaries and 10 tokens a sequence on average
-    run chunk by chunk on the tensor cores, with a temporary of 524 bytes per token and value head (in
-    groups of heads from 4 GiB on); others token by token in fp32.
+    run chunk by chunk on the tensor cores, whose operands hold the 24 bits of fp32 in three parts: final
+    states are as near to the definition as token by token. Their temporary takes 49,936 bytes per
+    value head for each of tokens / 64 + batch chunks, and 1024 bytes per token and key head more for
+    fp16 (in groups of heads from 4 GiB on). Other calls run token by token.
 
     Returns:
         (total_tokens, heads_v, dv) output.

@@ -14,32 +14,34 @@
 // spoils the rows of its chunk, earlier ones included; it reaches no earlier chunk, and no other
 // sequence (rows behind a sequence's end are zeroed).
 //
-// Precision. S, R, T, G and u are fp32 quantities. As operands they are split into two bf16 parts
-// (2^-17), and the products keep hi*hi + hi*lo + lo*hi: fp32 final states come out within 9e-6 of
-// the definition (2-norm, random keys; median 3e-6), and within 7e-5 where all keys of a sequence
-// are the same and u cancels over its tokens. Single bf16 operands would leave 2e-3; three parts
-// would take 1.6 times the products. Outputs of 16 bits are within 1.01 of their own rounding. The
-// state itself is carried in fp32 from chunk to chunk.
+// Precision. S, R, T, G and u are fp32 quantities. As operands they are split into three bf16 parts,
+// which hold all 24 bits; of the products of two split operands those of 2^-27 are left out, and
+// small products are added among themselves before they meet the large ones, because the tensor core
+// cuts its sums to fp32 after every step (summed the other way the errors are two to five times as
+// large). fp32 final states come out within 4e-7 of the definition (2-norm of a head; all together 1.3e-7,
+// as token by token), keys that are all the same among them. Two parts, which need 0.6 of the products,
+// left 2e-6 to 9e-6, and 7e-5 where all keys of a sequence are the same and u cancels over its tokens.
+// The state itself is carried in fp32 from chunk to chunk.
 //
 // Split of the work. Chunks of one sequence form a chain; heads, sequences and the columns of the
 // state are independent. T, G and the row factors do not depend on the state: a first kernel
-// (gdr_prep.cu) makes them for all chunks in parallel and leaves them in a workspace, 33.6 KB per
+// (gdr_prep.cu) makes them for all chunks in parallel and leaves them in a workspace, 50 KB per
 // chunk and head. (One kernel with warps for either part was tried first: a chunk's T and G take
 // longer than its step of the chain, and shared memory has no room for more of them in flight.)
 // The kernel here walks the chain: [K;Q] S0, R, [T;G] R, u, K^T u, S. A CTA takes one head of one
 // sequence and VS state columns; all its warps turn a product into the operand of the next together.
 // K, Q, T and G come by TMA and bulk copies a chunk or two ahead.
 //
-// Bound. The latency of the chain: 2950 cycles a chunk at VS = 32, of which the products take half
-// and the rest is TMEM loads, splitting, barriers. Tiles of 128 columns, for many heads, have a
-// kernel of their own (gdr_wide.cu); in the form used here they took 6800 cycles a chunk, two
-// independent chains of 64 in one CTA 7700, and two tiles in turn, with warps of their own for
-// products and loads, 7400 (3500 at 32 columns). Twice the threads at 32 columns: 3050.
+// Bound. The latency of the chain: 2.1 us a chunk at VS = 32 (8192 tokens x 12 heads 270 us), of which
+// the products take half and the rest is TMEM loads, splitting, barriers. Tiles of 128 columns, for
+// many heads, have a kernel of their own (gdr_wide.cu). Measured with operands in two parts: 2950
+// cycles a chunk at VS = 32; in this form 6800 with 128 columns, two independent chains of 64 in one CTA
+// 7700, and two tiles in turn, with warps of their own for products and loads, 7400 (3500 at 32
+// columns); twice the threads at 32 columns 3050.
 //
-// Stacking K over Q and T over G makes every product M = 128, the full tensor core rate; the two
-// parts of an operand lie side by side as one operand of 2 VS columns (measured: a K step of 16
-// costs 46 cycles up to 64 columns, 66 with 128 and 137 with 256, so one wide step beats two narrow
-// ones).
+// Stacking K over Q and T over G makes every product M = 128, the full tensor core rate; the parts of
+// an operand lie side by side as one operand of 3 VS columns (measured: a K step of 16 costs 46 cycles
+// up to 64 columns, 66 with 128 and 137 with 256, so one wide step beats two narrow ones).
 #include "gdr_chunk.cuh"
 
 namespace cc1d {
@@ -48,32 +50,48 @@ namespace {
 template <int VS, bool kLo>
 struct Layout {
     static constexpr int kRow = 2 * VS;        // bytes of a row of columns
-    static constexpr int kS = 128 * kRow;      // one part (hi or lo) of S
+    static constexpr int kS = 128 * kRow;      // one part of S
     static constexpr int kR = C * kRow;        // one part of R or u, or V
     static constexpr int kKQ = Parts<kLo>::kBytes;
-    static constexpr int kStages = VS == 32 && !kLo ? 3 : 2;
+    static constexpr int kStages = 2;                  // of K, Q and the row factors
+    static constexpr int kTgStages = kLo ? 1 : 2;      // of T and G
     static constexpr int KQ = 0;                       // stages x K and Q
-    static constexpr int TG = KQ + kStages * kKQ;      // stages x [hi, lo][128 rows][128 B]
-    static constexpr int SB = TG + kStages * 32768;    // S hi, S lo; R in S hi, u in S lo
-    static constexpr int V = SB + 2 * kS;              // [64 rows]
+    static constexpr int TG = KQ + kStages * kKQ;      // stages x [3 parts][128 rows][128 B]
+    static constexpr int SB = TG + kTgStages * kTgBytes;  // the parts of S; in their place those of R and u
+    static constexpr int V = SB + 3 * kS;              // [64 rows]
     static constexpr int VEC = V + kR;                 // stages x row factors
     static constexpr int END = VEC + kStages * kVectorBytes;
-    static constexpr int kTmem = 2 * VS;
+    static constexpr int kTmem = VS == 32 ? 128 : 256;  // a power of two from 3 VS on
 };
 constexpr int kThreads = 256;
 
 struct Shared {
-    uint64_t full[3], v_full, mma;
+    uint64_t full[2], tg_full[2], v_full, mma;
     uint32_t tmem;
     int abort;
     int row;  // sequence of this CTA
 };
 
-// One thread: D (+)= A B over kSteps K steps, the two parts of B side by side as one operand of 2 VS
-// columns, whose products are added on the way out of TMEM.
-template <int VS, int kSteps, int kA, bool kTransposedA>
-__device__ __forceinline__ void two_part_product(uint32_t d, uint64_t a, uint64_t b, bool accumulate) {
-    mma_steps<kSteps, kA, 2 * VS>(d, a, b, mma_desc(2 * VS, kTransposedA, true), accumulate);
+// One thread: D (+)= A B over kSteps K steps, the first kParts parts of B side by side as one operand
+// of kParts VS columns, whose products are added on the way out of TMEM.
+template <int VS, int kParts, int kSteps, int kA, bool kTransposedA>
+__device__ __forceinline__ void parts_product(uint32_t d, uint64_t a, uint64_t b, bool accumulate) {
+    mma_steps<kSteps, kA, 2 * VS>(d, a, b, mma_desc(kParts * VS, kTransposedA, true), accumulate);
+}
+
+// 16 columns of a product, its parts added.
+template <int VS>
+__device__ __forceinline__ void load_sum(uint32_t d, float2* f) {
+    float2 e[8], g[8];
+    tmem_ld16_async(d, f);
+    tmem_ld16_async(d + VS, e);
+    tmem_ld16_async(d + 2 * VS, g);
+    tmem_wait_ld();
+    tmem_ready(f);
+    tmem_ready(e);
+    tmem_ready(g);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = __fadd2_rn(f[k], __fadd2_rn(e[k], g[k]));
 }
 
 template <typename T, typename ST, int VS>
@@ -85,7 +103,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
     using Lay = Layout<VS, kLo>;
     constexpr uint64_t kSwz = VS == 64 ? kSwizzle128 : kSwizzle64;
     constexpr uint32_t kGroup = 8 * Lay::kRow;  // bytes of eight rows of V columns
-    constexpr int kStages = Lay::kStages;
+    constexpr int kStages = Lay::kStages, kTgStages = Lay::kTgStages;
     extern __shared__ __align__(1024) unsigned char raw[];
     __shared__ Shared sh;
     const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
@@ -107,7 +125,10 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
         static_cast<const ChunkImage*>(a.workspace) + chunk_base(tok0, row) * a.heads_v + h;
 
     if (tid == 0) {
-        for (int i = 0; i < 3; ++i) mbar_init(smem_addr(&sh.full[i]), 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_addr(&sh.full[i]), 1);
+            mbar_init(smem_addr(&sh.tg_full[i]), 1);
+        }
         mbar_init(smem_addr(&sh.v_full), 1);
         mbar_init(smem_addr(&sh.mma), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -125,14 +146,20 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
     const uint32_t tmem = sh.tmem;
     const uint32_t lanes = (uint32_t)w << 21;  // the warp's first TMEM lane, in bits 16..
 
-    // K, Q, T, G and the row factors of chunk c into stage st, which must be free; one thread.
+    // K, Q and the row factors of chunk c into stage st, which must be free; one thread.
     auto load = [&](int c, int st) {
         const uint32_t full = smem_addr(&sh.full[st]);
         const ChunkImage* from = image + (int64_t)c * a.heads_v;
-        mbar_expect(full, Lay::kKQ + 32768 + kVectorBytes);
+        mbar_expect(full, Lay::kKQ + kVectorBytes);
         load_kq<kLo>(base + Lay::KQ + st * Lay::kKQ, &mapk, &mapq, hk, (int)tok0 + c * C, full);
         bulk_load(base + Lay::VEC + st * kVectorBytes, from->in, kVectorBytes, full);
-        bulk_load(base + Lay::TG + st * 32768, from->tg, 32768, full);
+    };
+    // T and G of chunk c, into the stage of their own.
+    auto load_tg = [&](int c) {
+        const int st = c % kTgStages;
+        const uint32_t full = smem_addr(&sh.tg_full[st]);
+        mbar_expect(full, kTgBytes);
+        bulk_load(base + Lay::TG + st * kTgBytes, image[(int64_t)c * a.heads_v].tg, kTgBytes, full);
     };
     // V of chunk c.
     auto load_v = [&](int c) {
@@ -143,6 +170,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
     grid_dependency_wait();  // for the prep kernel's images
     if (tid == 0) {
         for (int c = 0; c < kStages && c < chunks; ++c) load(c, c);
+        for (int c = 0; c < kTgStages && c < chunks; ++c) load_tg(c);
         load_v(0);
     }
 
@@ -150,11 +178,10 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
     constexpr int W = VS * 128 / kThreads;
     const int first = warp / 4 * W;
     const bool lead = tid == 0;
-    const uint32_t D = tmem;  // [product with hi parts | with lo parts]
-    const uint32_t Dh = D + lanes + first, Dl = Dh + VS;
+    const uint32_t D = tmem;  // products with the parts of B, side by side
+    const uint32_t Dp = D + lanes + first;
     const uint32_t mma = smem_addr(&sh.mma);
-    const uint32_t s_hi = base + Lay::SB, s_lo = s_hi + Lay::kS;
-    const uint32_t r_hi = s_hi, r_lo = r_hi + Lay::kR, u_hi = s_lo, u_lo = u_hi + Lay::kR;
+    const uint32_t sb = base + Lay::SB, rb = sb, ub = rb + 3 * Lay::kR;
     const uint32_t vb = base + Lay::V;
     const int col = vt * VS + first;
     const bool initial = a.states != nullptr && a.has_initial_state != nullptr && a.has_initial_state[row];
@@ -182,20 +209,12 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
     for (int c = 0;; ++c) {
         // The state after the chunk before, and as an operand if there is another.
         if (c > 0) {
-            float2 d[W / 16][8], e[W / 16][8];
 #pragma unroll
             for (int g = 0; g < W / 16; ++g) {
-                tmem_ld16_async(Dh + 16 * g, d[g]);
-                tmem_ld16_async(Dl + 16 * g, e[g]);
-            }
-            tmem_wait_ld();
+                float2 d[8];
+                load_sum<VS>(Dp + 16 * g, d);
 #pragma unroll
-            for (int g = 0; g < W / 16; ++g) {
-                tmem_ready(d[g]);
-                tmem_ready(e[g]);
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    s[g][k] = __ffma2_rn(make_float2(decay, decay), s[g][k], __fadd2_rn(d[g][k], e[g][k]));
+                for (int k = 0; k < 8; ++k) s[g][k] = __ffma2_rn(make_float2(decay, decay), s[g][k], d[k]);
             }
         }
         if (c == chunks) break;
@@ -204,9 +223,9 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const uint32_t at = swz<Lay::kRow>(p, first / 8 + 2 * g + u);
-                store_split8(s_hi + at, s_lo + at, s[g] + 4 * u);
+                store_split8(sb + at, Lay::kS, s[g] + 4 * u);
             }
-        const uint32_t kq = base + Lay::KQ + st * Lay::kKQ, tg = base + Lay::TG + st * 32768;
+        const uint32_t kq = base + Lay::KQ + st * Lay::kKQ, tg = base + Lay::TG + c % kTgStages * kTgBytes;
         const int left = ntok - c * C;
         if (left < C) {
             // The copies of K went on into the next sequence: zeros there, whatever it holds
@@ -222,12 +241,13 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
         if (lead) {
             tc_fence_after();
             // [K;Q] S
-            const uint64_t k = operand(kq, 16, 1024, kSwizzle128), s = operand(s_hi, 128 * Lay::kRow, kGroup, kSwz);
-            two_part_product<VS, 4, 2, false>(D, k, s, false);
-            two_part_product<VS, 4, 2, false>(D, k + 1024, s + kGroup / 2, true);
+            const uint64_t k = operand(kq, 16, 1024, kSwizzle128), s = operand(sb, Lay::kS, kGroup, kSwz);
+            parts_product<VS, 3, 4, 2, false>(D, k, s, false);
+            parts_product<VS, 3, 4, 2, false>(D, k + 1024, s + kGroup / 2, true);
             if constexpr (kLo) {
-                mma_steps<4, 2, kGroup / 8>(D, k + 2048, s, mma_desc(VS, false, true), true);
-                mma_steps<4, 2, kGroup / 8>(D, k + 3072, s + kGroup / 2, mma_desc(VS, false, true), true);
+                // Their sums belong to the second and third parts'.
+                parts_product<VS, 2, 4, 2, false>(D + VS, k + 2048, s, true);
+                parts_product<VS, 2, 4, 2, false>(D + VS, k + 3072, s + kGroup / 2, true);
             }
             mma_commit(mma);
         }
@@ -241,99 +261,79 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
         mbar_wait(mma, phase, &sh.abort);
         phase ^= 1;
         tc_fence_after();
-        {
-            float2 d[W / 16][8], e[W / 16][8];
+        if (p < C) {
+            // R = V - r e^b (K S), zero behind the sequence's end, whatever V holds there
+            const bool live = p < left;
 #pragma unroll
             for (int g = 0; g < W / 16; ++g) {
-                tmem_ld16_async(Dh + 16 * g, d[g]);
-                tmem_ld16_async(Dl + 16 * g, e[g]);
+                uint4 v[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) v[u] = lds16(vb + swz<Lay::kRow>(p, first / 8 + 2 * g + u));
+                float2 d[8];
+                load_sum<VS>(Dp + 16 * g, d);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t vv[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+                    float2 f[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) f[k] = add_pair<T>(live ? vv[k] : 0u, mul2(d[4 * u + k], -in));
+                    store_split8(rb + swz<Lay::kRow>(p, first / 8 + 2 * g + u), Lay::kR, f);
+                }
             }
-            if (p < C) {
-                // R = V - r e^b (K S), zero behind the sequence's end, whatever V holds there
-                const bool live = p < left;
-                uint4 v[W / 8];
+            fence_async_smem();
+        } else {
 #pragma unroll
-                for (int u = 0; u < W / 8; ++u) v[u] = lds16(vb + swz<Lay::kRow>(p, first / 8 + u));
-                tmem_wait_ld();
+            for (int g = 0; g < W / 16; ++g) {
+                float2 d[8];
+                load_sum<VS>(Dp + 16 * g, d);
 #pragma unroll
-                for (int g = 0; g < W / 16; ++g) {
-                    tmem_ready(d[g]);
-                    tmem_ready(e[g]);
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const uint32_t vv[4] = {v[2 * g + u].x, v[2 * g + u].y, v[2 * g + u].z, v[2 * g + u].w};
-                        float2 f[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            f[k] = add_pair<T>(live ? vv[k] : 0u, mul2(__fadd2_rn(d[g][4 * u + k], e[g][4 * u + k]), -in));
-                        const uint32_t at = swz<Lay::kRow>(p, first / 8 + 2 * g + u);
-                        store_split8(r_hi + at, r_lo + at, f);
-                    }
-                }
-                fence_async_smem();
-            } else {
-                tmem_wait_ld();
-#pragma unroll
-                for (int g = 0; g < W / 16; ++g) {
-                    tmem_ready(d[g]);
-                    tmem_ready(e[g]);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) q[8 * g + k] = mul2(__fadd2_rn(d[g][k], e[g][k]), in);
-                }
+                for (int k = 0; k < 8; ++k) q[8 * g + k] = mul2(d[k], in);
             }
         }
         tc_fence_before();
         __syncthreads();
         if (lead) {
+            mbar_wait(smem_addr(&sh.tg_full[c % kTgStages]), c / kTgStages & 1, &sh.abort);
             tc_fence_after();
-            // [T;G] R: hi [hi | lo], then lo hi
-            const uint64_t r = operand(r_hi, C * Lay::kRow, kGroup, kSwz);
-            two_part_product<VS, 4, 2, false>(D, operand(tg, 16, 1024, kSwizzle128), r, false);
-            mma_steps<4, 2, kGroup / 8>(D, operand(tg + 16384, 16, 1024, kSwizzle128), r, mma_desc(VS, false, true), true);
+            // [T;G] R, part by part of [T;G]
+            const uint64_t r = operand(rb, Lay::kR, kGroup, kSwz), g = operand(tg, 16, 1024, kSwizzle128);
+            parts_product<VS, 3, 4, 2, false>(D, g, r, false);
+            parts_product<VS, 2, 4, 2, false>(D + VS, g + 1024, r, true);
+            parts_product<VS, 1, 4, 2, false>(D + 2 * VS, g + 2048, r, true);
             mma_commit(mma);
             if (c + 1 < chunks) load_v(c + 1);
         }
         mbar_wait(mma, phase, &sh.abort);
         phase ^= 1;
         tc_fence_after();
-        {
-            float2 d[W / 16][8], e[W / 16][8];
 #pragma unroll
-            for (int g = 0; g < W / 16; ++g) {
-                tmem_ld16_async(Dh + 16 * g, d[g]);
-                tmem_ld16_async(Dl + 16 * g, e[g]);
+        for (int g = 0; g < W / 16; ++g) {
+            float2 d[8];
+            load_sum<VS>(Dp + 16 * g, d);
+            if (p < C) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) d[k] = mul2(d[k], out);
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    store_split8(ub + swz<Lay::kRow>(p, first / 8 + 2 * g + u), Lay::kR, d + 4 * u);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) q[8 * g + k] = __fadd2_rn(q[8 * g + k], d[k]);
             }
-            tmem_wait_ld();
-#pragma unroll
-            for (int g = 0; g < W / 16; ++g) {
-                tmem_ready(d[g]);
-                tmem_ready(e[g]);
-                if (p < C) {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) d[g][k] = mul2(__fadd2_rn(d[g][k], e[g][k]), out);
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const uint32_t at = swz<Lay::kRow>(p, first / 8 + 2 * g + u);
-                        store_split8(u_hi + at, u_lo + at, d[g] + 4 * u);
-                    }
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        q[8 * g + k] = __fadd2_rn(q[8 * g + k], __fadd2_rn(d[g][k], e[g][k]));
-                }
-            }
-            if (p < C) fence_async_smem();
         }
+        if (p < C) fence_async_smem();
         tc_fence_before();
         __syncthreads();
         if (lead) {
             tc_fence_after();
             // K^T u
-            const uint64_t k = operand(kq, 16384, 1024, kSwizzle128), u = operand(u_hi, C * Lay::kRow, kGroup, kSwz);
-            two_part_product<VS, 4, 128, true>(D, k, u, false);
-            if constexpr (kLo) mma_steps<4, 128, kGroup / 8>(D, k + 2048, u, mma_desc(VS, true, true), true);
+            const uint64_t k = operand(kq, 16384, 1024, kSwizzle128), u = operand(ub, Lay::kR, kGroup, kSwz);
+            parts_product<VS, 3, 4, 128, true>(D, k, u, false);
+            if constexpr (kLo) parts_product<VS, 2, 4, 128, true>(D + VS, k + 2048, u, true);
             mma_commit(mma);
         }
+        // [T;G] R is through: the next T and G into its place.
+        if (tid == 64 && c + kTgStages < chunks) load_tg(c + kTgStages);
         const int t = c * C + p - C;
         if (p >= C && t < ntok) {
             T* to = op + (int64_t)t * a.o_st;

@@ -15,13 +15,14 @@ constexpr int DK = 128;  // key head dim
 
 // What the prep kernel leaves of a chunk and value head for the scan kernel.
 struct ChunkImage {
-    unsigned char tg[2][128 * 128];  // [T;G], hi and lo bf16 parts, 128-byte rows, swizzled
+    unsigned char tg[3][128 * 128];  // [T;G] in three bf16 parts, 128-byte rows, swizzled
     float in[2 * C];                 // r_i e^(b_i) (rows of K), s_i e^(b_i) (rows of Q)
     float out[C];                    // r_j e^(b_C - b_j)
     float decay;                     // e^(b_C)
     float pad[3];
 };
-constexpr int kVectorBytes = (int)sizeof(ChunkImage) - 32768;  // what follows tg
+constexpr int kTgBytes = 3 * 128 * 128;
+constexpr int kVectorBytes = (int)sizeof(ChunkImage) - kTgBytes;  // what follows tg
 
 // The row factors of a ChunkImage, as they follow its T and G.
 struct Vectors {
@@ -48,13 +49,13 @@ __device__ __forceinline__ uint32_t swz(int r, int u) {
     }
 }
 
-// 8 values as two bf16 parts, one 16-byte unit each.
-__device__ __forceinline__ void store_split8(uint32_t hi, uint32_t lo, const float2* f) {
-    uint32_t h[4], l[4];
+// 8 values as three bf16 parts, one 16-byte unit each, `part` bytes apart.
+__device__ __forceinline__ void store_split8(uint32_t at, uint32_t part, const float2* f) {
+    uint32_t x[3][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) split2(f[i], h[i], l[i]);
-    sts16(hi, h[0], h[1], h[2], h[3]);
-    sts16(lo, l[0], l[1], l[2], l[3]);
+    for (int i = 0; i < 4; ++i) split3(f[i], x[0][i], x[1][i], x[2][i]);
+#pragma unroll
+    for (int m = 0; m < 3; ++m) sts16(at + m * part, x[m][0], x[m][1], x[m][2], x[m][3]);
 }
 __device__ __forceinline__ float2 mul2(float2 a, float b) {
     return __fmul2_rn(a, make_float2(b, b));

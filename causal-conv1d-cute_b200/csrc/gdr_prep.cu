@@ -2,20 +2,20 @@
 // gdr_chunk.cu has the mathematics; here, per chunk of 64 tokens and value head,
 //     L_ij = beta_i r_i r_j e^(b_i - b_j) k_i.k_j  (j < i),   T = (I + L)^-1 diag(beta),
 //     P_ij = s_i r_j e^(b_i - b_j) q_i.k_j         (j <= i),  G = P T,
-// and the row factors of the scan. The chunks are independent, so latency is hidden by four CTAs
-// per SM rather than inside one.
+// and the row factors of the scan. The chunks are independent, so latency is hidden by three
+// CTAs per SM (fp16: two) rather than inside one.
 //
 // A CTA of four warps takes one chunk of one query/key head: K and Q by TMA, [K;Q] K^T on the tensor
 // core and the norms once, then the value heads of the group one after another. The inverse goes in
 // blocks: 16 x 16 by substitution in registers (a lane owns a row, rows of L come as broadcasts),
-// the blocks below the diagonal by -inv_1 (L_21 inv_0) in two-part bf16 on the warp-level tensor
+// the blocks below the diagonal by -inv_1 (L_21 inv_0) in three-part bf16 on the warp-level tensor
 // core (120 dependent fp32 steps a row instead of the 2016 of plain substitution). G is a product on
 // the tensor core again. T leaves by a bulk copy, G from registers.
 //
-// Bound: instruction latency and issue, with 16 warps an SM (tensor memory and shared memory allow
-// four CTAs): 6200 warp instructions per chunk and value head at 0.4 a cycle and scheduler. 30600
-// chunks and heads take 424 us (3400 cycles each per SM), 1.0 GB written. Plain substitution over the
-// whole chunk took 5000 to 15000 cycles for the inverse alone.
+// Bound: instruction latency and issue, with 12 warps an SM (the parts of T and P leave shared memory
+// for three CTAs). 30600 chunks and heads take 632 us, 1.5 GB written. With T, P and G in two parts and
+// four CTAs it was 424 us (6200 warp instructions per chunk and value head at 0.4 a cycle and
+// scheduler). Plain substitution over the whole chunk took 5000 to 15000 cycles for the inverse alone.
 #include "gdr_chunk.cuh"
 
 namespace cc1d {
@@ -37,7 +37,8 @@ struct Gates {
 
 template <bool kLo>
 struct Smem {
-    unsigned char kq[Parts<kLo>::kBytes];  // K and Q; later T hi, T lo, P hi, P lo
+    // K and Q; later the parts of T, then those of P
+    unsigned char kq[Parts<kLo>::kBytes > 6 * 8192 ? Parts<kLo>::kBytes : 6 * 8192];
     Blocks blk;
     Gates gates[kHeads];
     alignas(16) float rk[C], ru[kHeads][32];  // inverse norms of the keys; with e^(b_31 - b_j)
@@ -73,14 +74,19 @@ __device__ __forceinline__ void mma_warp(float* d, const uint32_t* a, const uint
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
-__device__ __forceinline__ void mma_warp3(float* d, const uint32_t (*a)[4], const uint32_t (*b)[2]) {
-    mma_warp(d, a[0], b[0]);
+// The same of operands in three parts, the smallest products first: a sum is cut to fp32 after every
+// step. The products left out are 2^-27 of the whole.
+__device__ __forceinline__ void mma_warp_parts(float* d, const uint32_t (*a)[4], const uint32_t (*b)[2]) {
+    mma_warp(d, a[0], b[2]);
+    mma_warp(d, a[2], b[0]);
+    mma_warp(d, a[1], b[1]);
     mma_warp(d, a[0], b[1]);
     mma_warp(d, a[1], b[0]);
+    mma_warp(d, a[0], b[0]);
 }
 
 // The 16 x 16 tile inv1[r0.., :] (low inv0)[:, c0..] of a product of K x K matrices, K = 16 or 32,
-// by one warp in two-part bf16. The inner product is formed transposed, (inv0^T low^T): its
+// by one warp in three-part bf16. The inner product is formed transposed, (inv0^T low^T): its
 // accumulator fragments are then the B fragments of the outer one. d: accumulators of columns c0..
 // and c0 + 8...
 template <int K>
@@ -92,43 +98,43 @@ __device__ __forceinline__ void merge_tile(const float (*inv1)[LPAD], const floa
     float m[K / 16][K / 8][4];  // (low inv0)^T: rows c0.., 8 columns (rows of low) each
 #pragma unroll
     for (int k = 0; k < K / 16; ++k) {
-        uint32_t av[2][4];
+        uint32_t av[3][4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int col = c0 + g + e % 2 * 8, r = 16 * k + t2 + e / 2 * 8;
-            split2(make_float2(inv0[r][col], inv0[r + 1][col]), av[0][e], av[1][e]);
+            split3(make_float2(inv0[r][col], inv0[r + 1][col]), av[0][e], av[1][e], av[2][e]);
         }
 #pragma unroll
         for (int n = 0; n < K / 8; ++n) {
-            uint32_t bv[2][2];
+            uint32_t bv[3][2];
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-                split2(*reinterpret_cast<const float2*>(&low[8 * n + g][16 * k + t2 + 8 * e]), bv[0][e], bv[1][e]);
+                split3(*reinterpret_cast<const float2*>(&low[8 * n + g][16 * k + t2 + 8 * e]), bv[0][e], bv[1][e], bv[2][e]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) m[k][n][e] = 0.f;
-            mma_warp3(m[k][n], av, bv);
+            mma_warp_parts(m[k][n], av, bv);
         }
     }
     float s[K / 16][2][4];
 #pragma unroll
     for (int k = 0; k < K / 16; ++k) {
-        uint32_t av[2][4];
+        uint32_t av[3][4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            split2(*reinterpret_cast<const float2*>(&inv1[r0 + g + e % 2 * 8][16 * k + t2 + e / 2 * 8]), av[0][e], av[1][e]);
+            split3(*reinterpret_cast<const float2*>(&inv1[r0 + g + e % 2 * 8][16 * k + t2 + e / 2 * 8]), av[0][e], av[1][e], av[2][e]);
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            uint32_t bv[2][2];
+            uint32_t bv[3][2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 float2 f = make_float2(m[0][2 * k + e][2 * n], m[0][2 * k + e][2 * n + 1]);
                 if (K > 16)
                     f = __fadd2_rn(f, make_float2(m[K / 16 - 1][2 * k + e][2 * n], m[K / 16 - 1][2 * k + e][2 * n + 1]));
-                split2(f, bv[0][e], bv[1][e]);
+                split3(f, bv[0][e], bv[1][e], bv[2][e]);
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[k][n][e] = 0.f;
-            mma_warp3(s[k][n], av, bv);
+            mma_warp_parts(s[k][n], av, bv);
         }
     }
 #pragma unroll
@@ -148,12 +154,12 @@ __device__ __forceinline__ float bits_value(uint32_t b, int dtype) {
 }
 
 template <bool kLo>
-__global__ void __launch_bounds__(128, 4)
+__global__ void __launch_bounds__(128, kLo ? 2 : 3)
 gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__ CUtensorMap mapq,
                 const __grid_constant__ CUtensorMap mapk) {
     extern __shared__ __align__(1024) unsigned char raw[];
     Smem<kLo>& sh = *reinterpret_cast<Smem<kLo>*>(raw + ((1024 - (smem_addr(raw) & 1023)) & 1023));
-    const uint32_t kq = smem_addr(sh.kq), tb = kq, pb = kq + 16384;
+    const uint32_t kq = smem_addr(sh.kq), tb = kq, pb = kq + 24576;
     const int p = threadIdx.x, w = p / 32, lane = p % 32, i = p % C;
     const int hk = blockIdx.x % a.heads_k;
     const int64_t image = blockIdx.x / a.heads_k;
@@ -278,9 +284,13 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
     if (p == 0) {
         tc_fence_after();
         const uint64_t d = operand(kq, 16, 1024, kSwizzle128);
-        mma_steps<4, 2, 2>(D0, d, d, mma_desc(64, false, false), false);
-        mma_steps<4, 2, 2>(D0, d + 1024, d + 1024, mma_desc(64, false, false), true);
         if constexpr (kLo) {
+            // lo lo, then hi lo and lo hi, over the halves of dk
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const uint64_t lo = d + half * 1024 + 2048;
+                mma_steps<4, 2, 2>(D0, lo, lo, mma_desc(64, false, false), half > 0);
+            }
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const uint64_t hi = d + half * 1024, lo = hi + 2048;
@@ -288,6 +298,8 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
                 mma_steps<4, 2, 2>(D0, lo, hi, mma_desc(64, false, false), true);
             }
         }
+        mma_steps<4, 2, 2>(D0, d, d, mma_desc(64, false, false), kLo);
+        mma_steps<4, 2, 2>(D0, d + 1024, d + 1024, mma_desc(64, false, false), true);
         mma_commit(smem_addr(&sh.mma));
     }
     // Norm of row p of [K;Q].
@@ -318,7 +330,7 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
 #pragma unroll
         for (int u = 4; u < 8; ++u) {
 #pragma unroll
-            for (int m = 0; m < 4; ++m) sts16(kq + m * 8192 + swz<128>(p, u), 0, 0, 0, 0);
+            for (int m = 0; m < 6; ++m) sts16(kq + m * 8192 + swz<128>(p, u), 0, 0, 0, 0);
         }
     }
     __syncthreads();
@@ -337,12 +349,12 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
             tmem_ld16(DG + lanes + o, x);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                uint32_t hi[4], lo[4];
+                uint32_t g[3][4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) split2(x[4 * u + e], hi[e], lo[e]);
+                for (int e = 0; e < 4; ++e) split3(x[4 * u + e], g[0][e], g[1][e], g[2][e]);
                 const uint32_t at = swz<128>(p, o / 8 + u);
-                st16(out->tg[0] + at, make_uint4(hi[0], hi[1], hi[2], hi[3]));
-                st16(out->tg[1] + at, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+#pragma unroll
+                for (int m = 0; m < 3; ++m) st16(out->tg[m] + at, make_uint4(g[m][0], g[m][1], g[m][2], g[m][3]));
             }
         }
         tc_fence_before();
@@ -420,7 +432,7 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         const uint32_t at = pb + swz<128>(i, 4 * hf + o / 8 + u);
-                        store_split8(at, at + 8192, x + 4 * u);
+                        store_split8(at, 8192, x + 4 * u);
                     }
                 }
             }
@@ -464,11 +476,12 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
                 const float2 bt = make_float2(-ga.beta[col], -ga.beta[col + 1]);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    uint32_t hi, lo;
-                    split2(__fmul2_rn(make_float2(d[n][2 * e], d[n][2 * e + 1]), bt), hi, lo);
+                    uint32_t x[3];
+                    split3(__fmul2_rn(make_float2(d[n][2 * e], d[n][2 * e + 1]), bt), x[0], x[1], x[2]);
                     const uint32_t at = tb + swz<128>(32 + fr + 8 * e, col / 8) + col % 8 * 2;
-                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(hi) : "memory");
-                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + 8192), "r"(lo) : "memory");
+#pragma unroll
+                    for (int m = 0; m < 3; ++m)
+                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + m * 8192), "r"(x[m]) : "memory");
                 }
             }
             // The diagonal blocks: row p / 2, half of its 32 columns.
@@ -483,7 +496,7 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
                     f[e] = __fmul2_rn(*reinterpret_cast<const float2*>(from + 2 * e),
                                       *reinterpret_cast<const float2*>(bt + 2 * e));
                 const uint32_t at = tb + swz<128>(r, r / 32 * 4 + o / 8 + u);
-                store_split8(at, at + 8192, f);
+                store_split8(at, 8192, f);
             }
         }
         fence_async_smem();
@@ -492,15 +505,18 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
         if (p == 96) {
             // A thread of the warps that wait for this product next.
             tc_fence_after();
-            // G = P T in rows 64..: hi hi, hi lo, lo hi. The 8 KB before either part of P are other
-            // parts of T or P; the rows 0..63 they make are of no use.
+            // G = P T in rows 64.., by parts. The 8 KB before a part of P are other parts of T or P; the
+            // rows 0..63 they make are of no use.
             const uint64_t P = operand(pb - 8192, 16, 1024, kSwizzle128), T = operand(tb, 16384, 1024, kSwizzle128);
-            mma_steps<4, 2, 128>(DG, P, T, mma_desc(64, false, true), false);
-            mma_steps<4, 2, 128>(DG, P, T + 512, mma_desc(64, false, true), true);
-            mma_steps<4, 2, 128>(DG, P + 512, T, mma_desc(64, false, true), true);
+#pragma unroll
+            for (int sum = 2; sum >= 0; --sum)
+#pragma unroll
+                for (int m = 0; m <= sum; ++m)
+                    mma_steps<4, 2, 128>(DG, P + m * 512, T + (sum - m) * 512, mma_desc(64, false, true),
+                                         sum < 2 || m > 0);
             mma_commit(smem_addr(&sh.mma));
 #pragma unroll
-            for (int part = 0; part < 2; ++part)
+            for (int part = 0; part < 3; ++part)
                 asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], 8192;" ::"l"(
                                  out->tg[part]), "r"(tb + part * 8192)
                              : "memory");

@@ -3,21 +3,21 @@
 // The mathematics, the images of the prep kernel, the precision and the loop are those of
 // gdr_chunk.cu, transposed: state columns lie along M, so
 //     [K;Q] S  is  S^T [K;Q]^T,    [T;G] R  is  R^T [T;G]^T,    K^T u  is  u^T K.
-// The operands that the CTA makes (S, R, u, in two bf16 parts) are then the A of their products,
+// The operands that the CTA makes (S, R, u, in three bf16 parts) are then the A of their products,
 // which the tensor core reads from tensor memory: shared memory holds copies only, and every warp
 // has a share of every row (with the rows of K and Q along M, the warps of two of the SM's four
 // partitions made all of R and u). The state stays in registers, fp32. R, u and the outputs use
 // the matrix fragment shapes of tensor memory, so that V comes in and outputs go out by transposes of
 // 8 x 8 matrices instead of 2-byte accesses.
 //
-// Bound. A chunk takes 5400 cycles (6800 in the form of gdr_chunk.cu): products 3100 of them
-// (36 steps of 76 cycles, and their latency), splitting S, R and u 1000, 450 and 450, outputs 250,
-// the rest waits. 40807 tokens x 48 heads: 687 us against 845, a seventh of it the starts and ends of
-// chains. Measured on the way: products issued by a worker (58 cycles a step, which it waits for)
-// 812 us; by a warp of their own, 739; outputs read before the last product is issued, since a
-// TMEM load that starts beside a product waits for its end, 708; fragments instead of a row to a
-// thread for V and the outputs, 691. Slower: those reads in flight across the arrival (772), the
-// state's update and split interleaved in two halves (726).
+// Bound. The products, 60 steps of some 76 cycles and their latency, take two thirds of a chunk; the
+// rest is splitting S, R and u, outputs and waits. 40807 tokens x 48 heads: 937 us. Measured on the way
+// with operands in two parts (36 steps): the form of gdr_chunk.cu 845 us; products issued by a worker
+// (58 cycles a step, which it waits for) 812; by a warp of their own, 739; outputs read before the last
+// product is issued, since a TMEM load that starts beside a product waits for its end, 708; fragments
+// instead of a row to a thread for V and the outputs, 691; rows of the state by thread, 687. Slower:
+// those reads in flight across the arrival (772), the state's update and split interleaved in two
+// halves (726).
 #include "gdr_chunk.cuh"
 
 namespace cc1d {
@@ -29,22 +29,25 @@ constexpr int kWorkers = 512, kThreads = kWorkers + 64;  // a warp each issues p
 template <bool kLo>
 struct Layout {
     static constexpr int kKQ = Parts<kLo>::kBytes;
-    static constexpr int kStages = kLo ? 2 : 3;
+    static constexpr int kStages = 2;                      // of K, Q and the row factors
+    static constexpr int kTgStages = kLo ? 1 : 2;          // of T and G
     static constexpr int KQ = 0;                           // stages x K and Q
-    static constexpr int TG = KQ + kStages * kKQ;          // stages x [hi, lo][T, G rows][128 B]
-    static constexpr int V = TG + kStages * 32768;         // [2 halves of 64 columns][64 rows][128 B]
+    static constexpr int TG = KQ + kStages * kKQ;          // stages x [3 parts][T, G rows][128 B]
+    static constexpr int V = TG + kTgStages * kTgBytes;    // [2 halves of 64 columns][64 rows][128 B]
     static constexpr int O = V + C * VS * 2;               // 512 bytes a warp: outputs on their way out
     static constexpr int VEC = O + kWorkers / 32 * 512;    // stages x row factors
     static constexpr int END = VEC + kStages * kVectorBytes;
 };
 
-// Tensor memory columns. An operand's two parts lie one behind the other, two values to a column.
+// Tensor memory columns. An operand's three parts lie one behind the other, two values to a column.
 enum : uint32_t {
-    kSP = 0,           // S, hi and lo (64 columns each)
-    kRP = 0, kUP = 64, // R and u in its place (32 each part)
-    kDK = 128,         // S^T [K;Q]^T
-    kDT = 256,         // R^T [T;G]^T
-    kDS = 384,         // u^T K
+    kSP = 0,           // S (64 columns each part)
+    kRP = 0, kUP = 96, // R and u in its place (32 each part)
+    kDK = 192,         // S^T [K;Q]^T
+    kDT = 320,         // R^T [T;G]^T
+    kDS = kDT,         // u^T K: all of kDT has been read by then
+    // All of it: a prep CTA could not start beside this one, and this one waits for the prep kernel. Their
+    // shared memory (above 180 KB and above 70 KB) keeps them from meeting on an SM.
     kColumns = 512
 };
 
@@ -52,7 +55,7 @@ enum : uint32_t {
 enum { kHaveS = 1, kHaveR, kHaveU };
 
 struct Shared {
-    uint64_t full[3], v_full, mma;
+    uint64_t full[2], tg_full[2], v_full, mma;
     uint32_t tmem;
     int abort;
     int row;  // sequence of this CTA
@@ -135,7 +138,7 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
                 const __grid_constant__ CUtensorMap mapk, const __grid_constant__ CUtensorMap mapv, int tiles) {
     constexpr bool kLo = std::is_same<T, f16>::value;  // fp16 keys and queries come in two bf16 parts
     using Lay = Layout<kLo>;
-    constexpr int kStages = Lay::kStages;
+    constexpr int kStages = Lay::kStages, kTgStages = Lay::kTgStages;
     extern __shared__ __align__(1024) unsigned char raw[];
     __shared__ Shared sh;
     const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
@@ -157,7 +160,10 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
         static_cast<const ChunkImage*>(a.workspace) + chunk_base(tok0, row) * a.heads_v + h;
 
     if (tid == 0) {
-        for (int i = 0; i < 3; ++i) mbar_init(smem_addr(&sh.full[i]), 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_addr(&sh.full[i]), 1);
+            mbar_init(smem_addr(&sh.tg_full[i]), 1);
+        }
         mbar_init(smem_addr(&sh.v_full), 1);
         mbar_init(smem_addr(&sh.mma), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -179,32 +185,43 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
         // Products, one thread.
         uint32_t st_phase = 0;
         for (int c = 0, st = 0; c < chunks; ++c) {
-            const uint32_t kq = base + Lay::KQ + st * Lay::kKQ, tg = base + Lay::TG + st * 32768;
+            const uint32_t kq = base + Lay::KQ + st * Lay::kKQ, tg = base + Lay::TG + c % kTgStages * kTgBytes;
             const uint32_t mma = smem_addr(&sh.mma);
             mbar_wait(smem_addr(&sh.full[st]), st_phase, &sh.abort);
             named_sync(kHaveS, kThreads);
             if (lane == 0) {
                 tc_fence_after();
-                // S^T [K;Q]^T, over the halves of dk
+                // S^T [K;Q]^T, over the halves of dk. Here as below the smallest products come first: a
+                // sum is cut to fp32 after every step.
+                if constexpr (kLo)
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const uint64_t k = operand(kq + half * 16384, 16, 1024, kSwizzle128);
-                    const uint32_t s = tmem + kSP + half * 32;
-                    mma_steps_ts<4, 2>(tmem + kDK, s, k, mma_desc(128, false, false), half > 0);
-                    mma_steps_ts<4, 2>(tmem + kDK, s + 64, k, mma_desc(128, false, false), true);
-                    if constexpr (kLo)
-                        mma_steps_ts<4, 2>(tmem + kDK, s, k + 2048, mma_desc(128, false, false), true);
-                }
+                    for (int m = 1; m >= 0; --m)
+#pragma unroll
+                        for (int half = 0; half < 2; ++half)
+                            mma_steps_ts<4, 2>(tmem + kDK, tmem + kSP + 64 * m + 32 * half,
+                                               operand(kq + 32768 + half * 16384, 16, 1024, kSwizzle128),
+                                               mma_desc(128, false, false), m == 0 || half > 0);
+#pragma unroll
+                for (int m = 2; m >= 0; --m)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half)
+                        mma_steps_ts<4, 2>(tmem + kDK, tmem + kSP + 64 * m + 32 * half,
+                                           operand(kq + half * 16384, 16, 1024, kSwizzle128),
+                                           mma_desc(128, false, false), kLo || m < 2 || half > 0);
                 mma_commit(mma);
             }
+            mbar_wait(smem_addr(&sh.tg_full[c % kTgStages]), c / kTgStages & 1, &sh.abort);
             named_sync(kHaveR, kThreads);
             if (lane == 0) {
                 tc_fence_after();
-                // R^T [T;G]^T: hi hi, hi lo, lo hi
+                // R^T [T;G]^T, by parts of both
                 const uint64_t g = operand(tg, 16, 1024, kSwizzle128);
-                mma_steps_ts<4, 2>(tmem + kDT, tmem + kRP, g, mma_desc(128, false, false), false);
-                mma_steps_ts<4, 2>(tmem + kDT, tmem + kRP, g + 1024, mma_desc(128, false, false), true);
-                mma_steps_ts<4, 2>(tmem + kDT, tmem + kRP + 32, g, mma_desc(128, false, false), true);
+#pragma unroll
+                for (int sum = 2; sum >= 0; --sum)
+#pragma unroll
+                    for (int m = 0; m <= sum; ++m)
+                        mma_steps_ts<4, 2>(tmem + kDT, tmem + kRP + 32 * m, g + 1024 * (sum - m),
+                                           mma_desc(128, false, false), sum < 2 || m > 0);
                 mma_commit(mma);
             }
             named_sync(kHaveU, kThreads);
@@ -212,10 +229,14 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
                 tc_fence_after();
                 // u^T K
                 const uint64_t k = operand(kq, 16384, 1024, kSwizzle128);
-                mma_steps_ts<4, 128>(tmem + kDS, tmem + kUP, k, mma_desc(128, false, true), false);
-                mma_steps_ts<4, 128>(tmem + kDS, tmem + kUP + 32, k, mma_desc(128, false, true), true);
                 if constexpr (kLo)
-                    mma_steps_ts<4, 128>(tmem + kDS, tmem + kUP, k + 2048, mma_desc(128, false, true), true);
+#pragma unroll
+                    for (int m = 1; m >= 0; --m)
+                        mma_steps_ts<4, 128>(tmem + kDS, tmem + kUP + 32 * m, k + 2048, mma_desc(128, false, true),
+                                             m == 0);
+#pragma unroll
+                for (int m = 2; m >= 0; --m)
+                    mma_steps_ts<4, 128>(tmem + kDS, tmem + kUP + 32 * m, k, mma_desc(128, false, true), kLo || m < 2);
                 mma_commit(mma);
             }
             if (++st == kStages) {
@@ -224,15 +245,20 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
             }
         }
     } else if (warp > kWorkers / 32) {
-        // Copies, one thread: K, Q, T, G and the row factors of chunk c into stage st, which must
-        // be free, and V of chunk c.
+        // Copies, one thread: K, Q and the row factors of chunk c into stage st, which must be free;
+        // T and G, into the stage of their own; V.
         auto load = [&](int c, int st) {
             const uint32_t full = smem_addr(&sh.full[st]);
             const ChunkImage* from = image + (int64_t)c * a.heads_v;
-            mbar_expect(full, Lay::kKQ + 32768 + kVectorBytes);
+            mbar_expect(full, Lay::kKQ + kVectorBytes);
             load_kq<kLo>(base + Lay::KQ + st * Lay::kKQ, &mapk, &mapq, hk, (int)tok0 + c * C, full);
             bulk_load(base + Lay::VEC + st * kVectorBytes, from->in, kVectorBytes, full);
-            bulk_load(base + Lay::TG + st * 32768, from->tg, 32768, full);
+        };
+        auto load_tg = [&](int c) {
+            const int st = c % kTgStages;
+            const uint32_t full = smem_addr(&sh.tg_full[st]);
+            mbar_expect(full, kTgBytes);
+            bulk_load(base + Lay::TG + st * kTgBytes, image[(int64_t)c * a.heads_v].tg, kTgBytes, full);
         };
         auto load_v = [&](int c) {
             const uint32_t full = smem_addr(&sh.v_full);
@@ -243,6 +269,7 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
         grid_dependency_wait();  // for the prep kernel's images
         if (lane == 0) {
             for (int c = 0; c < kStages && c < chunks; ++c) load(c, c);
+            for (int c = 0; c < kTgStages && c < chunks; ++c) load_tg(c);
             load_v(0);
         }
         for (int c = 0, st = 0; c < chunks; ++c) {
@@ -253,7 +280,9 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
             // They have read V.
             named_sync(kHaveR, kThreads);
             if (lane == 0 && c + 1 < chunks) load_v(c + 1);
+            // They have the product of T and G.
             named_sync(kHaveU, kThreads);
+            if (lane == 0 && c + kTgStages < chunks) load_tg(c + kTgStages);
             if (++st == kStages) st = 0;
         }
     } else {
@@ -292,11 +321,11 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
             // The state as an operand.
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
-                uint32_t hi[8], lo[8];
+                uint32_t x[3][8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) split2(s[8 * g + k], hi[k], lo[k]);
-                tmem_st8(mine + kSP + 16 * part + 8 * g, hi);
-                tmem_st8(mine + kSP + 64 + 16 * part + 8 * g, lo);
+                for (int k = 0; k < 8; ++k) split3(s[8 * g + k], x[0][k], x[1][k], x[2][k]);
+#pragma unroll
+                for (int m = 0; m < 3; ++m) tmem_st8(mine + kSP + 64 * m + 16 * part + 8 * g, x[m]);
             }
             if (left < C) {
                 // The copies of K went on into the next sequence: zeros there, whatever it holds
@@ -323,7 +352,7 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
                 tmem_ld_frag(mine + kDK + 16 * part, d);
                 tmem_wait_ld();
                 tmem_ready(d);
-                uint32_t hi[8], lo[8];
+                uint32_t x[3][8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
                     d[k] = add_pair<T>(vv[k], __fmul2_rn(d[k], make_float2(-f[k >> 1 & 1].x, -f[k >> 1 & 1].y)));
@@ -337,9 +366,9 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
                     }
                 }
 #pragma unroll
-                for (int k = 0; k < 8; ++k) split2(d[k], hi[k], lo[k]);
-                tmem_st_frag(mine + kRP + 8 * part, hi);
-                tmem_st_frag(mine + kRP + 32 + 8 * part, lo);
+                for (int k = 0; k < 8; ++k) split3(d[k], x[0][k], x[1][k], x[2][k]);
+#pragma unroll
+                for (int m = 0; m < 3; ++m) tmem_st_frag(mine + kRP + 32 * m + 8 * part, x[m]);
             }
             arrive(kHaveR);
             uint32_t o[8];
@@ -355,11 +384,11 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
                 tmem_ld_frag(mine + kDT + 16 * part, d);
                 tmem_wait_ld();
                 tmem_ready(d);
-                uint32_t hi[8], lo[8];
+                uint32_t x[3][8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) split2(__fmul2_rn(d[k], f[k >> 1 & 1]), hi[k], lo[k]);
-                tmem_st_frag(mine + kUP + 8 * part, hi);
-                tmem_st_frag(mine + kUP + 32 + 8 * part, lo);
+                for (int k = 0; k < 8; ++k) split3(__fmul2_rn(d[k], f[k >> 1 & 1]), x[0][k], x[1][k], x[2][k]);
+#pragma unroll
+                for (int m = 0; m < 3; ++m) tmem_st_frag(mine + kUP + 32 * m + 8 * part, x[m]);
                 // Outputs: read here, because a load that runs beside a product waits for its end.
                 float2 q[8];
                 tmem_ld_frag(mine + kDK + C + 16 * part, q);

@@ -212,14 +212,12 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
         : "memory");
 }
 
-// ------------------------------------------------------------------------------- two-part bf16
+// ----------------------------------------------------------------------------- three-part bf16
 
-// Two values as bf16 pairs: hi rounds to nearest, lo rounds the rest, so that hi + lo is within
-// 2^-17 of the value. The low halves hold f.x. The rest is x - hi as one mixed-precision FMA (the
-// shift and mask that widen hi would be two more instructions on the half-rate integer pipe, which
-// bounds this: 7.6 cycles a warp, 5.2 like this).
-__device__ __forceinline__ void split2(float2 f, uint32_t& hi, uint32_t& lo) {
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(f.y), "f"(f.x));
+// x minus the bf16 pair h, exactly: the products with -1 are exact and so is the difference, as h is
+// within an ulp of x. One mixed-precision FMA each (the shift and mask that widen a half would be
+// two more instructions on the half-rate integer pipe).
+__device__ __forceinline__ float2 rest2(float2 x, uint32_t h) {
     float2 r;
     asm("{\n\t.reg .b16 l, h, m;\n\t"
         "mov.b32 {l, h}, %2;\n\t"
@@ -227,8 +225,26 @@ __device__ __forceinline__ void split2(float2 f, uint32_t& hi, uint32_t& lo) {
         "fma.rn.f32.bf16 %0, l, m, %3;\n\t"
         "fma.rn.f32.bf16 %1, h, m, %4;\n\t}"
         : "=f"(r.x), "=f"(r.y)
-        : "r"(hi), "f"(f.x), "f"(f.y));
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(r.y), "f"(r.x));
+        : "r"(h), "f"(x.x), "f"(x.y));
+    return r;
+}
+__device__ __forceinline__ uint32_t bf16x2(float2 f) {
+    uint32_t v;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(f.y), "f"(f.x));
+    return v;
+}
+// Two values as two bf16 pairs, within 2^-17 of them: exact for fp16 values (11 bits).
+__device__ __forceinline__ void split2(float2 f, uint32_t& hi, uint32_t& lo) {
+    hi = bf16x2(f);
+    lo = bf16x2(rest2(f, hi));
+}
+// Two values as three bf16 pairs, whose sum holds the 24 bits of fp32: 8 bits and a sign each.
+// The low halves hold f.x.
+__device__ __forceinline__ void split3(float2 f, uint32_t& p0, uint32_t& p1, uint32_t& p2) {
+    p0 = bf16x2(f);
+    f = rest2(f, p0);
+    p1 = bf16x2(f);
+    p2 = bf16x2(rest2(f, p1));
 }
 // A pair of T (bf16 or fp16) plus two fp32 values.
 template <typename T>

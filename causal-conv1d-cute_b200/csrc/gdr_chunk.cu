@@ -412,19 +412,22 @@ cudaError_t go(const cc1d_gdr_args& a, const CUtensorMap& q, const CUtensorMap& 
 template <typename T, typename ST>
 cudaError_t pick(const cc1d_gdr_args& a, const CUtensorMap& q, const CUtensorMap& k, cudaStream_t stream) {
     const bool out32 = host_aligned32(a.out) && a.o_st % 16 == 0 && a.o_sh % 16 == 0;
-    // Columns per CTA. A chunk's step takes 1.6, 2.2 and 2.8 us with 32, 64 and 128 columns: wide
-    // tiles do more per SM, narrow ones finish a chain sooner. Many heads take the widest (bf16,
-    // uneven lengths, us with 32, 64, 128: 768 heads, 16384 tokens 800, 599, 458; 336 heads 235,
-    // 178, 160; 288 heads 226, 174, 172; 240 heads 221, 169, 196), few that leave SMs free the
-    // narrowest (12 heads, 4096 tokens 126, 162, 200; 48 heads in four sequences 104, 131, 162, in
-    // one 263, 198, 237). fp16 has no tile of 64, which would load twice the keys for no more than
-    // the narrow one's speed (768 heads 1014, 974, 639; 144 heads 552, 550, 508; 72 heads 184, 302,
-    // 282).
+    // Columns per CTA. A chunk's step takes 2.1, 2.9 and 3.7 us with 32, 64 and 128 columns: wide
+    // tiles do more per SM, narrow ones finish a chain sooner. Many heads (sequences x heads) take the
+    // widest (bf16, uneven lengths, us with 32, 64, 128 columns: 768 heads, 16384 tokens 1006, 826, 641;
+    // 336 heads 290, 236, 224; 288 heads 281, 232, 240; 240 heads 274, 226, 274), few the narrowest
+    // (144 heads 262, 286, 352 in 12 sequences, 260, 298, 367 in six of 8192 tokens; 96 heads 272, 372,
+    // 465; 48 heads, 4096 tokens 131, 179, 227), the more so as long as the CTAs of the longest sequences
+    // find an SM of their own. With fewer than four sequences all CTAs are long ones, and a second wave
+    // costs a whole chain (48 heads in one sequence 332, 273, 333; 12 heads 160, 220, 281). fp16 has no
+    // tile of 64, which would load twice the keys for no more than the narrow one's speed (us with 32,
+    // 128: 768 heads 1273, 853; 240 heads 340, 347 and in five sequences 1194, 1099; 192 heads 330, 380;
+    // 144 heads 328, 442).
     constexpr bool kF16 = std::is_same<T, f16>::value;
     const int64_t heads = a.rows * a.heads_v;
-    if (a.dv % 128 == 0 && heads * (a.dv / 128) >= (kF16 ? 148 : 296)) return launch_gdr_wide(a, q, k, stream);
+    if (a.dv % 128 == 0 && heads * (a.dv / 128) >= (kF16 ? 222 : 296)) return launch_gdr_wide(a, q, k, stream);
     if constexpr (!kF16) {
-        if (a.dv % 64 == 0 && heads * (a.dv / 32) > (a.rows >= 4 ? 296 : 148))
+        if (a.dv % 64 == 0 && heads * (a.dv / 32) > (a.rows >= 4 ? 592 : 148))
             return go<T, ST, 64>(a, q, k, out32, stream);
     }
     return go<T, ST, 32>(a, q, k, out32, stream);

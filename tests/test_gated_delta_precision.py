@@ -41,7 +41,7 @@ def states_case(lengths, hk, hv, dtype, dv=128, raw=True, seed=0, change=None, t
 @pytest.mark.parametrize("dtype", [BF, F16])
 @pytest.mark.parametrize("lengths,hk,hv,dv", [
     ([700], 1, 3, 128),  # few heads: tiles of 32 columns
-    ([130, 64, 65, 200], 4, 24, 128),  # more: 64 (bf16)
+    ([130, 64, 65, 200], 20, 40, 128),  # more: 64 (bf16)
     ([65, 130, 64, 90, 20, 97, 10, 33], 20, 40, 128),  # many: 128
     ([129, 77, 300], 1, 2, 256),
 ])

@@ -41,6 +41,7 @@ SIGNATURES = {
     "cc1d_update_unpack": [_p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _i32,
                            _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _p],
     "cc1d_gdr_workspace": [_p, _p],
+    "cc1d_set_wait_limit": [_i64],
     "cc1d_gdr_update": [_p, _p],
     "cc1d_gdr_varlen": [_p, _p],
     "cc1d_rms_norm_gated": [_p, _p],
@@ -53,8 +54,9 @@ SIGNATURES = {
 # host less than setting the fields of a ctypes structure: pointers, then int64, int32 and float.
 GDR_ARGS = struct.Struct("16P34q13if")
 NORM_ARGS = struct.Struct("4P9q2if4x")
-# The workspace's fields in the first: the last pointer and the last int64.
-GDR_WORKSPACE, GDR_WORKSPACE_AT = struct.Struct("P"), 15 * 8
+# What a call with a workspace sets in the first: the last two pointers (status word, workspace) and
+# the last int64 (its size).
+GDR_WORKSPACE, GDR_WORKSPACE_AT = struct.Struct("2P"), 14 * 8
 GDR_WORKSPACE_BYTES, GDR_WORKSPACE_BYTES_AT = struct.Struct("q"), (16 + 33) * 8
 
 EXPORTS = ("cc1d_abi_version", "cc1d_status_string", "cc1d_last_error", *SIGNATURES)

@@ -11,7 +11,9 @@ layout it is given.
 Device status. When checks are enabled (set_device_checks(True)), every call passes a per-device
 int32 status word that kernels OR a bit into when they skip an index outside the caches (a slot
 outside the state cache, sequence bounds outside the packed tokens). device_status() reads and
-clears it. Checks are off by default so that no call allocates anything.
+clears it. Checks are off by default so that no call allocates anything. The chunked delta rule, which
+allocates a workspace anyway, always has the word: it also says there if a wait of its kernels ran out
+(the first such call on a device has to come before a CUDA graph capture to have one).
 """
 
 import ctypes
@@ -43,8 +45,8 @@ def device_status(device=None, clear=True):
     return v
 
 
-def _status_ptr(device):
-    if not _checks:
+def _status_ptr(device, always=False):
+    if not (_checks or always):
         return None
     t = _status.get(device.index)
     if t is None:
@@ -262,9 +264,11 @@ def _gdr_args(q, k, v, g, beta, a_log, dt_bias, out, states, inter, idx, iidx, q
 
 
 def _with_workspace(args, workspace):
-    """The same argument block with a workspace tensor."""
+    """The same argument block with a workspace tensor, and the status word whatever _checks is: the
+    kernels that use a workspace wait for their own copies, and say there if such a wait ran out."""
     block = bytearray(args)
-    _lib.GDR_WORKSPACE.pack_into(block, _lib.GDR_WORKSPACE_AT, workspace.data_ptr())
+    status = _status_ptr(workspace.device, always=True) or 0
+    _lib.GDR_WORKSPACE.pack_into(block, _lib.GDR_WORKSPACE_AT, status, workspace.data_ptr())
     _lib.GDR_WORKSPACE_BYTES.pack_into(block, _lib.GDR_WORKSPACE_BYTES_AT, workspace.numel())
     return bytes(block)
 

@@ -127,6 +127,10 @@ def gated_delta_rule_varlen_fn(
     value head for each of tokens / 64 + batch chunks, and 1024 bytes per token and key head more for
     fp16 (in groups of heads from 4 GiB on). Other calls run token by token.
 
+    The chunked kernels wait for copies of their own. Should such a wait ever take above two seconds,
+    the outputs that depend on it are NaN, the slot keeps its state, and device_status() says so
+    (_lib.DEV_TIMEOUT).
+
     Returns:
         (total_tokens, heads_v, dv) output.
     """

@@ -4,12 +4,15 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "kernels.h"
 
 namespace {
 
 thread_local char g_last_error[512] = "";
+std::atomic<int64_t> g_wait_limit_ns{2000000000};
 
 cc1d_status_t fail(cc1d_status_t code, const char* fmt, ...) {
     va_list ap;
@@ -103,6 +106,8 @@ bool overlap(const void* p, int64_t np, const void* q, int64_t nq) {
 }
 
 }  // namespace
+
+int64_t cc1d::wait_limit_ns() { return g_wait_limit_ns.load(std::memory_order_relaxed); }
 
 extern "C" {
 
@@ -350,6 +355,12 @@ cc1d_status_t cc1d_update_unpack(const void* qkvz, int64_t q_sb, const void* ba,
     if (cc1d_status_t s = bind_stream(stream)) return s;
     return from_cuda(cc1d::launch_unpack(args, width, dtype, (cudaStream_t)stream),
                      "cc1d_update_unpack");
+}
+
+cc1d_status_t cc1d_set_wait_limit(int64_t ns) {
+    if (ns < 0) return fail(CC1D_ERR_INVALID, "a limit of %lld ns", (long long)ns);
+    g_wait_limit_ns.store(ns, std::memory_order_relaxed);
+    return ok();
 }
 
 cc1d_status_t cc1d_gdr_workspace(const cc1d_gdr_args* args, int64_t* bytes) {

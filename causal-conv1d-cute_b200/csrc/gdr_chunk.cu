@@ -66,9 +66,10 @@ struct Layout {
 constexpr int kThreads = 256;
 
 struct Shared {
-    uint64_t full[2], tg_full[2], v_full, mma;
+    uint64_t full[2], tg_full[2], v_full, mma, last;
+    int begun[5];  // copies begun on the first five of these
     uint32_t tmem;
-    int abort;
+    int abort, late;
     int row;  // sequence of this CTA
 };
 
@@ -98,7 +99,7 @@ template <typename T, typename ST, int VS>
 __global__ void __launch_bounds__(kThreads, 1)
 gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__ CUtensorMap mapq,
                  const __grid_constant__ CUtensorMap mapk, const __grid_constant__ CUtensorMap mapv,
-                 int tiles, bool out32) {
+                 int tiles, bool out32, int64_t wait_ns) {
     constexpr bool kLo = std::is_same<T, f16>::value;  // fp16 keys and queries come in two bf16 parts
     using Lay = Layout<VS, kLo>;
     constexpr uint64_t kSwz = VS == 64 ? kSwizzle128 : kSwizzle64;
@@ -131,8 +132,10 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
         }
         mbar_init(smem_addr(&sh.v_full), 1);
         mbar_init(smem_addr(&sh.mma), 1);
+        mbar_init(smem_addr(&sh.last), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        sh.abort = 0;
+        for (int i = 0; i < 5; ++i) sh.begun[i] = 0;
+        sh.abort = sh.late = 0;
     }
     if (warp == 0) {
         tmem_alloc(smem_addr(&sh.tmem), Lay::kTmem);
@@ -146,8 +149,12 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
     const uint32_t tmem = sh.tmem;
     const uint32_t lanes = (uint32_t)w << 21;  // the warp's first TMEM lane, in bits 16..
 
+    // Copies may be started: those of earlier chunks have been waited for.
+    auto live = [&] { return *(volatile int*)&sh.abort == 0 && wait_ns > 0; };
     // K, Q and the row factors of chunk c into stage st, which must be free; one thread.
     auto load = [&](int c, int st) {
+        if (!live()) return;
+        sh.begun[st] = c / kStages + 1;
         const uint32_t full = smem_addr(&sh.full[st]);
         const ChunkImage* from = image + (int64_t)c * a.heads_v;
         mbar_expect(full, Lay::kKQ + kVectorBytes);
@@ -156,13 +163,17 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
     };
     // T and G of chunk c, into the stage of their own.
     auto load_tg = [&](int c) {
+        if (!live()) return;
         const int st = c % kTgStages;
+        sh.begun[2 + st] = c / kTgStages + 1;
         const uint32_t full = smem_addr(&sh.tg_full[st]);
         mbar_expect(full, kTgBytes);
         bulk_load(base + Lay::TG + st * kTgBytes, image[(int64_t)c * a.heads_v].tg, kTgBytes, full);
     };
     // V of chunk c.
     auto load_v = [&](int c) {
+        if (!live()) return;
+        sh.begun[4] = c + 1;
         const uint32_t full = smem_addr(&sh.v_full);
         mbar_expect(full, C * VS * 2);
         tma_load(base + Lay::V, &mapv, vt * VS, h, (int)tok0 + c * C, full);
@@ -204,7 +215,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
     int st = 0;
     uint32_t phase = 0, st_phase = 0;
     float decay = 1.f;
-    mbar_wait(smem_addr(&sh.full[0]), 0, &sh.abort);
+    mbar_wait(smem_addr(&sh.full[0]), 0, &sh.abort, wait_ns);
 #pragma unroll 1
     for (int c = 0;; ++c) {
         // The state after the chunk before, and as an operand if there is another.
@@ -256,9 +267,10 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
         if (tid == 64 && c > 0 && c - 1 + kStages < chunks) load(c - 1 + kStages, st > 0 ? st - 1 : kStages - 1);
         const float in = vec[st].in[p], out = vec[st].out[p % C];
         decay = vec[st].decay;
+        if (tid == 96 && vec[st].failed) *(volatile int*)&sh.abort = 1;
         float2 q[W / 2];  // rows of Q: their outputs
-        if (p < C) mbar_wait(smem_addr(&sh.v_full), c & 1, &sh.abort);
-        mbar_wait(mma, phase, &sh.abort);
+        if (p < C) mbar_wait(smem_addr(&sh.v_full), c & 1, &sh.abort, wait_ns);
+        mbar_wait(mma, phase, &sh.abort, wait_ns);
         phase ^= 1;
         tc_fence_after();
         if (p < C) {
@@ -292,8 +304,8 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
         }
         tc_fence_before();
         __syncthreads();
+        if (lead) mbar_wait(smem_addr(&sh.tg_full[c % kTgStages]), c / kTgStages & 1, &sh.abort, wait_ns);
         if (lead) {
-            mbar_wait(smem_addr(&sh.tg_full[c % kTgStages]), c / kTgStages & 1, &sh.abort);
             tc_fence_after();
             // [T;G] R, part by part of [T;G]
             const uint64_t r = operand(rb, Lay::kR, kGroup, kSwz), g = operand(tg, 16, 1024, kSwizzle128);
@@ -303,7 +315,7 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
             mma_commit(mma);
             if (c + 1 < chunks) load_v(c + 1);
         }
-        mbar_wait(mma, phase, &sh.abort);
+        mbar_wait(mma, phase, &sh.abort, wait_ns);
         phase ^= 1;
         tc_fence_after();
 #pragma unroll
@@ -353,22 +365,35 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
             st_phase ^= 1;
         }
         // The next chunk's K, Q, T, G: there by now, and the look costs less here.
-        if (c + 1 < chunks) mbar_wait(smem_addr(&sh.full[st]), st_phase, &sh.abort);
-        mbar_wait(mma, phase, &sh.abort);
+        if (c + 1 < chunks) mbar_wait(smem_addr(&sh.full[st]), st_phase, &sh.abort, wait_ns);
+        mbar_wait(mma, phase, &sh.abort, wait_ns);
         phase ^= 1;
         tc_fence_after();
     }
-    if (sp != nullptr) {
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (sh.abort) {
+        // The cache keeps its state, and the outputs say that they are none.
+        if (tid == 0) {
+            mma_commit(smem_addr(&sh.last));
+            mbar_wait(smem_addr(&sh.last), 0, &sh.late, kDrainNs);
+            for (int i = 0; i < 5; ++i)
+                if (sh.begun[i] > 0)
+                    mbar_wait(smem_addr(sh.full) + 8 * i, (sh.begun[i] - 1) & 1, &sh.late, kDrainNs);
+            flag_status(a.dev_status, CC1D_DEV_TIMEOUT);
+        }
+        __syncthreads();
+        for (int64_t t = p - C; p >= C && t < ntok; t += C)
+#pragma unroll
+            for (int k = 0; k < W; k += 8) st16(op + t * a.o_st + k, nan16());
+    } else if (sp != nullptr) {
 #pragma unroll
         for (int g = 0; g < W / 16; ++g)
 #pragma unroll
             for (int k = 0; k < 16; k += SV) st16(sp + 16 * g + k, pack16<ST>(&s[g][0].x + k));
     }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
     if (warp == 0) tmem_dealloc(tmem, Lay::kTmem);
-    if (tid == 0 && sh.abort) flag_status(a.dev_status, CC1D_DEV_TIMEOUT);
 }
 
 using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -406,7 +431,7 @@ cudaError_t go(const cc1d_gdr_args& a, const CUtensorMap& q, const CUtensorMap& 
     const cudaError_t err = limit.raise(gdr_chunk_kernel<T, ST, VS>, smem);
     if (err != cudaSuccess) return err;
     return launch_dependent(gdr_chunk_kernel<T, ST, VS>, (unsigned)grid, kThreads, smem, stream, a, q, k, v,
-                            tiles, out32);
+                            tiles, out32, wait_limit_ns());
 }
 
 template <typename T, typename ST>

@@ -19,14 +19,16 @@ struct ChunkImage {
     float in[2 * C];                 // r_i e^(b_i) (rows of K), s_i e^(b_i) (rows of Q)
     float out[C];                    // r_j e^(b_C - b_j)
     float decay;                     // e^(b_C)
-    float pad[3];
+    int32_t failed;                  // the prep kernel gave up a wait: nothing here is valid
+    int32_t pad[2];
 };
 constexpr int kTgBytes = 3 * 128 * 128;
 constexpr int kVectorBytes = (int)sizeof(ChunkImage) - kTgBytes;  // what follows tg
 
 // The row factors of a ChunkImage, as they follow its T and G.
 struct Vectors {
-    float in[2 * C], out[C], decay, pad[3];
+    float in[2 * C], out[C], decay;
+    int32_t failed, pad[2];
 };
 static_assert(sizeof(Vectors) == kVectorBytes, "");
 
@@ -149,6 +151,12 @@ bool have_maps();
 
 cudaError_t launch_gdr_prep(const cc1d_gdr_args& a, const CUtensorMap& q, const CUtensorMap& k,
                             cudaStream_t stream);
+// What a CTA that has given up waits for its own copies and products at most, one by one.
+constexpr int64_t kDrainNs = 2000000000;
+
+// 16 bytes of NaN of either 16-bit type: the outputs of a CTA that gave up.
+__device__ __forceinline__ uint4 nan16() { return make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu); }
+
 // The split of fp16 keys and queries, into the workspace at `to`.
 cudaError_t launch_gdr_split(const cc1d_gdr_args& a, void* to, cudaStream_t stream);
 

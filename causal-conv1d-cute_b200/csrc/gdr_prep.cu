@@ -42,9 +42,9 @@ struct Smem {
     Blocks blk;
     Gates gates[kHeads];
     alignas(16) float rk[C], ru[kHeads][32];  // inverse norms of the keys; with e^(b_31 - b_j)
-    uint64_t full, mma;
+    uint64_t full, mma, last;
     uint32_t tmem;
-    int abort, seq;
+    int abort, late, seq;
 };
 
 // Row i of the inverse of I + l (l strictly lower triangular, 16 x 16, zeros above) by backward
@@ -156,7 +156,7 @@ __device__ __forceinline__ float bits_value(uint32_t b, int dtype) {
 template <bool kLo>
 __global__ void __launch_bounds__(128, kLo ? 2 : 3)
 gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__ CUtensorMap mapq,
-                const __grid_constant__ CUtensorMap mapk) {
+                const __grid_constant__ CUtensorMap mapk, int64_t wait_ns) {
     extern __shared__ __align__(1024) unsigned char raw[];
     Smem<kLo>& sh = *reinterpret_cast<Smem<kLo>*>(raw + ((1024 - (smem_addr(raw) & 1023)) & 1023));
     const uint32_t kq = smem_addr(sh.kq), tb = kq, pb = kq + 24576;
@@ -187,8 +187,9 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
     if (p == 0) {
         mbar_init(smem_addr(&sh.full), 1);
         mbar_init(smem_addr(&sh.mma), 1);
+        mbar_init(smem_addr(&sh.last), 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        sh.abort = 0;
+        sh.abort = sh.late = 0;
     }
     if (w == 0) {
         tmem_alloc(smem_addr(&sh.tmem), 128);
@@ -199,7 +200,7 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
     tc_fence_after();
     const uint32_t D0 = sh.tmem, DG = D0 + 64;  // [K;Q] K^T; G
     const uint32_t lanes = (uint32_t)w << 21;   // the warp's first TMEM lane, in bits 16..
-    if (p == 0) {
+    if (p == 0 && wait_ns > 0) {
         const uint32_t full = smem_addr(&sh.full);
         mbar_expect(full, Parts<kLo>::kBytes);
         load_kq<kLo>(kq, &mapk, &mapq, hk, (int)tok0, full);
@@ -268,7 +269,7 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
     if (w < group) load_gates(hk * group + w);
     if (w < group) make_gates(sh.gates[w]);
 
-    mbar_wait(smem_addr(&sh.full), 0, &sh.abort);
+    mbar_wait(smem_addr(&sh.full), 0, &sh.abort, wait_ns);
     if (left < C) {
         // The copies went on into the next sequence: zeros there, whatever it holds.
         for (int e = p; e < (C - left) * 32; e += 128) {
@@ -323,7 +324,7 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
     if (p < C) sh.rk[p] = norm;
     __syncthreads();
     sh.ru[w][lane] = sh.rk[lane] * sh.gates[w].far[lane];
-    mbar_wait(smem_addr(&sh.mma), phase, &sh.abort);
+    mbar_wait(smem_addr(&sh.mma), phase, &sh.abort, wait_ns);
     phase ^= 1;
     // K and Q are through; T and P are zero above their diagonal blocks from here on.
     if (p < 32) {
@@ -340,7 +341,7 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
     // G of value head h, once its product is there: rows 64.. of the product, by warps 2 and 3.
     auto store_g = [&](int h) {
         ChunkImage* out = static_cast<ChunkImage*>(a.workspace) + image * a.heads_v + h;
-        mbar_wait(smem_addr(&sh.mma), phase, &sh.abort);
+        mbar_wait(smem_addr(&sh.mma), phase, &sh.abort, wait_ns);
         phase ^= 1;
         tc_fence_after();
 #pragma unroll 1
@@ -376,7 +377,10 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
         const float mul = norm * (p < C ? ga.beta[i] : a.scale);  // of row i of L or P
         out->in[p] = ga.grow[i] * (p < C ? norm : mul);
         if (p < C) out->out[i] = norm * ga.out[i];
-        if (p == C - 1) out->decay = ga.grow[i];
+        if (p == C - 1) {
+            out->decay = ga.grow[i];
+            out->failed = 0;
+        }
         // The head before: its G, while warps 0 and 1 are at L and its inverse.
         if (p >= C && v > 0) store_g(h - 1);
         // Warps 0 and 1 make L (columns j < i) of rows of K K^T, warps 2 and 3 make P (columns
@@ -505,9 +509,10 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
         if (p == 96) {
             // A thread of the warps that wait for this product next.
             tc_fence_after();
-            // G = P T in rows 64.., by parts. The 8 KB before a part of P are other parts of T or P; the
-            // rows 0..63 they make are of no use.
-            const uint64_t P = operand(pb - 8192, 16, 1024, kSwizzle128), T = operand(tb, 16384, 1024, kSwizzle128);
+            // G = P T in rows 64.., by parts. The 8 KB before a part of P are other parts of T or P;
+            // the rows 0..63 they make are of no use.
+            const uint64_t P = operand(pb - 8192, 16, 1024, kSwizzle128);
+            const uint64_t T = operand(tb, 16384, 1024, kSwizzle128);
 #pragma unroll
             for (int sum = 2; sum >= 0; --sum)
 #pragma unroll
@@ -528,8 +533,19 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
     if (p == 96) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     __syncthreads();
     tc_fence_after();
+    if (sh.abort) {
+        // What the two threads that issue products have issued.
+        if (p == 0 || p == 96) mma_commit(smem_addr(&sh.last));
+        if (p == 0) {
+            mbar_wait(smem_addr(&sh.last), 0, &sh.late, kDrainNs);
+            if (wait_ns > 0) mbar_wait(smem_addr(&sh.full), 0, &sh.late, kDrainNs);
+        }
+        for (int v = p; v < group; v += 128)
+            (static_cast<ChunkImage*>(a.workspace) + image * a.heads_v + hk * group + v)->failed = 1;
+        if (p == 0) flag_status(a.dev_status, CC1D_DEV_TIMEOUT);
+        __syncthreads();
+    }
     if (w == 0) tmem_dealloc(sh.tmem, 128);
-    if (p == 0 && sh.abort) flag_status(a.dev_status, CC1D_DEV_TIMEOUT);
 }
 
 // fp16 keys and queries to bf16 parts, four values a lane; bound by HBM. One warp per token and head.
@@ -567,7 +583,7 @@ cudaError_t launch_gdr_prep(const cc1d_gdr_args& a, const CUtensorMap& q, const 
         static SmemLimit limit;
         const cudaError_t err = limit.raise(gdr_prep_kernel<kLo>, smem);
         if (err != cudaSuccess) return err;
-        gdr_prep_kernel<kLo><<<(unsigned)grid, 128, smem, stream>>>(a, q, k);
+        gdr_prep_kernel<kLo><<<(unsigned)grid, 128, smem, stream>>>(a, q, k, wait_limit_ns());
         return cudaGetLastError();
     };
     return a.dtype == CC1D_F16 ? go(std::true_type()) : go(std::false_type());

@@ -51,13 +51,14 @@ enum : uint32_t {
     kColumns = 512
 };
 
-// Named barriers: the operand of a product is written.
-enum { kHaveS = 1, kHaveR, kHaveU };
+// Named barriers: the operand of a product is written; nobody starts anything any more.
+enum { kHaveS = 1, kHaveR, kHaveU, kDone };
 
 struct Shared {
-    uint64_t full[2], tg_full[2], v_full, mma;
+    uint64_t full[2], tg_full[2], v_full, mma, last;
+    int begun[5];  // copies begun on the first five of these
     uint32_t tmem;
-    int abort;
+    int abort, late;
     int row;  // sequence of this CTA
 };
 
@@ -135,7 +136,8 @@ __device__ __forceinline__ uint32_t pack2(float2 f) {
 template <typename T, typename ST>
 __global__ void __launch_bounds__(kThreads, 1)
 gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__ CUtensorMap mapq,
-                const __grid_constant__ CUtensorMap mapk, const __grid_constant__ CUtensorMap mapv, int tiles) {
+                const __grid_constant__ CUtensorMap mapk, const __grid_constant__ CUtensorMap mapv, int tiles,
+                int64_t wait_ns) {
     constexpr bool kLo = std::is_same<T, f16>::value;  // fp16 keys and queries come in two bf16 parts
     using Lay = Layout<kLo>;
     constexpr int kStages = Lay::kStages, kTgStages = Lay::kTgStages;
@@ -166,8 +168,10 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
         }
         mbar_init(smem_addr(&sh.v_full), 1);
         mbar_init(smem_addr(&sh.mma), 1);
+        mbar_init(smem_addr(&sh.last), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        sh.abort = 0;
+        for (int i = 0; i < 5; ++i) sh.begun[i] = 0;
+        sh.abort = sh.late = 0;
     }
     if (warp == 0) {
         tmem_alloc(smem_addr(&sh.tmem), kColumns);
@@ -187,7 +191,7 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
         for (int c = 0, st = 0; c < chunks; ++c) {
             const uint32_t kq = base + Lay::KQ + st * Lay::kKQ, tg = base + Lay::TG + c % kTgStages * kTgBytes;
             const uint32_t mma = smem_addr(&sh.mma);
-            mbar_wait(smem_addr(&sh.full[st]), st_phase, &sh.abort);
+            mbar_wait(smem_addr(&sh.full[st]), st_phase, &sh.abort, wait_ns);
             named_sync(kHaveS, kThreads);
             if (lane == 0) {
                 tc_fence_after();
@@ -210,7 +214,7 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
                                            mma_desc(128, false, false), kLo || m < 2 || half > 0);
                 mma_commit(mma);
             }
-            mbar_wait(smem_addr(&sh.tg_full[c % kTgStages]), c / kTgStages & 1, &sh.abort);
+            mbar_wait(smem_addr(&sh.tg_full[c % kTgStages]), c / kTgStages & 1, &sh.abort, wait_ns);
             named_sync(kHaveR, kThreads);
             if (lane == 0) {
                 tc_fence_after();
@@ -244,10 +248,19 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
                 st_phase ^= 1;
             }
         }
+        named_sync(kDone, kThreads);
+        if (sh.abort && lane == 0) {
+            mma_commit(smem_addr(&sh.last));
+            mbar_wait(smem_addr(&sh.last), 0, &sh.late, kDrainNs);
+        }
     } else if (warp > kWorkers / 32) {
         // Copies, one thread: K, Q and the row factors of chunk c into stage st, which must be free;
         // T and G, into the stage of their own; V.
+        // Copies may be started: those of earlier chunks have been waited for.
+        auto live = [&] { return *(volatile int*)&sh.abort == 0 && wait_ns > 0; };
         auto load = [&](int c, int st) {
+            if (!live()) return;
+            sh.begun[st] = c / kStages + 1;
             const uint32_t full = smem_addr(&sh.full[st]);
             const ChunkImage* from = image + (int64_t)c * a.heads_v;
             mbar_expect(full, Lay::kKQ + kVectorBytes);
@@ -255,12 +268,16 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
             bulk_load(base + Lay::VEC + st * kVectorBytes, from->in, kVectorBytes, full);
         };
         auto load_tg = [&](int c) {
+            if (!live()) return;
             const int st = c % kTgStages;
+            sh.begun[2 + st] = c / kTgStages + 1;
             const uint32_t full = smem_addr(&sh.tg_full[st]);
             mbar_expect(full, kTgBytes);
             bulk_load(base + Lay::TG + st * kTgBytes, image[(int64_t)c * a.heads_v].tg, kTgBytes, full);
         };
         auto load_v = [&](int c) {
+            if (!live()) return;
+            sh.begun[4] = c + 1;
             const uint32_t full = smem_addr(&sh.v_full);
             mbar_expect(full, C * VS * 2);
             for (int half = 0; half < 2; ++half)
@@ -284,6 +301,13 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
             named_sync(kHaveU, kThreads);
             if (lane == 0 && c + kTgStages < chunks) load_tg(c + kTgStages);
             if (++st == kStages) st = 0;
+        }
+        named_sync(kDone, kThreads);
+        if (sh.abort && lane == 0) {
+            for (int i = 0; i < 5; ++i)
+                if (sh.begun[i] > 0)
+                    mbar_wait(smem_addr(sh.full) + 8 * i, (sh.begun[i] - 1) & 1, &sh.late, kDrainNs);
+            flag_status(a.dev_status, CC1D_DEV_TIMEOUT);
         }
     } else {
         // This thread's state: column 32 w + lane of the tile, rows 32 part ..
@@ -313,7 +337,7 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
 
         int st = 0;
         uint32_t phase = 0, st_phase = 0;
-        mbar_wait(smem_addr(&sh.full[0]), 0, &sh.abort);
+        mbar_wait(smem_addr(&sh.full[0]), 0, &sh.abort, wait_ns);
 #pragma unroll 1
         for (int c = 0; c < chunks; ++c) {
             const uint32_t kq = base + Lay::KQ + st * Lay::kKQ;
@@ -339,13 +363,13 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
             arrive(kHaveS);
             {
                 // R = V - r e^b (K S)
-                mbar_wait(smem_addr(&sh.v_full), c & 1, &sh.abort);
+                mbar_wait(smem_addr(&sh.v_full), c & 1, &sh.abort, wait_ns);
                 uint32_t vv[8];
                 ldsm_t(vb + swz<128>(v_row, v_unit), vv);
                 ldsm_t(vb + swz<128>(v_row, v_unit + 2), vv + 4);
                 const uint32_t at = vec_at + st * kVectorBytes + 4 * (16 * part + pair);
                 const float2 f[2] = {lds_pair(at), lds_pair(at + 32)};
-                mbar_wait(mma, phase, &sh.abort);
+                mbar_wait(mma, phase, &sh.abort, wait_ns);
                 phase ^= 1;
                 tc_fence_after();
                 float2 d[8];
@@ -377,7 +401,7 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
                 const uint32_t at = vec_at + st * kVectorBytes + 4 * (16 * part + pair);
                 const float2 f[2] = {lds_pair(at + 8 * C), lds_pair(at + 8 * C + 32)};
                 const float2 fq[2] = {lds_pair(at + 4 * C), lds_pair(at + 4 * C + 32)};
-                mbar_wait(mma, phase, &sh.abort);
+                mbar_wait(mma, phase, &sh.abort, wait_ns);
                 phase ^= 1;
                 tc_fence_after();
                 float2 d[8];
@@ -411,13 +435,15 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
                     if (16 * part + 8 * b + lane / 4 < left) st16_stream(to + 8 * b * a.o_st, x);
                 }
             }
-            const float decay = reinterpret_cast<const Vectors*>(gen + Lay::VEC)[st].decay;
+            const Vectors& vec = reinterpret_cast<const Vectors*>(gen + Lay::VEC)[st];
+            const float decay = vec.decay;
+            if (tid == 0 && vec.failed) *(volatile int*)&sh.abort = 1;
             if (++st == kStages) {
                 st = 0;
                 st_phase ^= 1;
             }
-            if (c + 1 < chunks) mbar_wait(smem_addr(&sh.full[st]), st_phase, &sh.abort);
-            mbar_wait(mma, phase, &sh.abort);
+            if (c + 1 < chunks) mbar_wait(smem_addr(&sh.full[st]), st_phase, &sh.abort, wait_ns);
+            mbar_wait(mma, phase, &sh.abort, wait_ns);
             phase ^= 1;
             tc_fence_after();
 #pragma unroll
@@ -429,7 +455,12 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
                     s[8 * g + k] = __ffma2_rn(make_float2(decay, decay), s[8 * g + k], d[k]);
             }
         }
-        if (sp != nullptr) {
+        named_sync(kDone, kThreads);
+        if (sh.abort) {
+            // The cache keeps its state, and the outputs say that they are none.
+            for (int64_t t = 16 * part + lane / 4; t < ntok; t += t % 16 < 8 ? 8 : C - 8)
+                st16(op + (t - 16 * part - lane / 4) * a.o_st, nan16());
+        } else if (sp != nullptr) {
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
                 ST* at = sp + 2 * k * a.s_sk;
@@ -443,7 +474,6 @@ gdr_wide_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
     __syncthreads();
     tc_fence_after();
     if (warp == 0) tmem_dealloc(tmem, kColumns);
-    if (tid == 0 && sh.abort) flag_status(a.dev_status, CC1D_DEV_TIMEOUT);
 }
 
 template <typename T, typename ST>
@@ -457,7 +487,8 @@ cudaError_t go(const cc1d_gdr_args& a, const CUtensorMap& q, const CUtensorMap& 
     static SmemLimit limit;
     const cudaError_t err = limit.raise(gdr_wide_kernel<T, ST>, smem);
     if (err != cudaSuccess) return err;
-    return launch_dependent(gdr_wide_kernel<T, ST>, (unsigned)grid, kThreads, smem, stream, a, q, k, v, tiles);
+    return launch_dependent(gdr_wide_kernel<T, ST>, (unsigned)grid, kThreads, smem, stream, a, q, k, v, tiles,
+                            wait_limit_ns());
 }
 
 }  // namespace

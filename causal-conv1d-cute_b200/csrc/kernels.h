@@ -142,6 +142,9 @@ cudaError_t launch_gdr_recurrent(const cc1d_gdr_args& a, bool varlen, cudaStream
 bool gdr_chunk_serves(const cc1d_gdr_args& a);
 int64_t gdr_chunk_workspace(const cc1d_gdr_args& a);
 cudaError_t launch_gdr_chunk(const cc1d_gdr_args& a, cudaStream_t stream);
+// How long the chunked kernels wait for a copy or a product of their own, which takes microseconds. 0:
+// they start no copy, and the waits for them run out.
+int64_t wait_limit_ns();
 cudaError_t launch_norm(const cc1d_norm_args& a, cudaStream_t stream);
 // same: the table's src and dst are the same caches (a source may be an earlier destination).
 cudaError_t launch_slots_copy(const cc1d_slot_cache* table, int ncaches, const int32_t* src,

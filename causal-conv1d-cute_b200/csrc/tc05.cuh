@@ -29,9 +29,10 @@ __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
                  : "memory");
 }
-// Wait until the phase of the given parity has completed, for two seconds at most (a chunk takes
-// microseconds). When one wait of the CTA has run out, *abort is set and every later wait returns
-// at once, so that the CTA runs to its end, with wrong results that it reports, and frees its TMEM.
+// Wait until the phase of the given parity has completed, for limit_ns at most. When one wait of the
+// CTA has run out, *abort is set and every later wait returns at once, so that the CTA runs to its end:
+// it starts no further copy, waits for what is in flight (drain), says that its results are invalid and
+// frees its TMEM.
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     uint32_t done;
     asm volatile(
@@ -43,20 +44,22 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
         : "memory");
     return done != 0;
 }
-static __device__ __noinline__ void mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort) {
+static __device__ __noinline__ void mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort,
+                                                   int64_t limit_ns) {
     unsigned long long start, now;
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(start));
     while (!*abort) {
         for (int i = 0; i < 64; ++i)
             if (mbar_try(bar, parity)) return;
         asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
-        if (now - start > 2000000000ull) *abort = 1;
+        if (now - start > (unsigned long long)limit_ns) *abort = 1;
     }
 }
-__device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+__device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort,
+                                          int64_t limit_ns) {
     for (int i = 0; i < 16; ++i)
         if (mbar_try(bar, parity)) return;
-    mbar_wait_slow(bar, parity, abort);
+    mbar_wait_slow(bar, parity, abort, limit_ns);
 }
 // Barrier of `threads` threads (whole warps) of the CTA.
 __device__ __forceinline__ void named_sync(int id, int threads) {

@@ -48,7 +48,7 @@ enum {
     CC1D_DEV_BAD_SLOT = 1,       /* a conv-state / ring slot outside [0, nslots) and != pad */
     CC1D_DEV_BAD_QSL = 2,        /* query_start_loc outside [0, ntokens] or decreasing */
     CC1D_DEV_BAD_INTER_SLOT = 4, /* a per-step state slot outside [0, inter_nslots) */
-    CC1D_DEV_TIMEOUT = 8         /* a wait inside a kernel ran out; that call's results are invalid */
+    CC1D_DEV_TIMEOUT = 8         /* a wait inside a kernel ran out (cc1d_set_wait_limit) */
 };
 
 /* ABI revision; bumped on any signature change. */
@@ -264,6 +264,15 @@ typedef struct {
  * by token. The workspace holds nothing between calls.
  */
 cc1d_status_t cc1d_gdr_workspace(const cc1d_gdr_args* args, int64_t* bytes);
+
+/*
+ * The chunked kernels wait for copies and products of their own, which takes microseconds. A wait that
+ * takes longer than ns (2 s unless set; for the process, later calls) is given up: the outputs of that
+ * sequence and head (or of some of its columns) are NaN, its slot keeps its state there, and
+ * CC1D_DEV_TIMEOUT is reported. With 0 nothing is copied and every wait runs out, which shows what a
+ * caller does about it.
+ */
+cc1d_status_t cc1d_set_wait_limit(int64_t ns);
 
 cc1d_status_t cc1d_gdr_update(const cc1d_gdr_args* args, void* stream);
 cc1d_status_t cc1d_gdr_varlen(const cc1d_gdr_args* args, void* stream);

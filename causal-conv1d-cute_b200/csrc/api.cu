@@ -88,21 +88,35 @@ cc1d_status_t check_gdr(const cc1d_gdr_args& a) {
     return CC1D_OK;
 }
 
-cc1d_status_t check_slots(const cc1d_slot_cache* table, int32_t ncaches) {
+// Bytes from the first slot's first byte to the last slot's last (slots that do not overlap).
+int64_t slots_span(int64_t nslots, int64_t stride, int64_t row) {
+    return nslots < 1 || row < 1 ? 0 : (nslots - 1) * stride + row;
+}
+
+// One side of a cache; a group without slots, or rows without bytes, need no memory.
+bool slots_ok(const void* p, int64_t nslots, int64_t stride, int64_t row) {
+    if (row < 0) return false;
+    if (nslots < 1 || row == 0) return true;
+    return p != nullptr && (nslots == 1 || (stride >= row && stride <= (INT64_MAX - row) / (nslots - 1)));
+}
+
+cc1d_status_t check_slots(const cc1d_slot_cache* table, int32_t ncaches, int64_t dst_nslots,
+                          int64_t src_nslots) {
     if (ncaches < 0 || ncaches > CC1D_MAX_CACHES)
         return fail(CC1D_ERR_INVALID, "%d caches (at most %d a call)", ncaches, CC1D_MAX_CACHES);
     if (ncaches > 0 && table == nullptr) return fail(CC1D_ERR_INVALID, "table is NULL");
     for (int32_t i = 0; i < ncaches; ++i)
-        if (table[i].dst == nullptr || table[i].src == nullptr || table[i].row_bytes < 0 ||
-            table[i].dst_stride < table[i].row_bytes || table[i].src_stride < table[i].row_bytes)
+        if (!slots_ok(table[i].dst, dst_nslots, table[i].dst_stride, table[i].row_bytes) ||
+            !slots_ok(table[i].src, src_nslots, table[i].src_stride, table[i].row_bytes))
             return fail(CC1D_ERR_INVALID, "cache %d has a NULL pointer or overlapping slots", i);
     return CC1D_OK;
 }
 
+// Two ranges of bytes share one.
 bool overlap(const void* p, int64_t np, const void* q, int64_t nq) {
     const char* a = (const char*)p;
     const char* b = (const char*)q;
-    return a < b + nq && b < a + np;
+    return np > 0 && nq > 0 && a < b + nq && b < a + np;
 }
 
 }  // namespace
@@ -428,25 +442,28 @@ cc1d_status_t cc1d_slots_copy(const cc1d_slot_cache* table, int32_t ncaches,
                               const int32_t* src_indices, const int32_t* dst_indices,
                               int64_t npairs, int64_t src_nslots, int64_t dst_nslots,
                               int32_t pad, int32_t* dev_status, void* stream) {
-    if (cc1d_status_t s = check_slots(table, ncaches)) return s;
     if (npairs < 0 || npairs > INT32_MAX || src_nslots < 0 || dst_nslots < 0 ||
         src_nslots > INT32_MAX || dst_nslots > INT32_MAX)
         return fail(CC1D_ERR_INVALID, "%lld pairs, %lld and %lld slots", (long long)npairs,
                     (long long)src_nslots, (long long)dst_nslots);
+    if (cc1d_status_t s = check_slots(table, ncaches, dst_nslots, src_nslots)) return s;
     if (npairs == 0 || ncaches == 0) return ok();
     if (!src_indices || !dst_indices) return fail(CC1D_ERR_INVALID, "an index list is NULL");
     // A source group either is the destination group or lies apart from it.
-    int32_t same = 0;
+    int32_t same = 0, all = 0;
     for (int32_t i = 0; i < ncaches; ++i) {
-        if (table[i].src == table[i].dst && table[i].src_stride == table[i].dst_stride) {
+        const cc1d_slot_cache& c = table[i];
+        if (c.row_bytes == 0) continue;
+        ++all;
+        if (c.src == c.dst && c.src_stride == c.dst_stride) {
             ++same;
-        } else if (overlap(table[i].dst, dst_nslots * table[i].dst_stride, table[i].src,
-                           src_nslots * table[i].src_stride)) {
+        } else if (overlap(c.dst, slots_span(dst_nslots, c.dst_stride, c.row_bytes), c.src,
+                           slots_span(src_nslots, c.src_stride, c.row_bytes))) {
             return fail(CC1D_ERR_INVALID, "source and destination of cache %d overlap", i);
         }
     }
-    if (same != 0 && (same != ncaches || src_nslots != dst_nslots))
-        return fail(CC1D_ERR_INVALID, "%d of %d caches are their own source", same, ncaches);
+    if (same != 0 && (same != all || src_nslots != dst_nslots))
+        return fail(CC1D_ERR_INVALID, "%d of %d caches are their own source", same, all);
     if (cc1d_status_t s = bind_stream(stream)) return s;
     return from_cuda(cc1d::launch_slots_copy(table, ncaches, src_indices, dst_indices, npairs,
                                              src_nslots, dst_nslots, same != 0, pad, dev_status,
@@ -457,9 +474,9 @@ cc1d_status_t cc1d_slots_copy(const cc1d_slot_cache* table, int32_t ncaches,
 cc1d_status_t cc1d_slots_compact(const cc1d_slot_cache* table, int32_t ncaches,
                                  const uint8_t* live, int64_t nslots, int32_t* remap,
                                  int32_t* count, int32_t* moves, void* stream) {
-    if (cc1d_status_t s = check_slots(table, ncaches)) return s;
     if (nslots < 0 || nslots > INT32_MAX / 2 - 1)
         return fail(CC1D_ERR_INVALID, "%lld slots", (long long)nslots);
+    if (cc1d_status_t s = check_slots(table, ncaches, nslots, nslots)) return s;
     if (!count || !moves || (nslots > 0 && (!live || !remap)))
         return fail(CC1D_ERR_INVALID, "a required pointer is NULL");
     for (int32_t i = 0; i < ncaches; ++i)

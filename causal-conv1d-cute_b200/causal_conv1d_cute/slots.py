@@ -16,6 +16,24 @@ from .functional import PAD_SLOT_ID, _flags, _int32, _unsupported
 _MAX_CACHES = 64  # caches one launch takes
 
 
+def _apart(slots, spans):
+    """Whether no byte belongs to two of the caches (address, bytes from slot to slot, bytes of a slot).
+
+    Caches whose address ranges meet are apart if they are interleaved layers of one allocation: equal
+    strides, and the rows of one between those of the other.
+    """
+    spans = sorted(spans)
+    for i, (p, ps, pr) in enumerate(spans):
+        end = p + (slots - 1) * ps + pr
+        for q, qs, qr in spans[i + 1 :]:
+            if q >= end:
+                break
+            at = (q - p) % ps
+            if ps != qs or at < pr or at + qr > ps:
+                return False
+    return True
+
+
 class StateSlots:
     """A group of caches whose first axis is the slot.
 
@@ -58,19 +76,10 @@ class StateSlots:
             self._rows.append((c.data_ptr(), stride, row))
             if row:
                 spans.append((c.data_ptr(), stride, row))
-        self._check_apart(spans)
-        self._own = None
-
-    def _check_apart(self, spans):
-        """No byte belongs to two caches (a later move would depend on the launch order)."""
-        spans = sorted(spans)
-        for (p, ps, pr), (q, qs, qr) in zip(spans, spans[1:]):
-            if q >= p + (self.slots - 1) * ps + pr:
-                continue
-            # Interleaved layers of one allocation: equal strides, rows side by side.
-            if ps == qs and q >= p + pr and q + qr <= p + ps:
-                continue
+        # A byte of two caches would make a later move depend on the launch order.
+        if not _apart(self.slots, spans):
             raise ValueError("two caches of a group share memory")
+        self._own = None
 
     def _table(self, source):
         """cc1d_slot_cache arrays of at most 64 caches each, for moves out of source, as (address,

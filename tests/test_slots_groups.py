@@ -1,10 +1,46 @@
 """Groups of state caches beside one another in memory, and groups without slots."""
 
+import itertools
+
 import pytest
 import torch
 
 import causal_conv1d_cute as C
+from causal_conv1d_cute.slots import _apart
 from test_slots import apply, int32, same
+
+
+@pytest.mark.parametrize("slots,stride", [(1, 10), (2, 10), (4, 10), (3, 7)])
+def test_apart_is_exact_for_equal_strides(slots, stride):
+    """Every placement of up to three caches against the sets of their bytes."""
+
+    def bytes_of(p, row):
+        return {p + s * stride + b for s in range(slots) for b in range(row)}
+
+    rows = (3, 4, 5)[: stride // 3]
+    for q, r in itertools.product(range(0, slots * stride + 6, 1), repeat=2):
+        spans = [(20, stride, rows[0]), (20 + q, stride, rows[1]), (14 + r, stride, rows[-1])]
+        if slots == 1:  # one slot: the stride is the row
+            spans = [(p, row, row) for p, _, row in spans]
+        sets = [bytes_of(p, row) for p, _, row in spans]
+        want = not any(a & b for a, b in itertools.combinations(sets, 2))
+        assert _apart(slots, spans) == want, spans
+
+
+def test_third_cache_in_the_next_slot_of_the_first():
+    assert not _apart(4, [(0, 100, 40), (50, 100, 40), (95, 100, 40)])
+    assert not _apart(4, [(0, 10, 4), (4, 10, 4), (8, 10, 4)])
+    assert _apart(4, [(0, 12, 4), (4, 12, 4), (8, 12, 4)])
+    assert not _apart(4, [(0, 100, 40), (50, 60, 10)])
+
+
+@pytest.mark.gpu
+def test_group_with_such_a_cache_is_refused():
+    memory = torch.zeros(64, device="cuda")
+    views = [memory[at:].as_strided((4, 4), (10, 1)) for at in (0, 4, 8)]
+    with pytest.raises(ValueError, match="share"):
+        C.StateSlots(views)
+    C.StateSlots(views[:2])
 
 
 @pytest.mark.gpu

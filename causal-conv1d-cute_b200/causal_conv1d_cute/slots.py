@@ -14,6 +14,7 @@ from . import _ops
 from .functional import PAD_SLOT_ID, _flags, _int32, _unsupported
 
 _MAX_CACHES = 64  # caches one launch takes
+_data_ptr, _numel, _stride = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.stride
 
 
 def _apart(slots, spans):
@@ -37,7 +38,9 @@ def _apart(slots, spans):
 class StateSlots:
     """A group of caches whose first axis is the slot.
 
-    The caches keep their own storage and dtypes; the object holds references to them.
+    The caches keep their own storage and dtypes; the object holds references to them. Addresses are
+    taken once, and again when a cache has been given other memory, size or strides (cache.data = ...,
+    set_, resize_), which then has to satisfy the constructor's rules.
     """
 
     def __init__(self, caches):
@@ -49,7 +52,23 @@ class StateSlots:
             ValueError: shapes that do not form a group, or caches that share memory.
             Unsupported: CPU tensors, or slots that are not contiguous.
         """
-        caches = list(caches)
+        self.caches = list(caches)
+        self._layout()
+
+    def _place(self):
+        """What the addresses of the slots depend on (0.3 us a cache)."""
+        c = self.caches
+        return [*map(_data_ptr, c), *map(_numel, c), *map(_stride, c)]
+
+    def _fresh(self):
+        if self._place() != self._placed:
+            self._layout()
+        return self
+
+    def _layout(self):
+        """Check the caches and take their addresses."""
+        caches = self.caches
+        self._placed = self._own = None  # nothing is kept of caches that are refused
         if not caches or any(c.dim() < 1 for c in caches):
             raise ValueError("StateSlots needs one cache at least, each with a slot axis")
         if any(c.shape[0] != caches[0].shape[0] for c in caches):
@@ -61,7 +80,6 @@ class StateSlots:
         for c in caches:
             if c.shape[0] and not c[0].is_contiguous():
                 _unsupported(f"slots of a cache with strides {c.stride()} are not contiguous")
-        self.caches = caches
         self.slots = caches[0].shape[0]
         self.device = caches[0].device
         # (pointer, bytes from slot to slot, bytes of a slot) of each cache that holds anything
@@ -79,7 +97,7 @@ class StateSlots:
         # A byte of two caches would make a later move depend on the launch order.
         if not _apart(self.slots, spans):
             raise ValueError("two caches of a group share memory")
-        self._own = None
+        self._placed = self._place()
 
     def _table(self, source):
         """cc1d_slot_cache arrays of at most 64 caches each, for moves out of source, as (address,
@@ -111,7 +129,8 @@ class StateSlots:
                 of a verified draft, viewed as (rows * steps, ...).
             pad_slot_id: the index value described above.
         """
-        source = self if source is None else source
+        self._fresh()
+        source = self if source is None else source._fresh()
         if src_indices.dim() != 1 or src_indices.shape != dst_indices.shape:
             raise ValueError(
                 f"index lists of shapes {tuple(src_indices.shape)} and {tuple(dst_indices.shape)}"
@@ -152,6 +171,7 @@ class StateSlots:
             (remap, count): int32 (slots,) new slot of each old one (-1: not live), and int32 ()
             the number of live slots, both on the device (nothing is synchronised).
         """
+        self._fresh()
         if tuple(live.shape) != (self.slots,):
             raise ValueError(f"live must have shape ({self.slots},), got {tuple(live.shape)}")
         live = _flags(live, self.device)

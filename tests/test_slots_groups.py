@@ -73,3 +73,55 @@ def test_source_without_slots():
     group.copy(int32([-1]), int32([1]), source=none)
     assert group.caches[0].sum(1).tolist() == [8, 0, 8]
     none.copy(int32([]), int32([]), source=group)
+
+
+def swap_data(cache, other):
+    cache.data = other
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("change", [swap_data, lambda cache, other: cache.set_(other)])
+@pytest.mark.parametrize("step", ["copy", "compact", "source"])
+def test_cache_with_other_memory(change, step):
+    """A cache is followed to the memory that it was given; the memory before is left alone."""
+    caches = [torch.randn(4, 8, device="cuda"), torch.randn(4, 3, device="cuda")]
+    rec = [torch.randn(2, 8, device="cuda"), torch.randn(2, 3, device="cuda")]
+    group, source = C.StateSlots(caches), C.StateSlots(rec)
+    live = torch.tensor([0, 1, 0, 1], dtype=torch.bool, device="cuda")
+    group.copy(int32([0]), int32([1]))
+    group.copy(int32([0]), int32([1]), source=source)
+    moved = rec if step == "source" else caches
+    old = moved[0].detach()
+    before = old.clone()
+    change(moved[0], torch.randn(len(old), 8, device="cuda"))
+    want = [c.clone() for c in caches]
+    if step == "copy":
+        group.copy(int32([0, -1]), int32([1, 3]))
+        apply(want, [0, -1], [1, 3])
+    elif step == "compact":
+        group.compact(live)
+        apply(want, [3], [0])
+    else:
+        group.copy(int32([1]), int32([2]), source=source)
+        apply(want, [1], [2], source=rec)
+    same(caches, want)
+    assert torch.equal(old, before)
+
+
+@pytest.mark.gpu
+def test_cache_with_memory_that_does_not_fit():
+    caches = [torch.zeros(4, 8, device="cuda"), torch.zeros(4, 3, device="cuda")]
+    group = C.StateSlots(caches)
+    caches[0].data = torch.zeros(5, 8, device="cuda")
+    for _ in range(2):
+        with pytest.raises(ValueError, match="slots"):
+            group.copy(int32([0]), int32([1]))
+    caches[0].data = torch.zeros(4, 3, 8, device="cuda").transpose(1, 2)
+    with pytest.raises(C.Unsupported):
+        group.compact(torch.ones(4, dtype=torch.bool, device="cuda"))
+    caches[0].data = caches[1].data
+    with pytest.raises(ValueError, match="share"):
+        group.copy(int32([0]), int32([1]))
+    caches[0].data, caches[1].data = torch.ones(6, 8, device="cuda"), torch.ones(6, 3, device="cuda")
+    group.copy(int32([-1]), int32([5]))
+    assert len(group) == 6 and [c.sum().item() for c in caches] == [40, 15]

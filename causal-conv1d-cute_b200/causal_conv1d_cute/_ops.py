@@ -298,7 +298,7 @@ def _gdr_varlen_impl(q, k, v, g, beta, a_log, dt_bias, out, states, qsl, idx, hi
     # work only. Heads do not depend on one another, so a call that would need too much goes in groups.
     hk, r = q.shape[1], v.shape[1] // q.shape[1]
     n = -(-hk // min(hk, -(-need.value // _GDR_WORKSPACE)))
-    space = torch.empty(-(-need.value // hk) * n + 128, dtype=torch.uint8, device=q.device)
+    space = torch.empty(-(-need.value // hk) * n + 512, dtype=torch.uint8, device=q.device)
     if n == hk:
         return _run(q.device, lib.cc1d_gdr_varlen, _with_workspace(args, space))
 

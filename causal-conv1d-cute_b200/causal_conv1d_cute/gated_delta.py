@@ -121,11 +121,16 @@ def gated_delta_rule_varlen_fn(
             and their slots untouched).
         out: optional output of the shape and dtype of v.
 
-    bf16 and fp16 calls with dk = 128, rows on 16-byte boundaries and 10 tokens a sequence on average
-    run chunk by chunk on the tensor cores, whose operands hold the 24 bits of fp32 in three parts: final
-    states are as near to the definition as token by token. Their temporary takes 49,936 bytes per
-    value head for each of tokens / 64 + batch chunks, and 1024 bytes per token and key head more for
-    fp16 (in groups of heads from 4 GiB on). Other calls run token by token.
+    Two forms serve a call. Chunk by chunk of 64 tokens on the tensor cores: bf16 and fp16 with dk = 128,
+    dv a multiple of 32 and rows on 16-byte boundaries, where sequences have 12 tokens on average; in other
+    batches of 128 tokens and more the long sequences (above 32 tokens, or where there are more than 32
+    such above 64, 128, ..). Token by token: all else. Both hold the precision of fp32 (the operands of the
+    tensor cores have its 24 bits, in three parts), but they round differently, so that the last bits of a
+    sequence depend on the batch it came in, and where a value is not finite the chunked form spoils
+    the rows of its whole chunk, earlier ones included, token by token only its own and later ones. The
+    chunked form's temporary takes 49,936 bytes per value head for each of tokens / 64 + batch chunks
+    (32 or fewer instead of batch for long sequences alone), and 1024 bytes per token and key head more for fp16
+    (in groups of heads from 4 GiB on).
 
     The chunked kernels wait for copies of their own. Should such a wait ever take above two seconds,
     the outputs that depend on it are NaN, the slot keeps its state, and device_status() says so

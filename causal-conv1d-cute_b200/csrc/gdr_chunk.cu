@@ -42,6 +42,8 @@
 // Stacking K over Q and T over G makes every product M = 128, the full tensor core rate; the parts of
 // an operand lie side by side as one operand of 3 VS columns (measured: a K step of 16 costs 46 cycles
 // up to 64 columns, 66 with 128 and 137 with 256, so one wide step beats two narrow ones).
+#include <algorithm>
+
 #include "gdr_chunk.cuh"
 
 namespace cc1d {
@@ -99,7 +101,7 @@ template <typename T, typename ST, int VS>
 __global__ void __launch_bounds__(kThreads, 1)
 gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__ CUtensorMap mapq,
                  const __grid_constant__ CUtensorMap mapk, const __grid_constant__ CUtensorMap mapv,
-                 int tiles, bool out32, int64_t wait_ns) {
+                 int tiles, bool out32, Sequences seqs, int64_t wait_ns) {
     constexpr bool kLo = std::is_same<T, f16>::value;  // fp16 keys and queries come in two bf16 parts
     using Lay = Layout<VS, kLo>;
     constexpr uint64_t kSwz = VS == 64 ? kSwizzle128 : kSwizzle64;
@@ -117,13 +119,19 @@ gdr_chunk_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant_
     int64_t row = blockIdx.x / tiles / a.heads_v;
     const int hk = h / (a.heads_v / a.heads_k);
 
-    row = longest_first(a, row, reinterpret_cast<int*>(gen), &sh.row);
+    int64_t seq = row;
+    if (seqs.list != nullptr) {
+        if (seq >= seqs.list[0]) return;
+        row = seqs.list[2 + seq];
+    } else {
+        seq = row = longest_first(a, row, reinterpret_cast<int*>(gen), &sh.row);
+    }
     int64_t tok0, slot;
     int ntok;
     if (!gdr_row(a, true, row, tok0, ntok, slot, h == 0 && vt == 0 && tid == 0)) return;
     const int chunks = (ntok + C - 1) / C;
     const ChunkImage* image =
-        static_cast<const ChunkImage*>(a.workspace) + chunk_base(tok0, row) * a.heads_v + h;
+        static_cast<const ChunkImage*>(a.workspace) + chunk_base(tok0, seq) * a.heads_v + h;
 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -414,16 +422,25 @@ Encode encoder() {
 }
 
 // The chunk images, in whole 128-byte lines.
-int64_t images_bytes(const cc1d_gdr_args& a) {
-    return ceil_div(chunk_slots(a.tokens, a.rows) * a.heads_v * (int64_t)sizeof(ChunkImage), 128) * 128;
+int64_t images_bytes(const cc1d_gdr_args& a, const Sequences& seqs) {
+    return ceil_div(chunk_slots(a.tokens, seqs.n) * a.heads_v * (int64_t)sizeof(ChunkImage), 128) * 128;
 }
 
+// Whether a batch is of mostly short sequences, and may hold long ones all the same.
+bool mostly_short(const cc1d_gdr_args& a) { return a.tokens < 12 * a.rows; }
+
+// Those that run in chunks, with their list (in the workspace, behind the rest) still to come.
+Sequences sequences(const cc1d_gdr_args& a) {
+    return {nullptr, mostly_short(a) ? std::min<int64_t>(kListMax, a.tokens / (kLong + 1)) : a.rows};
+}
+constexpr int64_t kListBytes = 256;  // of a list
+
 template <typename T, typename ST, int VS>
-cudaError_t go(const cc1d_gdr_args& a, const CUtensorMap& q, const CUtensorMap& k, bool out32,
-               cudaStream_t stream) {
+cudaError_t go(const cc1d_gdr_args& a, const Sequences& seqs, const CUtensorMap& q, const CUtensorMap& k,
+               bool out32, cudaStream_t stream) {
     constexpr int smem = Layout<VS, std::is_same<T, f16>::value>::END + 1024;
     const int tiles = a.dv / VS;
-    const int64_t grid = a.rows * a.heads_v * tiles;
+    const int64_t grid = seqs.n * a.heads_v * tiles;
     if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
     CUtensorMap v;
     if (!make_map(&v, a.v, a.tokens, a.heads_v, a.dv, a.v_st, a.v_sh, VS)) return cudaErrorInvalidValue;
@@ -431,11 +448,12 @@ cudaError_t go(const cc1d_gdr_args& a, const CUtensorMap& q, const CUtensorMap& 
     const cudaError_t err = limit.raise(gdr_chunk_kernel<T, ST, VS>, smem);
     if (err != cudaSuccess) return err;
     return launch_dependent(gdr_chunk_kernel<T, ST, VS>, (unsigned)grid, kThreads, smem, stream, a, q, k, v,
-                            tiles, out32, wait_limit_ns());
+                            tiles, out32, seqs, wait_limit_ns());
 }
 
 template <typename T, typename ST>
-cudaError_t pick(const cc1d_gdr_args& a, const CUtensorMap& q, const CUtensorMap& k, cudaStream_t stream) {
+cudaError_t pick(const cc1d_gdr_args& a, const Sequences& seqs, const CUtensorMap& q, const CUtensorMap& k,
+                 cudaStream_t stream) {
     const bool out32 = host_aligned32(a.out) && a.o_st % 16 == 0 && a.o_sh % 16 == 0;
     // Columns per CTA. A chunk's step takes 2.1, 2.9 and 3.7 us with 32, 64 and 128 columns: wide
     // tiles do more per SM, narrow ones finish a chain sooner. Many heads (sequences x heads) take the
@@ -447,15 +465,15 @@ cudaError_t pick(const cc1d_gdr_args& a, const CUtensorMap& q, const CUtensorMap
     // costs a whole chain (48 heads in one sequence 332, 273, 333; 12 heads 160, 220, 281). fp16 has no
     // tile of 64, which would load twice the keys for no more than the narrow one's speed (us with 32,
     // 128: 768 heads 1273, 853; 240 heads 340, 347 and in five sequences 1194, 1099; 192 heads 330, 380;
-    // 144 heads 328, 442).
+    // 144 heads 328, 442). Listed sequences, few as a rule, take the narrowest.
     constexpr bool kF16 = std::is_same<T, f16>::value;
-    const int64_t heads = a.rows * a.heads_v;
+    const int64_t heads = seqs.list != nullptr ? 0 : a.rows * a.heads_v;
     if (a.dv % 128 == 0 && heads * (a.dv / 128) >= (kF16 ? 222 : 296)) return launch_gdr_wide(a, q, k, stream);
     if constexpr (!kF16) {
         if (a.dv % 64 == 0 && heads * (a.dv / 32) > (a.rows >= 4 ? 592 : 148))
-            return go<T, ST, 64>(a, q, k, out32, stream);
+            return go<T, ST, 64>(a, seqs, q, k, out32, stream);
     }
-    return go<T, ST, 32>(a, q, k, out32, stream);
+    return go<T, ST, 32>(a, seqs, q, k, out32, stream);
 }
 
 }  // namespace
@@ -475,10 +493,12 @@ bool make_map(CUtensorMap* map, const void* p, int64_t tokens, int heads, int di
 }
 
 int64_t gdr_chunk_workspace(const cc1d_gdr_args& a) {
-    return images_bytes(a) + (a.dtype == CC1D_F16 ? a.tokens * a.heads_k * 4 * DK * 2 : 0);
+    return images_bytes(a, sequences(a)) + (a.dtype == CC1D_F16 ? a.tokens * a.heads_k * 4 * DK * 2 : 0) +
+           (mostly_short(a) ? kListBytes : 0);
 }
 
 bool gdr_chunk_serves(const cc1d_gdr_args& a) {
+    constexpr int64_t kMixed = 128;
     auto rows_ok = [](const void* p, int64_t s0, int64_t s1, int64_t per) {
         return host_aligned16(p) && s0 % per == 0 && s1 % per == 0;
     };
@@ -487,20 +507,34 @@ bool gdr_chunk_serves(const cc1d_gdr_args& a) {
         return rows_ok(p, st, sh, 8) && st > 0 && sh > 0 && st < (1ll << 38) && sh < (1ll << 38);
     };
     const int64_t sv = a.sdtype == CC1D_F32 ? 4 : 8;
-    // Token by token is faster up to some 10 tokens a sequence (measured, uneven lengths: 6 heads,
-    // one sequence of 12 tokens 17 us against 19, four of 6 on average 21 against 19; 128 sequences
-    // x 48 heads, 8 on average, 492 against 621, 12 on average 696 against 625).
+    // Token by token is faster up to some 12 tokens a sequence where the GPU is full, and up to 16 or 20
+    // with few heads (measured: 48 heads, 128 sequences of 8, 12, 16 tokens 480, 677, 876 us, in chunks 682;
+    // 12 heads, 32 sequences 35, 48, 61, chunks 51; 6 heads, 4 sequences 13, 18, 22, chunks 24). Whether a batch with fewer
+    // on average holds a long sequence all the same is known on the device only: from kMixed tokens on,
+    // which would take 1.2 us each in a row, the device lists those for the chunks, and the rest goes token
+    // by token. 512 sequences of one token and one of 4096, 48 heads: 7243 us token by token, 2749 all in
+    // chunks, 1090 like this; 64 of one and one of 100, 6 heads: 122, 52, 43. Batches without a long
+    // sequence pay for launches that find nothing to do (512 of 8, 48 heads 1872 -> 1930 us; 16 of 9, 6
+    // heads 18 -> 25).
     return (a.dtype == CC1D_BF16 || a.dtype == CC1D_F16) && a.dk == DK && a.dv % 32 == 0 && a.q_sd == 1 && a.k_sd == 1 &&
            a.v_sd == 1 && a.o_sd == 1 && map_ok(a.q, a.q_st, a.q_sh) && map_ok(a.k, a.k_st, a.k_sh) &&
            map_ok(a.v, a.v_st, a.v_sh) && rows_ok(a.out, a.o_st, a.o_sh, 8) &&
            rows_ok(a.states, a.s_slot, a.s_sh, sv) && a.s_sk % sv == 0 &&
-           a.tokens >= 10 * a.rows && have_maps();
+           (!mostly_short(a) || a.tokens >= kMixed) && have_maps();
 }
 
 cudaError_t launch_gdr_chunk(const cc1d_gdr_args& a, cudaStream_t stream) {
     CUtensorMap q, k;
+    Sequences seqs = sequences(a);
+    if (mostly_short(a)) {
+        int32_t* list = reinterpret_cast<int32_t*>(static_cast<char*>(a.workspace) + gdr_chunk_workspace(a) - kListBytes);
+        cudaError_t err = launch_gdr_list(a, seqs, list, stream);
+        if (err == cudaSuccess) err = launch_gdr_recurrent(a, true, stream, list);
+        if (err != cudaSuccess) return err;
+        seqs.list = list;
+    }
     if (a.dtype == CC1D_F16) {
-        void* parts = static_cast<char*>(a.workspace) + images_bytes(a);
+        void* parts = static_cast<char*>(a.workspace) + images_bytes(a, seqs);
         const cudaError_t err = launch_gdr_split(a, parts, stream);
         if (err != cudaSuccess) return err;
         if (!make_map(&k, parts, a.tokens, 4 * a.heads_k, a.dk, 4 * a.heads_k * a.dk, a.dk, 64))
@@ -510,11 +544,11 @@ cudaError_t launch_gdr_chunk(const cc1d_gdr_args& a, cudaStream_t stream) {
                !make_map(&k, a.k, a.tokens, a.heads_k, a.dk, a.k_st, a.k_sh, 64)) {
         return cudaErrorInvalidValue;
     }
-    const cudaError_t err = launch_gdr_prep(a, q, k, stream);
+    const cudaError_t err = launch_gdr_prep(a, seqs, q, k, stream);
     if (err != cudaSuccess) return err;
     if (a.dtype == CC1D_F16)
-        return a.sdtype == CC1D_F32 ? pick<f16, float>(a, q, k, stream) : pick<f16, f16>(a, q, k, stream);
-    return a.sdtype == CC1D_F32 ? pick<bf16, float>(a, q, k, stream) : pick<bf16, bf16>(a, q, k, stream);
+        return a.sdtype == CC1D_F32 ? pick<f16, float>(a, seqs, q, k, stream) : pick<f16, f16>(a, seqs, q, k, stream);
+    return a.sdtype == CC1D_F32 ? pick<bf16, float>(a, seqs, q, k, stream) : pick<bf16, bf16>(a, seqs, q, k, stream);
 }
 
 }  // namespace cc1d

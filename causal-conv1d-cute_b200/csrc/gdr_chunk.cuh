@@ -32,7 +32,16 @@ struct Vectors {
 };
 static_assert(sizeof(Vectors) == kVectorBytes, "");
 
-// Image slots: the chunks of sequence n start at slot floor(first token / 64) + n, which leaves
+// The sequences that run in chunks: all of them, or in a batch of mostly short ones those that the
+// device has listed, list = {count, tokens of the longest sequence left out, indices in order}.
+struct Sequences {
+    const int32_t* list;  // NULL: all
+    int64_t n;            // how many there are at most
+};
+constexpr int kListMax = 32;  // sequences a list holds
+constexpr int kLong = 32;     // they have more tokens than this
+
+// Image slots: the chunks of the n-th of them start at slot floor(first token / 64) + n, which leaves
 // every sequence room for its chunks without a prefix sum over the lengths.
 __device__ __forceinline__ int64_t chunk_base(int64_t first_token, int64_t n) {
     return first_token / C + n;
@@ -149,7 +158,10 @@ cudaError_t launch_gdr_wide(const cc1d_gdr_args& a, const CUtensorMap& q, const 
 // Whether the driver offers tensor maps.
 bool have_maps();
 
-cudaError_t launch_gdr_prep(const cc1d_gdr_args& a, const CUtensorMap& q, const CUtensorMap& k,
+cudaError_t launch_gdr_prep(const cc1d_gdr_args& a, const Sequences& seqs, const CUtensorMap& q,
+                            const CUtensorMap& k, cudaStream_t stream);
+// Lists the sequences that are long enough for chunks, seqs.n at most.
+cudaError_t launch_gdr_list(const cc1d_gdr_args& a, const Sequences& seqs, int32_t* list,
                             cudaStream_t stream);
 // What a CTA that has given up waits for its own copies and products at most, one by one.
 constexpr int64_t kDrainNs = 2000000000;

@@ -156,7 +156,7 @@ __device__ __forceinline__ float bits_value(uint32_t b, int dtype) {
 template <bool kLo>
 __global__ void __launch_bounds__(128, kLo ? 2 : 3)
 gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__ CUtensorMap mapq,
-                const __grid_constant__ CUtensorMap mapk, int64_t wait_ns) {
+                const __grid_constant__ CUtensorMap mapk, Sequences seqs, int64_t wait_ns) {
     extern __shared__ __align__(1024) unsigned char raw[];
     Smem<kLo>& sh = *reinterpret_cast<Smem<kLo>*>(raw + ((1024 - (smem_addr(raw) & 1023)) & 1023));
     const uint32_t kq = smem_addr(sh.kq), tb = kq, pb = kq + 24576;
@@ -169,18 +169,20 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_args a, const __grid_constant__
     // The sequence whose chunk this is.
     if (p == 0) sh.seq = -1;
     __syncthreads();
-    for (int64_t n = p; n < a.rows; n += 128) {
-        const int64_t t0 = a.query_start_loc[n], t1 = a.query_start_loc[n + 1];
+    const int64_t n_seqs = seqs.list != nullptr ? seqs.list[0] : seqs.n;
+    for (int64_t n = p; n < n_seqs; n += 128) {
+        const int64_t at = seqs.list != nullptr ? seqs.list[2 + n] : n;
+        const int64_t t0 = a.query_start_loc[at], t1 = a.query_start_loc[at + 1];
         if (t0 < 0 || t1 <= t0 || t1 > a.tokens) continue;
         const int64_t first = chunk_base(t0, n);
         if (image >= first && image < first + (t1 - t0 + C - 1) / C) sh.seq = (int)n;
     }
     __syncthreads();
-    const int64_t row = sh.seq;
+    const int seq = sh.seq;
     int64_t tok0, slot;
     int ntok;
-    if (row < 0 || !gdr_row(a, true, row, tok0, ntok, slot, false)) return;
-    const int c = (int)(image - chunk_base(tok0, row));
+    if (seq < 0 || !gdr_row(a, true, seqs.list != nullptr ? seqs.list[2 + seq] : seq, tok0, ntok, slot, false)) return;
+    const int c = (int)(image - chunk_base(tok0, seq));
     tok0 += c * C;
     const int left = ntok - c * C;
 
@@ -571,11 +573,59 @@ gdr_split_kernel(const __grid_constant__ cc1d_gdr_args a, uint2* to) {
     }
 }
 
+// Lists at most `most_listed` sequences of more than kLong tokens, in order: those above the smallest of
+// kLong, 2 kLong, 4 kLong, .. tokens that leaves so few. One CTA.
+__global__ void __launch_bounds__(1024)
+gdr_list_kernel(const __grid_constant__ cc1d_gdr_args a, int most_listed, int32_t* list) {
+    __shared__ int above[27], warp_sum[32], most;  // above[k]: sequences of more than kLong 2^k tokens
+    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+    auto length = [&](int64_t n) {
+        int64_t tok0, slot;
+        int ntok;
+        return n < a.rows && gdr_row(a, true, n, tok0, ntok, slot, false) ? ntok : 0;
+    };
+    if (tid < 27) above[tid] = 0;
+    __syncthreads();
+    for (int64_t n = tid; n < a.rows; n += 1024) {
+        const int ntok = length(n);
+        for (int k = 0; k < 26 && ntok > ((int64_t)kLong << k); ++k) atomicAdd(&above[k], 1);
+    }
+    __syncthreads();
+    if (tid == 0) {
+        int k = 0;
+        while (above[k] > most_listed) ++k;  // above[26] is 0
+        list[0] = above[k];
+        list[1] = most = k < 26 ? kLong << k : INT32_MAX;
+    }
+    __syncthreads();
+    int base = 0;
+    for (int64_t at = 0; at < a.rows; at += 1024) {
+        const bool on = length(at + tid) > most;
+        const unsigned mask = __ballot_sync(~0u, on);
+        __syncthreads();
+        if (lane == 0) warp_sum[warp] = __popc(mask);
+        __syncthreads();
+        int before = 0, all = 0;
+        for (int m = 0; m < 32; ++m) {
+            before += m < warp ? warp_sum[m] : 0;
+            all += warp_sum[m];
+        }
+        if (on) list[2 + base + before + __popc(mask & ((1u << lane) - 1u))] = (int32_t)(at + tid);
+        base += all;
+    }
+}
+
 }  // namespace
 
-cudaError_t launch_gdr_prep(const cc1d_gdr_args& a, const CUtensorMap& q, const CUtensorMap& k,
+cudaError_t launch_gdr_list(const cc1d_gdr_args& a, const Sequences& seqs, int32_t* list,
                             cudaStream_t stream) {
-    const int64_t grid = chunk_slots(a.tokens, a.rows) * a.heads_k;
+    gdr_list_kernel<<<1, 1024, 0, stream>>>(a, (int)seqs.n, list);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_gdr_prep(const cc1d_gdr_args& a, const Sequences& seqs, const CUtensorMap& q,
+                            const CUtensorMap& k, cudaStream_t stream) {
+    const int64_t grid = chunk_slots(a.tokens, seqs.n) * a.heads_k;
     if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
     auto go = [&](auto lo) {
         constexpr bool kLo = decltype(lo)::value;
@@ -583,7 +633,7 @@ cudaError_t launch_gdr_prep(const cc1d_gdr_args& a, const CUtensorMap& q, const 
         static SmemLimit limit;
         const cudaError_t err = limit.raise(gdr_prep_kernel<kLo>, smem);
         if (err != cudaSuccess) return err;
-        gdr_prep_kernel<kLo><<<(unsigned)grid, 128, smem, stream>>>(a, q, k, wait_limit_ns());
+        gdr_prep_kernel<kLo><<<(unsigned)grid, 128, smem, stream>>>(a, q, k, seqs, wait_limit_ns());
         return cudaGetLastError();
     };
     return a.dtype == CC1D_F16 ? go(std::true_type()) : go(std::false_type());

@@ -57,7 +57,7 @@ __device__ __forceinline__ void store_n(E* p, bool vec, int valid, const float* 
 template <typename T, typename ST, int NW, int CPL>
 __global__ void __launch_bounds__(32 * NW, NW == 4 ? 6 : 1)
 gdr_recurrent_kernel(const __grid_constant__ cc1d_gdr_args a, bool varlen, bool svec, bool iovec,
-                     int tiles) {
+                     int tiles, const int32_t* list) {
     constexpr int KP = 32 * NW, COLS = 8 * CPL;
     __shared__ __align__(16) float sq[kTokTile][KP], sk[kTokTile][KP];
     __shared__ __align__(16) float part[2][NW][2 * COLS];
@@ -78,6 +78,7 @@ gdr_recurrent_kernel(const __grid_constant__ cc1d_gdr_args a, bool varlen, bool 
     int64_t tok0, slot;
     int ntok;
     if (!gdr_row(a, varlen, row, tok0, ntok, slot, h == 0 && tile == 0 && threadIdx.x == 0)) return;
+    if (list != nullptr && ntok > list[1]) return;
     int64_t islot = -1;
     if (a.inter != nullptr) {
         islot = a.inter_indices != nullptr ? a.inter_indices[row] : slot;
@@ -400,7 +401,7 @@ bool vec_ok(const void* p, int64_t bytes, int64_t n, std::initializer_list<int64
 }
 
 template <typename T, typename ST>
-cudaError_t launch(const cc1d_gdr_args& a, bool varlen, cudaStream_t stream) {
+cudaError_t launch(const cc1d_gdr_args& a, bool varlen, cudaStream_t stream, const int32_t* list) {
     constexpr int CPL = 4;
     const int tiles = (int)ceil_div(a.dv, 8 * CPL);
     const int64_t grid = a.rows * a.heads_v * tiles;
@@ -426,7 +427,7 @@ cudaError_t launch(const cc1d_gdr_args& a, bool varlen, cudaStream_t stream) {
     auto go = [&](auto nw) {
         constexpr int NW = decltype(nw)::value;
         gdr_recurrent_kernel<T, ST, NW, CPL>
-            <<<(unsigned)grid, 32 * NW, 0, stream>>>(a, varlen, svec, iovec, tiles);
+            <<<(unsigned)grid, 32 * NW, 0, stream>>>(a, varlen, svec, iovec, tiles, list);
     };
     if (a.dk <= 32)
         go(std::integral_constant<int, 1>());
@@ -441,11 +442,12 @@ cudaError_t launch(const cc1d_gdr_args& a, bool varlen, cudaStream_t stream) {
 
 }  // namespace
 
-cudaError_t launch_gdr_recurrent(const cc1d_gdr_args& a, bool varlen, cudaStream_t stream) {
+cudaError_t launch_gdr_recurrent(const cc1d_gdr_args& a, bool varlen, cudaStream_t stream,
+                                 const int32_t* list) {
     if (a.sdtype == CC1D_F32) {
-        CC1D_DISPATCH_DTYPE(a.dtype, return launch<T, float>(a, varlen, stream));
+        CC1D_DISPATCH_DTYPE(a.dtype, return launch<T, float>(a, varlen, stream, list));
     } else {
-        CC1D_DISPATCH_DTYPE(a.dtype, return launch<T, T>(a, varlen, stream));
+        CC1D_DISPATCH_DTYPE(a.dtype, return launch<T, T>(a, varlen, stream, list));
     }
     return cudaErrorInvalidValue;
 }

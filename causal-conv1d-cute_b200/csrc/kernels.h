@@ -137,7 +137,9 @@ cudaError_t launch_ring(const RingArgs& a, int width, int dtype, cudaStream_t st
 cudaError_t launch_ring_convert(const RingConvArgs& a, int width, int dtype, cudaStream_t stream);
 cudaError_t launch_varlen(const VarArgs& a, int width, int dtype, cudaStream_t stream);
 cudaError_t launch_unpack(const UnpackArgs& a, int width, int dtype, cudaStream_t stream);
-cudaError_t launch_gdr_recurrent(const cc1d_gdr_args& a, bool varlen, cudaStream_t stream);
+// list: NULL, or a list (gdr_chunk.cuh) of sequences that are left out.
+cudaError_t launch_gdr_recurrent(const cc1d_gdr_args& a, bool varlen, cudaStream_t stream,
+                                 const int32_t* list = nullptr);
 // Packed prefill chunk by chunk on the tensor cores, where it serves the types and layout.
 bool gdr_chunk_serves(const cc1d_gdr_args& a);
 int64_t gdr_chunk_workspace(const cc1d_gdr_args& a);

@@ -259,7 +259,7 @@ typedef struct {
 
 /*
  * Bytes of workspace (128-byte aligned) with which cc1d_gdr_varlen runs chunk by chunk on the
- * tensor cores; 0 where it does not (other types or layouts, short sequences). It depends on the
+ * tensor cores; 0 where it does not (other types or layouts, few tokens). It depends on the
  * sizes, strides, pointers' alignment and types of args alone. With less, or NULL, the call runs token
  * by token. The workspace holds nothing between calls.
  */

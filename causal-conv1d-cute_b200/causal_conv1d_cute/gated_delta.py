@@ -67,9 +67,8 @@ def gated_delta_rule_reason(q, k, v, g, beta, states=None, A_log=None, dt_bias=N
         return f"dtypes {q.dtype}, {k.dtype}, {v.dtype} are not one of bf16, fp16 or fp32"
     if g.dtype not in _DTYPES or beta.dtype not in _DTYPES:
         return f"gate dtypes {g.dtype}, {beta.dtype} are not bf16, fp16 or fp32"
-    if A_log is not None and (A_log.dtype not in _DTYPES or dt_bias.dtype != A_log.dtype
-                              or not A_log.is_contiguous() or not dt_bias.is_contiguous()):
-        return "A_log and dt_bias must share one dtype of bf16, fp16, fp32 and be contiguous"
+    if A_log is not None and (A_log.dtype not in _DTYPES or dt_bias.dtype not in _DTYPES):
+        return f"A_log and dt_bias dtypes {A_log.dtype}, {dt_bias.dtype} are not bf16, fp16 or fp32"
     if q.shape[-1] > 256:
         return f"a key head dim of {q.shape[-1]} is above 256"
     if states is not None:
@@ -78,6 +77,15 @@ def gated_delta_rule_reason(q, k, v, g, beta, states=None, A_log=None, dt_bias=N
         if states.stride(-1) != 1:
             return f"state strides {states.stride()} (the last axis must be contiguous)"
     return None
+
+
+def _params(A_log, dt_bias):
+    """The gates' parameters contiguous and of one dtype, as the kernels read them (fp32 holds all)."""
+    if A_log is None:
+        return None, None
+    if A_log.dtype != dt_bias.dtype:
+        A_log, dt_bias = A_log.float(), dt_bias.float()
+    return A_log.contiguous(), dt_bias.contiguous()
 
 
 def _index(index, device):
@@ -114,7 +122,8 @@ def gated_delta_rule_varlen_fn(
         has_initial_state: optional (batch,) bool/uint8: start from the cached state.
         states: optional (slots, heads_v, dk, dv) cache of fp32 or the input dtype, updated in
             place with the final state of each sequence (sequences of zero tokens leave theirs).
-        A_log, dt_bias: optional (heads_v,) parameters of raw gates.
+        A_log, dt_bias: optional (heads_v,) parameters of raw gates (where their dtypes differ, or for
+            strided views, the call makes copies).
         scale: output scale (default dk ** -0.5).
         qk_l2norm: scale q and k to unit length first (eps 1e-6 under the root).
         pad_slot_id: cache_indices value marking sequences to skip (their outputs are undefined
@@ -162,7 +171,7 @@ def gated_delta_rule_varlen_fn(
     hinit = _flags(has_initial_state, dev) if states is not None else None
     if hinit is not None and not hinit.is_contiguous():
         hinit = hinit.contiguous()
-    _ops.gdr_varlen(q, k, v, g, beta, A_log, dt_bias, out, states, qsl, idx, hinit,
+    _ops.gdr_varlen(q, k, v, g, beta, *_params(A_log, dt_bias), out, states, qsl, idx, hinit,
                     q.shape[-1] ** -0.5 if scale is None else scale, qk_l2norm, pad_slot_id)
     return out
 
@@ -224,7 +233,7 @@ def gated_delta_rule_fn(
         hinit = None
         if initial_states is not None:
             hinit = torch.ones(B, dtype=torch.uint8, device=q.device)
-        _ops.gdr_varlen(*(t.flatten(0, 1) for t in (q, k, v, g, beta)), A_log, dt_bias,
+        _ops.gdr_varlen(*(t.flatten(0, 1) for t in (q, k, v, g, beta)), *_params(A_log, dt_bias),
                         out.flatten(0, 1), final, qsl, None, hinit,
                         dk**-0.5 if scale is None else scale, qk_l2norm, PAD_SLOT_ID)
     return (out, final) if return_final_states else out
@@ -294,7 +303,7 @@ def gated_delta_rule_update(
     dev = q.device
     idx = _index(state_indices, dev)
     iidx = _index(intermediate_state_indices, dev) if inter is not None else None
-    _ops.gdr_update(q, k, v, g, beta, A_log, dt_bias, out, states, idx, inter, iidx,
+    _ops.gdr_update(q, k, v, g, beta, *_params(A_log, dt_bias), out, states, idx, inter, iidx,
                     q.shape[-1] ** -0.5 if scale is None else scale, qk_l2norm, update_states,
                     pad_slot_id)
     return out

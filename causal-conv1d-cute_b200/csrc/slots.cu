@@ -221,7 +221,7 @@ cudaError_t launch_slots_compact(const cc1d_slot_cache* table, int ncaches, cons
                                  cudaStream_t stream) {
     slots_plan_kernel<<<1, 1024, 0, stream>>>(live, (int)nslots, remap, count, moves);
     cudaError_t err = cudaGetLastError();
-    if (err != cudaSuccess || ncaches == 0) return err;
+    if (err != cudaSuccess || ncaches == 0 || nslots == 0) return err;
     SlotTable t;
     const int64_t tiles = build_table(table, ncaches, t);
     if (tiles == 0) return cudaSuccess;

@@ -307,7 +307,7 @@ cc1d_status_t cc1d_rms_norm_gated(const cc1d_norm_args* args, void* stream);
  * make slots 0..m-1 the live ones. remap[s] is the new place of slot s (-1: not live), *count is
  * m. moves is a workspace of 2*nslots + 1 int32.
  *
- * At most CC1D_MAX_CACHES caches a call, nslots up to 2^31 - 1.
+ * At most CC1D_MAX_CACHES caches a call; up to 2^31 - 1 slots (compaction: 2^30 - 2).
  */
 #define CC1D_MAX_CACHES 64
 typedef struct {

@@ -1,11 +1,13 @@
 """Groups of state caches beside one another in memory, and groups without slots."""
 
+import ctypes
 import itertools
 
 import pytest
 import torch
 
 import causal_conv1d_cute as C
+from causal_conv1d_cute import _lib
 from causal_conv1d_cute.slots import _apart
 from test_slots import apply, int32, same
 
@@ -125,3 +127,15 @@ def test_cache_with_memory_that_does_not_fit():
     caches[0].data, caches[1].data = torch.ones(6, 8, device="cuda"), torch.ones(6, 3, device="cuda")
     group.copy(int32([-1]), int32([5]))
     assert len(group) == 6 and [c.sum().item() for c in caches] == [40, 15]
+
+
+@pytest.mark.gpu
+def test_compaction_of_no_slots_through_c():
+    """Caches whose slots have bytes, but of which there are none: the count is 0 and nothing moves."""
+    memory = torch.arange(64, dtype=torch.uint8, device="cuda")
+    work = torch.full((2,), 7, dtype=torch.int32, device="cuda")
+    table = (ctypes.c_int64 * 5)(memory.data_ptr(), memory.data_ptr(), 16, 16, 16)
+    lib = _lib.load()
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.cc1d_slots_compact(table, 1, None, 0, None, work[:1].data_ptr(), work[1:].data_ptr(), stream) == 0
+    assert work.tolist() == [0, 0] and memory.tolist() == list(range(64))

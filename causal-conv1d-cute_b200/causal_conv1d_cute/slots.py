@@ -35,6 +35,13 @@ def _apart(slots, spans):
     return True
 
 
+def _slot_list(index, device):
+    """Slots as contiguous int32 on device; wider ones outside it stay outside every cache."""
+    if index.dtype == torch.int64:
+        index = index.clamp(-(2**31), 2**31 - 1)
+    return _int32(index, device).contiguous()
+
+
 class StateSlots:
     """A group of caches whose first axis is the slot.
 
@@ -143,9 +150,7 @@ class StateSlots:
             ]:
                 raise ValueError("source caches differ in slot shape or dtype")
             self._check_other(source)
-        src, dst = _int32(src_indices, self.device), _int32(dst_indices, self.device)
-        src = src if src.is_contiguous() else src.contiguous()
-        dst = dst if dst.is_contiguous() else dst.contiguous()
+        src, dst = _slot_list(src_indices, self.device), _slot_list(dst_indices, self.device)
         for at, n, _ in self._table(source):
             _ops.slots_copy(self.caches, source.caches if source is not self else [], at, n, src, dst,
                             source.slots, self.slots, pad_slot_id)

@@ -139,3 +139,19 @@ def test_compaction_of_no_slots_through_c():
     stream = torch.cuda.current_stream().cuda_stream
     assert lib.cc1d_slots_compact(table, 1, None, 0, None, work[:1].data_ptr(), work[1:].data_ptr(), stream) == 0
     assert work.tolist() == [0, 0] and memory.tolist() == list(range(64))
+
+
+@pytest.mark.gpu
+def test_wide_indices_outside_int32(request):
+    """Their low 32 bits name slots; they are skipped and reported all the same."""
+    request.node._expect_status = True
+    cache = torch.arange(6.0, device="cuda").reshape(6, 1).repeat(1, 4)
+    want = cache.clone()
+    wide = lambda *x: torch.tensor(x, device="cuda")  # noqa: E731
+    group = C.StateSlots([cache])
+    group.copy(wide(2**32, 1, 2**32 + 3), wide(2, 2**32 + 3, 4))
+    assert C.device_status() == _lib.DEV_BAD_SLOT and torch.equal(cache, want)
+    group.copy(wide(-(2**32) - 1, 5, -1), wide(1, -(2**32) - 1, 2**32 - 1))
+    assert C.device_status() == _lib.DEV_BAD_SLOT and torch.equal(cache, want)
+    group.copy(wide(1, -1), wide(0, 5))
+    assert C.device_status() == 0 and cache[:, 0].tolist() == [1, 1, 2, 3, 4, 0]

@@ -21,10 +21,7 @@ __device__ __forceinline__ uint32_t smem_addr(const void* p) {
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// The same, announcing bytes that bulk copies will bring.
+// One arrival, announcing bytes that bulk copies will bring.
 __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
                  : "memory");
@@ -141,16 +138,6 @@ __device__ __forceinline__ void tmem_wait_ld() {
 __device__ __forceinline__ void tmem_ready(float2* f) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) asm volatile("" : "+f"(f[i].x), "+f"(f[i].y));
-}
-// The reverse; tmem_wait_st() before another load of the same columns.
-__device__ __forceinline__ void tmem_st16(uint32_t t0, const float2* f) {
-    __syncwarp();
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {" CC1D_R0 "};" ::"f"(f[0].x), "f"(f[0].y),
-        "f"(f[1].x), "f"(f[1].y), "f"(f[2].x), "f"(f[2].y), "f"(f[3].x), "f"(f[3].y), "f"(f[4].x),
-        "f"(f[4].y), "f"(f[5].x), "f"(f[5].y), "f"(f[6].x), "f"(f[6].y), "f"(f[7].x), "f"(f[7].y),
-        "r"(t0)
-        : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");

@@ -18,9 +18,9 @@
 // which hold all 24 bits; of the products of two split operands those of 2^-27 are left out, and
 // small products are added among themselves before they meet the large ones, because the tensor core
 // cuts its sums to fp32 after every step (summed the other way the errors are two to five times as
-// large). fp32 final states come out within 4e-7 of the definition (2-norm of a head; all together 1.3e-7,
-// as token by token), keys that are all the same among them. Two parts, which need 0.6 of the products,
-// left 2e-6 to 9e-6, and 7e-5 where all keys of a sequence are the same and u cancels over its tokens.
+// large). fp32 final states come out within 2.5e-7 of the definition (2-norm) where keys are random, and
+// within 7e-7 where the keys of a sequence repeat and u cancels over its tokens; fp32 arithmetic token by
+// token leaves up to 4e-7 and 9e-7. Two parts, which need 0.6 of the products, left 2e-6 to 9e-6, and 7e-5.
 // The state itself is carried in fp32 from chunk to chunk.
 //
 // Split of the work. Chunks of one sequence form a chain; heads, sequences and the columns of the
@@ -32,7 +32,7 @@
 // sequence and VS state columns; all its warps turn a product into the operand of the next together.
 // K, Q, T and G come by TMA and bulk copies a chunk or two ahead.
 //
-// Bound. The latency of the chain: 2.1 us a chunk at VS = 32 (8192 tokens x 12 heads 270 us), of which
+// Bound. The latency of the chain: 2.2 us a chunk at VS = 32 (8192 tokens x 12 heads 285 us), of which
 // the products take half and the rest is TMEM loads, splitting, barriers. Tiles of 128 columns, for
 // many heads, have a kernel of their own (gdr_wide.cu). Measured with operands in two parts: 2950
 // cycles a chunk at VS = 32; in this form 6800 with 128 columns, two independent chains of 64 in one CTA
@@ -455,7 +455,7 @@ template <typename T, typename ST>
 cudaError_t pick(const cc1d_gdr_args& a, const Sequences& seqs, const CUtensorMap& q, const CUtensorMap& k,
                  cudaStream_t stream) {
     const bool out32 = host_aligned32(a.out) && a.o_st % 16 == 0 && a.o_sh % 16 == 0;
-    // Columns per CTA. A chunk's step takes 2.1, 2.9 and 3.7 us with 32, 64 and 128 columns: wide
+    // Columns per CTA. A chunk's step takes 2.2, 3.0 and 4.0 us with 32, 64 and 128 columns: wide
     // tiles do more per SM, narrow ones finish a chain sooner. Many heads (sequences x heads) take the
     // widest (bf16, uneven lengths, us with 32, 64, 128 columns: 768 heads, 16384 tokens 1006, 826, 641;
     // 336 heads 290, 236, 224; 288 heads 281, 232, 240; 240 heads 274, 226, 274), few the narrowest

@@ -285,11 +285,12 @@ def _gdr_update_impl(q, k, v, g, beta, a_log, dt_bias, out, states, idx, inter, 
 
 
 def _gdr_varlen_impl(q, k, v, g, beta, a_log, dt_bias, out, states, qsl, idx, hinit, scale,
-                     l2norm, pad):
-    """Gated delta rule over packed sequences (cc1d_gdr_varlen): (tokens, heads, dim)."""
+                     l2norm, pad, longest=0):
+    """Gated delta rule over packed sequences (cc1d_gdr_varlen): (tokens, heads, dim). longest: tokens of
+    the longest sequence where the caller knows them."""
     lib = load()
 
-    rest = (None, idx, None, qsl, hinit, qsl.numel() - 1, q.shape[0], 0, scale, l2norm, True, pad)
+    rest = (None, idx, None, qsl, hinit, qsl.numel() - 1, q.shape[0], longest, scale, l2norm, True, pad)
     args, need = _gdr_args(q, k, v, g, beta, a_log, dt_bias, out, states, *rest), ctypes.c_int64()
     check(lib.cc1d_gdr_workspace(args, ctypes.byref(need)))
     if not need.value:
@@ -380,7 +381,7 @@ _SCHEMAS = {
     "gdr_varlen": (
         "gdr_varlen(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor? a_log, "
         "Tensor? dt_bias, Tensor(a!) out, Tensor(b!)? states, Tensor qsl, Tensor? idx, "
-        "Tensor? hinit, float scale, bool l2norm, int pad) -> ()"
+        "Tensor? hinit, float scale, bool l2norm, int pad, int longest=0) -> ()"
     ),
     "rms_norm_gated": (
         "rms_norm_gated(Tensor x, Tensor? z, Tensor weight, float eps, Tensor(a!) out) -> ()"

@@ -235,7 +235,7 @@ def gated_delta_rule_fn(
             hinit = torch.ones(B, dtype=torch.uint8, device=q.device)
         _ops.gdr_varlen(*(t.flatten(0, 1) for t in (q, k, v, g, beta)), *_params(A_log, dt_bias),
                         out.flatten(0, 1), final, qsl, None, hinit,
-                        dk**-0.5 if scale is None else scale, qk_l2norm, PAD_SLOT_ID)
+                        dk**-0.5 if scale is None else scale, qk_l2norm, PAD_SLOT_ID, L)
     return (out, final) if return_final_states else out
 
 

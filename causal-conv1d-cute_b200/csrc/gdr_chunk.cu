@@ -520,7 +520,7 @@ bool gdr_chunk_serves(const cc1d_gdr_args& a) {
            a.v_sd == 1 && a.o_sd == 1 && map_ok(a.q, a.q_st, a.q_sh) && map_ok(a.k, a.k_st, a.k_sh) &&
            map_ok(a.v, a.v_st, a.v_sh) && rows_ok(a.out, a.o_st, a.o_sh, 8) &&
            rows_ok(a.states, a.s_slot, a.s_sh, sv) && a.s_sk % sv == 0 &&
-           (!mostly_short(a) || a.tokens >= kMixed) && have_maps();
+           (!mostly_short(a) || (a.tokens >= kMixed && (a.steps < 1 || a.steps > kLong))) && have_maps();
 }
 
 cudaError_t launch_gdr_chunk(const cc1d_gdr_args& a, cudaStream_t stream) {

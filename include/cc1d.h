@@ -236,7 +236,8 @@ cc1d_status_t cc1d_copy(void* dst, const void* src, int64_t bytes, void* stream)
  *     [query_start_loc[n], query_start_loc[n+1]) of `tokens` (the *_sb are not used). It starts
  *     from states[indices[n]] if has_initial_state[n] != 0 and from zeros otherwise, and that slot
  *     receives its final state; sequences of zero tokens and of slot `pad` leave the cache
- *     untouched (those of slot `pad` leave their outputs unwritten). states may be NULL.
+ *     untouched (those of slot `pad` leave their outputs unwritten). states may be NULL. steps may say
+ *     how many tokens the longest sequence has (0: not known); results do not depend on it.
  * states is (nslots, heads_v, dk, dv) of sdtype with unit stride along dv. Live slots must be
  * distinct. dk is 1..256; sdtype is fp32 or `dtype`.
  */

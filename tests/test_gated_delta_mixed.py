@@ -42,13 +42,13 @@ def test_mixed_without_cache_and_with_a_pad(states, pad):
     varlen_case([2] * 40 + [33, 130] + [1] * 20, states=states, pad=pad)
 
 
-def block(rows, tokens, hk=16, hv=48):
+def block(rows, tokens, hk=16, hv=48, longest=0):
     """A packed argument block of bf16 tensors, for questions that touch no memory."""
     d, at = 128, 1 << 20
     heads = (0, (2 * hk + hv) * d, d, 1)
     return _lib.GDR_ARGS.pack(at, at, at, at, at, 0, 0, at, at, 0, 0, 0, at, 0, 0, 0, *heads, *heads, *heads, 0, hv * d, d, 1,
                               0, hv, 1, 0, hv, 1, hv * d * d, d * d, d, 0, 0, 0, 0, rows, tokens, rows, 0, 0,
-                              0, hk, hv, d, d, 0, 0, 0, 2, 2, 1, 1, -1, 1.0)
+                              longest, hk, hv, d, d, 0, 0, 0, 2, 2, 1, 1, -1, 1.0)
 
 
 def workspace(*args, **kw):
@@ -66,6 +66,27 @@ def test_workspace_of_mixed_batches():
     assert (2 + 4) * chunk > workspace(20, 130) >= (2 + 3) * chunk
     assert workspace(64, 127) == 0 and workspace(10, 119) == 0
     assert workspace(10, 120) >= (1 + 10) * chunk
+
+
+@pytest.mark.gpu
+def test_no_long_ones_are_looked_for_where_there_are_none():
+    assert workspace(64, 512) > 0 and workspace(64, 512, longest=33) == workspace(64, 512)
+    assert workspace(64, 512, longest=8) == 0 and workspace(64, 512, longest=32) == 0
+    assert workspace(4, 512, longest=128) == workspace(4, 512) > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,L", [(20, 7), (13, 11), (12, 40)])
+def test_dense_batches_of_short_sequences(B, L):
+    """The same bits as the packed call, which does not know the lengths."""
+    q, k, v, g, b, A, dt = (gpu(t) for t in make(B * L, 1, 2, 128, 128, BF))
+    args = dict(A_log=A, dt_bias=dt, qk_l2norm=True)
+    st = torch.randn(B, 2, 128, 128, device="cuda")
+    out, fin = C.gated_delta_rule_fn(*(t.unflatten(0, (B, L)) for t in (q, k, v, g, b)), st, True, **args)
+    start = torch.arange(0, B * L + 1, L, dtype=torch.int32, device="cuda")
+    hinit = torch.ones(B, dtype=torch.bool, device="cuda")
+    packed = C.gated_delta_rule_varlen_fn(q, k, v, g, b, start, None, hinit, st, **args)
+    assert torch.equal(out.flatten(0, 1), packed) and torch.equal(fin, st)
 
 
 @pytest.mark.gpu

@@ -142,6 +142,8 @@ class StateSlots:
             raise ValueError(
                 f"index lists of shapes {tuple(src_indices.shape)} and {tuple(dst_indices.shape)}"
             )
+        if not -(2**31) <= pad_slot_id < 2**31:
+            raise ValueError(f"pad_slot_id {pad_slot_id} is not a 32-bit index")
         if source is not self:
             if source.device != self.device:
                 _unsupported("source caches are on another device")

@@ -155,3 +155,15 @@ def test_wide_indices_outside_int32(request):
     assert C.device_status() == _lib.DEV_BAD_SLOT and torch.equal(cache, want)
     group.copy(wide(1, -1), wide(0, 5))
     assert C.device_status() == 0 and cache[:, 0].tolist() == [1, 1, 2, 3, 4, 0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pad", [2**32, 2**31, -(2**31) - 1, -(2**63)])
+def test_pad_outside_int32(pad):
+    """Its low 32 bits name a slot, which would then be cleared or skipped."""
+    cache = torch.ones(3, 4, device="cuda")
+    with pytest.raises(ValueError, match="pad_slot_id"):
+        C.StateSlots([cache]).copy(int32([0]), int32([1]), pad_slot_id=pad)
+    assert (cache == 1).all()
+    C.StateSlots([cache]).copy(int32([2**31 - 1]), int32([1]), pad_slot_id=2**31 - 1)
+    assert cache.sum(1).tolist() == [4, 0, 4]
